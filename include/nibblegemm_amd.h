@@ -50,7 +50,7 @@
 extern "C" {
 #endif
 
-#define NIBBLE_ABI_VERSION 15
+#define NIBBLE_ABI_VERSION 16
 
 #if defined(__GNUC__) || defined(__clang__)
 #define NIBBLE_API __attribute__((visibility("default")))
@@ -424,6 +424,36 @@ NIBBLE_API int nibble_chain_destroy(void* chain);
  * want more strips than this gives).  A weight converted at either width
  * serves both.  Pure host computation. */
 NIBBLE_API int64_t nibble_chain_strip_cols(int64_t K, int64_t N, int64_t group_size, int64_t M);
+
+/*
+ * Microscaled 4-bit floats (OCP MXFP4).  No counterpart in the reference.  A
+ * matrix [rows, K], K a multiple of 32, is
+ *   codes   uint8 [rows, K / 2], two codes a byte along K, the even k low:
+ *           sign | exponent (2 bits) | mantissa (1 bit), the values 0, 0.5, 1,
+ *           1.5, 2, 3, 4, 6; 16-byte aligned;
+ *   scales  uint8 [ceil(K / 128), rows, 4], the power of two of each block of
+ *           32 k, biased by 127 (255: the block is NaN), four neighbouring
+ *           blocks to a word, zero behind the last; 4-byte aligned.
+ * ceil(K / 128) * rows * 4 must be below 2^31, K at most 2^24.
+ * dtype: 0 fp16, 1 bf16, 2 fp32.
+ */
+
+/* Quantises X [rows, K]: element (r, k) at r row_stride + k k_stride elements,
+ * one of the strides 1.  A block's power of two is that of its largest
+ * magnitude less 2 (at least 2^-127), its codes the nearest of v / 2^e, ties
+ * to even, at most 6; a block with an infinity or a NaN becomes NaN. */
+NIBBLE_API int nibble_mx_quantize(const void* X, int64_t rows, int64_t K, int64_t row_stride,
+                                  int64_t k_stride, int64_t dtype, void* codes, void* scales,
+                                  void* stream);
+/* The values of a matrix, out [rows, K], 16-byte aligned: exact in bf16 and
+ * fp32, rounded once in fp16. */
+NIBBLE_API int nibble_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K,
+                                    int64_t dtype, void* out, void* stream);
+/* Y [M, N] = x w^T of x [M, K] and w [N, K]: summed in fp32, rounded once to
+ * dtype.  Y is 16-byte aligned; M at most 65535 * 64. */
+NIBBLE_API int nibble_mx_matmul(const void* x_codes, const void* x_scales, int64_t M,
+                                const void* w_codes, const void* w_scales, int64_t N, int64_t K,
+                                int64_t dtype, void* Y, void* stream);
 
 /*
  * Measurement: a streaming read of `bytes` (a positive multiple of 16) from

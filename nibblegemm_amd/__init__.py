@@ -14,6 +14,7 @@ as stubs that raise ``NotImplementedError``, so ``from nibblegemm_amd import
 """
 
 from . import convert
+from .mx import MXMatrix, dequantize_mx, matmul_mx, mx_from_blocks, quantize_mx
 from .ops import (DECODE_MAX_M, QuantLinear, dequant, extension, gemm, gemv, matmul, matmul_bias,
                   matmul_swiglu, rmsnorm_matmul, strip_major_cols, to_strip_major)
 from .quant import (
@@ -33,6 +34,7 @@ from .quant import (
 __all__ = [
     "DECODE_MAX_M",
     "HessianAccumulator",
+    "MXMatrix",
     "QuantLinear",
     "QuantizedWeight",
     "concat_columns",
@@ -40,6 +42,7 @@ __all__ = [
     "gptq_quantize",
     "dequant",
     "dequantize",
+    "dequantize_mx",
     "extension",
     "find_decoder_blocks",
     "from_strip_major",
@@ -48,11 +51,14 @@ __all__ = [
     "interleave_swiglu",
     "matmul",
     "matmul_bias",
+    "matmul_mx",
     "matmul_swiglu",
+    "mx_from_blocks",
     "pack_nibbles",
     "quantize",
     "quantize_device",
     "quantize_model_gptq",
+    "quantize_mx",
     "reference_matmul",
     "rmsnorm_matmul",
     "StripMajorWeight",

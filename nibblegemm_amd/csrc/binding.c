@@ -306,6 +306,46 @@ static PyObject* py_quantize(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(nibble_quantize_rtn(W, K, N, dt, g, Wq, S, stream));
 }
 
+/* mx_quantize(X, rows, K, row_stride, k_stride, dtype, codes, scales, stream) */
+static PyObject* py_mx_quantize(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (!nargs_is(n, 9, "mx_quantize")) return NULL;
+  void *X, *codes, *scales, *stream;
+  long long rows, K, rs, ks, dt;
+  if (!take_ptr(a[0], &X) || !take_i64(a[1], &rows) || !take_i64(a[2], &K) ||
+      !take_i64(a[3], &rs) || !take_i64(a[4], &ks) || !take_i64(a[5], &dt) ||
+      !take_ptr(a[6], &codes) || !take_ptr(a[7], &scales) || !take_ptr(a[8], &stream))
+    return NULL;
+  return PyLong_FromLong(nibble_mx_quantize(X, rows, K, rs, ks, dt, codes, scales, stream));
+}
+
+/* mx_dequantize(codes, scales, rows, K, dtype, out, stream) */
+static PyObject* py_mx_dequantize(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (!nargs_is(n, 7, "mx_dequantize")) return NULL;
+  void *codes, *scales, *out, *stream;
+  long long rows, K, dt;
+  if (!take_ptr(a[0], &codes) || !take_ptr(a[1], &scales) || !take_i64(a[2], &rows) ||
+      !take_i64(a[3], &K) || !take_i64(a[4], &dt) || !take_ptr(a[5], &out) ||
+      !take_ptr(a[6], &stream))
+    return NULL;
+  return PyLong_FromLong(nibble_mx_dequantize(codes, scales, rows, K, dt, out, stream));
+}
+
+/* mx_matmul(x_codes, x_scales, M, w_codes, w_scales, N, K, dtype, Y, stream) */
+static PyObject* py_mx_matmul(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (!nargs_is(n, 10, "mx_matmul")) return NULL;
+  void *xc, *xs, *wc, *ws, *Y, *stream;
+  long long M, N, K, dt;
+  if (!take_ptr(a[0], &xc) || !take_ptr(a[1], &xs) || !take_i64(a[2], &M) ||
+      !take_ptr(a[3], &wc) || !take_ptr(a[4], &ws) || !take_i64(a[5], &N) ||
+      !take_i64(a[6], &K) || !take_i64(a[7], &dt) || !take_ptr(a[8], &Y) ||
+      !take_ptr(a[9], &stream))
+    return NULL;
+  return PyLong_FromLong(nibble_mx_matmul(xc, xs, M, wc, ws, N, K, dt, Y, stream));
+}
+
 /* gemm_strip_major(X, xr, xc, Wt, St, K, N, g, sw, version, Y, ws, ws_bytes, stream) */
 static PyObject* py_sm_gemm(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   (void)self;
@@ -447,6 +487,11 @@ static PyMethodDef kMethods[] = {
      "nibble_gemm_w4a16_fused"},
     {"quantize_rtn", (PyCFunction)(void (*)(void))py_quantize, METH_FASTCALL,
      "nibble_quantize_rtn"},
+    {"mx_quantize", (PyCFunction)(void (*)(void))py_mx_quantize, METH_FASTCALL,
+     "nibble_mx_quantize"},
+    {"mx_dequantize", (PyCFunction)(void (*)(void))py_mx_dequantize, METH_FASTCALL,
+     "nibble_mx_dequantize"},
+    {"mx_matmul", (PyCFunction)(void (*)(void))py_mx_matmul, METH_FASTCALL, "nibble_mx_matmul"},
     {"gemm_strip_major", (PyCFunction)(void (*)(void))py_sm_gemm, METH_FASTCALL,
      "nibble_gemm_w4a16_strip_major"},
     {"dequant_strip_major", (PyCFunction)(void (*)(void))py_sm_dequant, METH_FASTCALL,

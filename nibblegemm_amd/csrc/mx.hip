@@ -1,0 +1,505 @@
+// Microscaled 4-bit floats (OCP MXFP4): quantisation, its inverse, and the
+// product of two such matrices on the scaled MFMA of gfx950.
+//
+// A matrix [rows, K] (K a multiple of 32) is held as
+//   codes   uint8 [rows, K / 2]            two a byte along K, the even k low;
+//   scales  uint8 [ceil(K / 128), rows, 4]  one power of two (biased by 127) per
+//                                          block of 32 k, four blocks a word;
+//                                          zero behind the last block.
+// A code is sign | exponent (2) | mantissa (1): 0, 0.5, 1, 1.5, 2, 3, 4, 6.
+// The words of one k group lie side by side over the rows because that is how
+// the matrix cores take them: a lane holds one block (16 bytes of codes) of one
+// row, and the word of scales its four blocks need arrives with one load of
+// adjacent lanes' words.
+#include <algorithm>
+
+#include "nibble_common.h"
+#include "nibble_decode.h"
+#include "nibble_reduce.h"
+
+namespace nibble {
+namespace {
+
+constexpr int kMxF16 = 0, kMxBF16 = 1, kMxF32 = 2;
+constexpr int kMxBlock = 32;   // k of one scale
+constexpr int kMxGroup = 128;  // k of one word of scales
+
+typedef int i8_t __attribute__((ext_vector_type(8)));
+typedef unsigned short us8_t __attribute__((ext_vector_type(8)));
+
+template <int DT>
+struct MxElem {
+  using type = unsigned short;
+  static __device__ __forceinline__ float get(unsigned short v) {
+    return DT == kMxF16 ? static_cast<float>(__builtin_bit_cast(_Float16, v))
+                        : __builtin_bit_cast(float, static_cast<uint32_t>(v) << 16);
+  }
+  static __device__ __forceinline__ void load8(const type* p, float (&f)[8]) {
+    const us8_t v = __builtin_nontemporal_load(reinterpret_cast<const us8_t*>(p));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = get(v[i]);
+  }
+};
+template <>
+struct MxElem<kMxF32> {
+  using type = float;
+  static __device__ __forceinline__ float get(float v) { return v; }
+  static __device__ __forceinline__ void load8(const type* p, float (&f)[8]) {
+    const f4_t a = __builtin_nontemporal_load(reinterpret_cast<const f4_t*>(p));
+    const f4_t b = __builtin_nontemporal_load(reinterpret_cast<const f4_t*>(p) + 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = a[i], f[4 + i] = b[i];
+  }
+};
+
+// Biased exponent of a block whose largest magnitude has these bits:
+// floor(log2) - 2 (the largest code, 6, has exponent 2), never below -127.  A
+// block with an infinity or a NaN gets 255 and reads as NaN.
+__device__ __forceinline__ uint32_t mx_scale(uint32_t top) {
+  const uint32_t e = top >> 23;
+  return e == 255u ? 255u : e > 2u ? e - 2u : 0u;
+}
+// The power of two as a float (2^-127 is subnormal).
+__device__ __forceinline__ float mx_power(uint32_t e) {
+  return __builtin_bit_cast(float, e == 0u ? 0x00400000u : e << 23);
+}
+__device__ __forceinline__ uint32_t mag_bits(float f) {
+  return __builtin_bit_cast(uint32_t, f) & 0x7fffffffu;
+}
+
+// Codes of eight values over their block's power of two, rounded half to even
+// and capped at 6 by the conversion.  In a block that reads as NaN they are 0.
+__device__ __forceinline__ uint32_t mx_codes8(const float (&f)[8], uint32_t e) {
+  const float p = mx_power(e);
+  uint32_t c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[0], f[1], p, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[2], f[3], p, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[4], f[5], p, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, f[6], f[7], p, 3);
+  return e == 255u ? 0u : c;
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false));
+}
+
+// Rows whose k are adjacent in memory.  A workgroup takes 32 rows of 512 k;
+// wave w the k group w of them, 16 lanes a row: lane j holds k 8j .. 8j + 7,
+// four lanes a block.  The largest magnitude meets in the four lanes (DPP),
+// the four blocks' exponents in the row's first lane, which writes the word.
+constexpr int kMxRows = 32;
+constexpr int kMxPasses = kMxRows / 4;
+
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(const typename MxElem<DT>::type* X,
+                                                          int64_t ld, uint32_t* codes,
+                                                          uint32_t* scales, int64_t rows, int K,
+                                                          int col_tiles) {
+  using E = MxElem<DT>;
+  const int lane = threadIdx.x & 63;
+  const int64_t tile = blockIdx.x / col_tiles;
+  const int group = static_cast<int>(blockIdx.x % col_tiles) * 4 + (threadIdx.x >> 6);
+  const int j = lane & 15;
+  const int k = group * kMxGroup + 8 * j;
+  const int64_t row0 = tile * kMxRows + (lane >> 4);
+  if (group * kMxGroup >= K) return;
+  float f[kMxPasses][8];
+#pragma unroll
+  for (int p = 0; p < kMxPasses; ++p) {
+    const int64_t row = row0 + 4 * p;
+    const bool in = row < rows && k < K;
+    const typename E::type* x = X + row * ld + k;
+    if (VEC) {
+      if (in) {
+        E::load8(x, f[p]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[p][i] = 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[p][i] = in ? E::get(x[i]) : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < kMxPasses; ++p) {
+    const int64_t row = row0 + 4 * p;
+    uint32_t top = mag_bits(f[p][0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = max(top, mag_bits(f[p][i]));
+    top = max(top, dpp_u32<kDppXor1>(top));
+    top = max(top, dpp_u32<kDppXor2>(top));
+    const uint32_t e = mx_scale(top);
+    const uint32_t c = mx_codes8(f[p], e);
+    // lanes 0, 4, 8, 12 of the row hold the four exponents; a block behind K
+    // has exponent 0 (its values were taken as zeros)
+    uint32_t word = e << ((j >> 2) * 8);
+    word |= dpp_u32<kDppHalfMirror>(word);
+    word |= dpp_u32<kDppMirror>(word);
+    if (row < rows) {
+      if (k < K) codes[(row * K + k) >> 3] = c;
+      if (j == 0) scales[static_cast<int64_t>(group) * rows + row] = word;
+    }
+  }
+}
+
+// Rows that are adjacent in memory (a transposed view: element (row, k) at
+// k ld + row).  A workgroup takes 128 rows of one k group; wave w its block w,
+// lane l rows 2l and 2l + 1, whose 32 values it holds; the codes go through
+// LDS so that a row's 64 bytes are written together.
+constexpr int kMxCols = 128;
+
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void mx_quantize_t_kernel(const typename MxElem<DT>::type* X,
+                                                            int64_t ld, uint8_t* codes,
+                                                            uint32_t* scales, int64_t rows, int K,
+                                                            int groups) {
+  using E = MxElem<DT>;
+  typedef typename E::type pair_t __attribute__((ext_vector_type(2)));
+  __shared__ u4_t buf[kMxCols][4];
+  __shared__ uint8_t sbuf[kMxCols][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int group = static_cast<int>(blockIdx.x % groups);
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x / groups) * kMxCols;
+  const int64_t row = row0 + 2 * lane;
+  const int k0 = group * kMxGroup + wave * kMxBlock;
+  uint32_t e[2] = {0u, 0u};
+  u4_t word[2] = {};
+  if (k0 < K) {
+    float f[2][kMxBlock];
+    uint32_t top[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < kMxBlock; ++i) {
+      const typename E::type* x = X + (k0 + i) * ld + row;
+      if (VEC) {
+        const pair_t v = row < rows ? __builtin_nontemporal_load(reinterpret_cast<const pair_t*>(x))
+                                    : pair_t{};
+        f[0][i] = E::get(v[0]);
+        f[1][i] = E::get(v[1]);
+      } else {
+        f[0][i] = row < rows ? E::get(x[0]) : 0.0f;
+        f[1][i] = row + 1 < rows ? E::get(x[1]) : 0.0f;
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) top[r] = max(top[r], mag_bits(f[r][i]));
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      e[r] = mx_scale(top[r]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float g[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = f[r][8 * q + i];
+        word[r][q] = mx_codes8(g, e[r]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    buf[2 * lane + r][wave] = word[r];
+    sbuf[2 * lane + r][wave] = static_cast<uint8_t>(e[r]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int c = tid + 256 * u, r = c >> 2, b = c & 3;
+    const int k = group * kMxGroup + b * kMxBlock;
+    if (row0 + r < rows && k < K)
+      *reinterpret_cast<u4_t*>(codes + ((row0 + r) * K + k) / 2) = buf[r][b];
+  }
+  if (tid < kMxCols && row0 + tid < rows)
+    scales[static_cast<int64_t>(group) * rows + row0 + tid] =
+        *reinterpret_cast<const uint32_t*>(sbuf[tid]);
+}
+
+template <int DT>
+__device__ __forceinline__ typename MxElem<DT>::type mx_out(float v) {
+  if constexpr (DT == kMxF32) {
+    return v;
+  } else if constexpr (DT == kMxF16) {
+    return __builtin_bit_cast(unsigned short, static_cast<_Float16>(v));
+  } else {
+    return __builtin_bit_cast(unsigned short, static_cast<__bf16>(v));
+  }
+}
+
+// A code's value times the block's power of two, exact in 32 bits (down to
+// 2^-128; above 2^125 times 6 it overflows to infinity, as it should).
+__device__ __forceinline__ float mx_value(uint32_t code, uint32_t e) {
+  const uint32_t m = code & 7u;
+  // 2^(e2 - 1) (1 + m / 2), or m / 2 with a zero exponent
+  const float v = m < 2u ? 0.5f * static_cast<float>(m)
+                         : __builtin_bit_cast(float, ((m >> 1) + 126u) << 23 | (m & 1u) << 22);
+  const float s = e == 255u ? __builtin_nanf("") : v * mx_power(e);
+  return code & 8u ? -s : s;
+}
+
+// Thread t expands eight codes: a word of them read, 16 or 32 bytes written.
+template <int DT>
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* codes,
+                                                            const uint8_t* scales, int64_t rows,
+                                                            int K, typename MxElem<DT>::type* out) {
+  const int per_row = K / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= rows * per_row) return;
+  const int64_t row = i / per_row;
+  const int k = static_cast<int>(i - row * per_row) * 8;
+  const uint32_t c = codes[i];
+  const uint32_t e = scales[((k / kMxGroup) * rows + row) * 4 + k / kMxBlock % 4];
+  typedef typename MxElem<DT>::type vec __attribute__((ext_vector_type(4)));
+  vec v[2];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) v[u / 4][u % 4] = mx_out<DT>(mx_value(c >> (4 * u) & 15u, e));
+  vec* o = reinterpret_cast<vec*>(out + i * 8);
+  o[0] = v[0];
+  o[1] = v[1];
+}
+
+struct MxArgs {
+  const uint8_t* xc;  // x codes [M, K / 2]
+  const uint8_t* xs;  // x scales [groups, M, 4]
+  const uint8_t* wc;  // w codes [N, K / 2]
+  const uint8_t* ws;  // w scales [groups, N, 4]
+  void* y;            // [M, N]
+  int M, N, K;
+};
+
+constexpr int kMxChunk = 512;  // k of one step of a wave: a lane's four blocks
+constexpr int kMxWaves = 8;
+
+// One 16-row operand of a step as the matrix cores take it: lane l holds row
+// l % 16 and, of the step's 16 blocks, the four from 4 (l / 16) on: 64 adjacent
+// bytes and one word of scales.  (The sum over k may be taken in any order, so
+// the step's j-th product runs over the j-th block of every lane.)
+struct MxFrag {
+  u4_t c[4];
+  uint32_t s;
+};
+
+// Rows r0 .. r0 + 15 of a matrix as buffer resources; a row or block that is
+// not there reads as zeros (an offset no resource reaches).
+struct MxRows {
+  __amdgpu_buffer_rsrc_t codes, scales;
+  uint32_t code0, scale0;  // this lane's offsets at k = 0
+  uint32_t pitch;          // bytes between two words of scales of one row
+  int blocks;              // blocks from this lane's first one on
+  __device__ __forceinline__ MxRows(const uint8_t* c, const uint8_t* s, int rows, int K, int r0,
+                                    int lane) {
+    const int r = lane & 15, g = lane >> 4;
+    const int groups = (K + kMxGroup - 1) / kMxGroup;
+    const int here = min(16, rows - r0);
+    codes = make_rsrc(c + static_cast<int64_t>(r0) * (K / 2),
+                      static_cast<uint32_t>(max(here, 0)) * static_cast<uint32_t>(K / 2));
+    scales = make_rsrc(s, static_cast<uint32_t>(groups) * static_cast<uint32_t>(rows) * 4u);
+    const bool in = r < here;
+    code0 = in ? static_cast<uint32_t>(r) * (K / 2) + g * 64u : kOutOfRange;
+    scale0 = in ? (static_cast<uint32_t>(g) * rows + r0 + r) * 4u : kOutOfRange;
+    pitch = static_cast<uint32_t>(rows) * 4u;
+    blocks = K / kMxBlock - 4 * g;
+  }
+  __device__ __forceinline__ void load(MxFrag& f, int chunk) const {
+    const int first = chunk * 16;  // of the lane's blocks, counted from its own first
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      f.c[j] = __builtin_bit_cast(
+          u4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                    codes, first + j < blocks ? code0 + chunk * 256u + j * 16u : kOutOfRange, 0, 0));
+    f.s = __builtin_amdgcn_raw_buffer_load_b32(
+        scales, first < blocks ? scale0 + chunk * 4u * pitch : kOutOfRange, 0, 0);
+  }
+};
+
+template <int J>
+__device__ __forceinline__ f4_t mx_mfma16(const MxFrag& a, const MxFrag& b, f4_t c) {
+  const u4_t x = a.c[J], y = b.c[J];
+  const i8_t va = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], 0, 0, 0, 0};
+  const i8_t vb = {(int)y[0], (int)y[1], (int)y[2], (int)y[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, J, (int)a.s, J, (int)b.s);
+}
+
+// y = x w^T for few rows of x.  A workgroup takes 16 rows of w and 16 MT rows
+// of x; its eight waves share out the k in steps of 512 and meet in LDS, in
+// wave order.
+template <int MT, int DT>
+__global__ __launch_bounds__(64 * kMxWaves) void mx_rows_kernel(MxArgs a) {
+  __shared__ float part[kMxWaves][MT][16][17];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
+  const int chunks = (a.K + kMxChunk - 1) / kMxChunk;
+  const MxRows w(a.wc, a.ws, a.N, a.K, n0, lane);
+  f4_t acc[MT] = {};
+  for (int c = wave; c < chunks; c += kMxWaves) {
+    MxFrag fw;
+    w.load(fw, c);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const MxRows x(a.xc, a.xs, a.M, a.K, m0 + 16 * t, lane);
+      MxFrag fx;
+      x.load(fx, c);
+      acc[t] = mx_mfma16<0>(fw, fx, acc[t]);
+      acc[t] = mx_mfma16<1>(fw, fx, acc[t]);
+      acc[t] = mx_mfma16<2>(fw, fx, acc[t]);
+      acc[t] = mx_mfma16<3>(fw, fx, acc[t]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[wave][t][lane & 15][4 * (lane >> 4) + i] = acc[t][i];
+  __syncthreads();
+  auto* y = static_cast<typename MxElem<DT>::type*>(a.y);
+  for (int e = threadIdx.x; e < MT * 256; e += 64 * kMxWaves) {
+    const int t = e >> 8, m = e >> 4 & 15, n = e & 15;
+    float s = part[0][t][m][n];
+#pragma unroll
+    for (int v = 1; v < kMxWaves; ++v) s += part[v][t][m][n];
+    const int gm = m0 + 16 * t + m, gn = n0 + n;
+    if (gm < a.M && gn < a.N) y[static_cast<int64_t>(gm) * a.N + gn] = mx_out<DT>(s);
+  }
+}
+
+template <int DT>
+hipError_t launch_mx_matmul(const MxArgs& a, hipStream_t stream) {
+  const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.N, 16)),
+                  static_cast<unsigned>(ceil_div(a.M, 16 * mt)));
+  const int threads = 64 * kMxWaves;
+  if (mt == 1) mx_rows_kernel<1, DT><<<grid, threads, 0, stream>>>(a);
+  else if (mt == 2) mx_rows_kernel<2, DT><<<grid, threads, 0, stream>>>(a);
+  else mx_rows_kernel<4, DT><<<grid, threads, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_mx_quantize(const void* X, int64_t rows, int64_t K, int64_t row_stride,
+                              int64_t k_stride, void* codes, void* scales, hipStream_t stream) {
+  using T = typename MxElem<DT>::type;
+  const auto* x = static_cast<const T*>(X);
+  const int64_t groups = ceil_div(K, kMxGroup);
+  const int k = static_cast<int>(K);
+  if (k_stride == 1) {
+    const int64_t tiles = ceil_div(K, 4 * kMxGroup);
+    const dim3 grid(static_cast<unsigned>(tiles * ceil_div(rows, kMxRows)));
+    auto* c = static_cast<uint32_t*>(codes);
+    auto* s = static_cast<uint32_t*>(scales);
+    // 16-byte loads where every row starts on 16 bytes
+    if (aligned(X, 16) && row_stride * sizeof(T) % 16 == 0)
+      mx_quantize_kernel<DT, true><<<grid, 256, 0, stream>>>(x, row_stride, c, s, rows, k, (int)tiles);
+    else
+      mx_quantize_kernel<DT, false><<<grid, 256, 0, stream>>>(x, row_stride, c, s, rows, k, (int)tiles);
+  } else {
+    const dim3 grid(static_cast<unsigned>(groups * ceil_div(rows, kMxCols)));
+    auto* c = static_cast<uint8_t*>(codes);
+    auto* s = static_cast<uint32_t*>(scales);
+    // two rows a load where every k starts on both
+    if (aligned(X, 2 * sizeof(T)) && k_stride % 2 == 0 && rows % 2 == 0)
+      mx_quantize_t_kernel<DT, true><<<grid, 256, 0, stream>>>(x, k_stride, c, s, rows, k, (int)groups);
+    else
+      mx_quantize_t_kernel<DT, false><<<grid, 256, 0, stream>>>(x, k_stride, c, s, rows, k, (int)groups);
+  }
+  return hipGetLastError();
+}
+
+int check_mx(int64_t rows, int64_t K, int64_t dtype) {
+  NIBBLE_CHECK(rows >= 0 && K >= 0, "negative dimension");
+  NIBBLE_CHECK(K % kMxBlock == 0, "K=%lld is not a multiple of %d", (long long)K, kMxBlock);
+  // 32-bit offsets within 16 rows of codes and within the scales
+  NIBBLE_CHECK(K <= (1 << 24), "K above %d", 1 << 24);
+  NIBBLE_CHECK(rows <= (1 << 28) && ceil_div(K, kMxGroup) * rows * 4 < (int64_t(1) << 31),
+               "a matrix of %lld x %lld has 2^31 bytes of scales or more", (long long)rows,
+               (long long)K);
+  NIBBLE_CHECK(dtype == kMxF16 || dtype == kMxBF16 || dtype == kMxF32,
+               "dtype must be 0 (fp16), 1 (bf16) or 2 (fp32), got %lld", (long long)dtype);
+  return NIBBLE_OK;
+}
+
+}  // namespace
+}  // namespace nibble
+
+using namespace nibble;
+
+extern "C" int nibble_mx_quantize(const void* X, int64_t rows, int64_t K, int64_t row_stride,
+                                  int64_t k_stride, int64_t dtype, void* codes, void* scales,
+                                  void* stream_) {
+  const int rc = check_mx(rows, K, dtype);
+  if (rc != NIBBLE_OK) return rc;
+  if (rows == 0 || K == 0) return ok();
+  NIBBLE_CHECK(row_stride > 0 && k_stride > 0 && (k_stride == 1 || row_stride == 1),
+               "one of the strides must be 1 and neither below, got %lld and %lld",
+               (long long)row_stride, (long long)k_stride);
+  NIBBLE_CHECK(row_stride < (int64_t(1) << 40) && k_stride < (int64_t(1) << 40), "stride above 2^40");
+  NIBBLE_CHECK(X != nullptr && codes != nullptr && scales != nullptr, "null pointer");
+  NIBBLE_CHECK(aligned(X, dtype == kMxF32 ? 4 : 2) && aligned(codes, 16) && aligned(scales, 4),
+               "misaligned pointer");
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  DeviceGuard guard;
+  int dev = 0;
+  NIBBLE_HIP(guard.enter(stream, &dev));
+  const hipError_t e =
+      dtype == kMxF16    ? launch_mx_quantize<kMxF16>(X, rows, K, row_stride, k_stride, codes, scales, stream)
+      : dtype == kMxBF16 ? launch_mx_quantize<kMxBF16>(X, rows, K, row_stride, k_stride, codes, scales, stream)
+                         : launch_mx_quantize<kMxF32>(X, rows, K, row_stride, k_stride, codes, scales, stream);
+  if (e != hipSuccess) return hip_fail(e, "mx quantize kernel launch");
+  return ok();
+}
+
+extern "C" int nibble_mx_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K,
+                                    int64_t dtype, void* out, void* stream_) {
+  const int rc = check_mx(rows, K, dtype);
+  if (rc != NIBBLE_OK) return rc;
+  if (rows == 0 || K == 0) return ok();
+  NIBBLE_CHECK(codes != nullptr && scales != nullptr && out != nullptr, "null pointer");
+  NIBBLE_CHECK(aligned(codes, 16) && aligned(scales, 4) && aligned(out, 16), "misaligned pointer");
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  DeviceGuard guard;
+  int dev = 0;
+  NIBBLE_HIP(guard.enter(stream, &dev));
+  const auto* c = static_cast<const uint32_t*>(codes);
+  const auto* s = static_cast<const uint8_t*>(scales);
+  const dim3 grid(static_cast<unsigned>(ceil_div(rows * (K / 8), 256)));
+  if (dtype == kMxF32)
+    mx_dequantize_kernel<kMxF32><<<grid, 256, 0, stream>>>(c, s, rows, (int)K, static_cast<float*>(out));
+  else if (dtype == kMxF16)
+    mx_dequantize_kernel<kMxF16><<<grid, 256, 0, stream>>>(c, s, rows, (int)K,
+                                                         static_cast<unsigned short*>(out));
+  else
+    mx_dequantize_kernel<kMxBF16><<<grid, 256, 0, stream>>>(c, s, rows, (int)K,
+                                                          static_cast<unsigned short*>(out));
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return hip_fail(e, "mx dequantize kernel launch");
+  return ok();
+}
+
+extern "C" int nibble_mx_matmul(const void* x_codes, const void* x_scales, int64_t M,
+                                const void* w_codes, const void* w_scales, int64_t N, int64_t K,
+                                int64_t dtype, void* Y, void* stream_) {
+  int rc = check_mx(M, K, dtype);
+  if (rc != NIBBLE_OK) return rc;
+  rc = check_mx(N, K, dtype);
+  if (rc != NIBBLE_OK) return rc;
+  if (M == 0 || N == 0) return ok();
+  NIBBLE_CHECK(M <= 65535 * 64, "more than %d rows of x", 65535 * 64);
+  NIBBLE_CHECK(Y != nullptr, "null pointer");
+  NIBBLE_CHECK(K == 0 || (x_codes != nullptr && x_scales != nullptr && w_codes != nullptr &&
+                          w_scales != nullptr),
+               "null pointer");
+  NIBBLE_CHECK(aligned(x_codes, 16) && aligned(w_codes, 16) && aligned(x_scales, 4) &&
+                   aligned(w_scales, 4) && aligned(Y, 16),
+               "misaligned pointer");
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  DeviceGuard guard;
+  int dev = 0;
+  NIBBLE_HIP(guard.enter(stream, &dev));
+  const MxArgs a{static_cast<const uint8_t*>(x_codes), static_cast<const uint8_t*>(x_scales),
+                 static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), Y,
+                 static_cast<int>(M), static_cast<int>(N), static_cast<int>(K)};
+  const hipError_t e = dtype == kMxF16    ? launch_mx_matmul<kMxF16>(a, stream)
+                       : dtype == kMxBF16 ? launch_mx_matmul<kMxBF16>(a, stream)
+                                          : launch_mx_matmul<kMxF32>(a, stream);
+  if (e != hipSuccess) return hip_fail(e, "mx matmul kernel launch");
+  return ok();
+}

@@ -530,6 +530,16 @@ def _tracked(t: torch.Tensor) -> bool:
             or getattr(forward_ad, "_current_level", 0) >= 0 or modes_follow())
 
 
+def _check_no_backward(name: str, t: torch.Tensor) -> None:
+    """For operators without a backward: an input that autograd follows (in
+    reverse or forward mode) is refused rather than silently cut off."""
+    if (t.requires_grad and torch.is_grad_enabled()) or (
+            getattr(forward_ad, "_current_level", -1) >= 0
+            and forward_ad.unpack_dual(t).tangent is not None):
+        raise RuntimeError(f"{name} is followed by autograd, and this operator has no backward: "
+                           "detach it or call under torch.no_grad()")
+
+
 def matmul_bias(X: torch.Tensor, qw: QuantizedWeight, bias: torch.Tensor) -> torch.Tensor:
     """``matmul(X, qw) + bias`` -- the arithmetic of the reference's
     ``QuantLinear`` with a bias (ops.py:131-135): the fp16 product, then the
