@@ -426,6 +426,54 @@ NIBBLE_API int nibble_chain_destroy(void* chain);
 NIBBLE_API int64_t nibble_chain_strip_cols(int64_t K, int64_t N, int64_t group_size, int64_t M);
 
 /*
+ * The step around a layer's attention for several tokens of several
+ * sequences.  No counterpart in the reference's extension.  dtype: 0 fp16, 1
+ * bf16 (of every tensor but the rotary tables, which are fp32); head_dim 64 or
+ * 128.  Element (b, h, s, d) of a cache is at b batch_stride + h head_stride +
+ * s row_stride + d elements, the strides multiples of 8; max_seq rows.  All
+ * pointers are 16-byte aligned except the int32 arrays and tables (4) and
+ * the mask (1).
+ */
+
+/* Norms of the query and key heads (weights [head_dim], NULL: none), rotary
+ * embedding (tables [rope_rows, head_dim / 2], both NULL: none) and cache
+ * append: QKV [batch, tokens, (n_heads + 2 n_kv_heads) head_dim]; positions and
+ * slots int32 [batch, tokens]; the q heads go to Q_out [batch, tokens, n_heads
+ * head_dim], k and v to row `slots` of their sequence's caches.  A token whose
+ * slot or position does not exist writes no row, and zeros to Q_out. */
+NIBBLE_API int nibble_qk_norm_rope(const void* QKV, int64_t dtype, int64_t batch, int64_t tokens,
+                                   int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                   void* K_cache, int64_t k_batch_stride, int64_t k_head_stride,
+                                   int64_t k_row_stride, void* V_cache, int64_t v_batch_stride,
+                                   int64_t v_head_stride, int64_t v_row_stride, int64_t max_seq,
+                                   const void* positions, const void* slots, const void* q_weight,
+                                   const void* k_weight, float eps, const void* rope_cos,
+                                   const void* rope_sin, int64_t rope_rows, void* Q_out,
+                                   void* stream);
+
+/* Attention of trees of drafted tokens: Q [batch, tokens, n_heads head_dim];
+ * sequence b holds lengths[b] rows, and its tree's sizes[b] tokens (NULL:
+ * `tokens` each) lie in the rows behind them.  Token i sees all lengths[b]
+ * rows and the tree tokens j with mask[b][i][j] != 0 (uint8 [mask_batches,
+ * tokens, tokens], mask_batches 1 or batch; NULL: j <= i).  Out [batch, tokens,
+ * n_heads head_dim] = softmax(scale q k^T) v, zeros for tokens that see nothing
+ * and behind a tree's last.  Row strides are at most 2^22 elements.  The
+ * workspace (nibble_attention_tree_workspace_bytes, 256-byte aligned; NULL when
+ * that is 0) needs no initial contents. */
+NIBBLE_API int nibble_attention_tree(const void* Q, int64_t dtype, int64_t batch, int64_t tokens,
+                                     int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                     const void* K_cache, int64_t k_batch_stride,
+                                     int64_t k_head_stride, int64_t k_row_stride,
+                                     const void* V_cache, int64_t v_batch_stride,
+                                     int64_t v_head_stride, int64_t v_row_stride, int64_t max_seq,
+                                     const void* lengths, const void* mask, int64_t mask_batches,
+                                     const void* sizes, float scale, void* Out, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+NIBBLE_API size_t nibble_attention_tree_workspace_bytes(int64_t batch, int64_t tokens,
+                                                        int64_t n_heads, int64_t n_kv_heads,
+                                                        int64_t head_dim, int64_t max_seq);
+
+/*
  * Microscaled 4-bit floats (OCP MXFP4).  No counterpart in the reference.  A
  * matrix [rows, K], K a multiple of 32, is
  *   codes   uint8 [rows, K / 2], two codes a byte along K, the even k low:

@@ -30,7 +30,8 @@ LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libnibblegemm_amd.so")
 
 HIP_SOURCES = ["abi.hip", "dequant.hip", "gemv.hip", "gemm.hip", "glue.hip", "chain.hip", "probe.hip",
-               "quantize.hip", "mx.hip"]
+               "quantize.hip", "mx.hip",
+               "qk_norm.hip", "tree.hip"]
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [

@@ -252,6 +252,64 @@ static PyObject* py_attention_ws(PyObject* self, PyObject* const* a, Py_ssize_t 
   return Py_BuildValue("(nn)", (Py_ssize_t)ws, (Py_ssize_t)cb);
 }
 
+/* qk_norm_rope(QKV, dtype, batch, tokens, n_heads, n_kv, head_dim, Kc, kb, kh, kr, Vc, vb, vh, vr,
+ * max_seq, positions, slots, q_weight, k_weight, eps, cos, sin, rope_rows, Q_out, stream) */
+static PyObject* py_qk_norm_rope(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (!nargs_is(n, 26, "qk_norm_rope")) return NULL;
+  void *qkv, *kc, *vc, *pos, *slots, *qw, *kw, *rc, *rs, *out, *stream;
+  long long dt, B, T, nh, nkv, hd, kb, kh, kr, vb, vh, vr, ms, rows;
+  double eps = PyFloat_AsDouble(a[20]);
+  if (eps == -1.0 && PyErr_Occurred()) return NULL;
+  if (!take_ptr(a[0], &qkv) || !take_i64(a[1], &dt) || !take_i64(a[2], &B) ||
+      !take_i64(a[3], &T) || !take_i64(a[4], &nh) || !take_i64(a[5], &nkv) ||
+      !take_i64(a[6], &hd) || !take_ptr(a[7], &kc) || !take_i64(a[8], &kb) ||
+      !take_i64(a[9], &kh) || !take_i64(a[10], &kr) || !take_ptr(a[11], &vc) ||
+      !take_i64(a[12], &vb) || !take_i64(a[13], &vh) || !take_i64(a[14], &vr) ||
+      !take_i64(a[15], &ms) || !take_ptr(a[16], &pos) || !take_ptr(a[17], &slots) ||
+      !take_ptr(a[18], &qw) || !take_ptr(a[19], &kw) || !take_ptr(a[21], &rc) ||
+      !take_ptr(a[22], &rs) || !take_i64(a[23], &rows) || !take_ptr(a[24], &out) ||
+      !take_ptr(a[25], &stream))
+    return NULL;
+  return PyLong_FromLong(nibble_qk_norm_rope(qkv, dt, B, T, nh, nkv, hd, kc, kb, kh, kr, vc, vb, vh,
+                                             vr, ms, pos, slots, qw, kw, (float)eps, rc, rs, rows,
+                                             out, stream));
+}
+
+/* attention_tree(Q, dtype, batch, tokens, n_heads, n_kv, head_dim, Kc, kb, kh, kr, Vc, vb, vh, vr,
+ * max_seq, lengths, mask, mask_batches, sizes, scale, Out, ws, ws_bytes, stream) */
+static PyObject* py_attention_tree(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (!nargs_is(n, 25, "attention_tree")) return NULL;
+  void *q, *kc, *vc, *len, *mask, *sizes, *out, *ws, *stream;
+  long long dt, B, T, nh, nkv, hd, kb, kh, kr, vb, vh, vr, ms, mb, wsb;
+  double scale = PyFloat_AsDouble(a[20]);
+  if (scale == -1.0 && PyErr_Occurred()) return NULL;
+  if (!take_ptr(a[0], &q) || !take_i64(a[1], &dt) || !take_i64(a[2], &B) || !take_i64(a[3], &T) ||
+      !take_i64(a[4], &nh) || !take_i64(a[5], &nkv) || !take_i64(a[6], &hd) ||
+      !take_ptr(a[7], &kc) || !take_i64(a[8], &kb) || !take_i64(a[9], &kh) ||
+      !take_i64(a[10], &kr) || !take_ptr(a[11], &vc) || !take_i64(a[12], &vb) ||
+      !take_i64(a[13], &vh) || !take_i64(a[14], &vr) || !take_i64(a[15], &ms) ||
+      !take_ptr(a[16], &len) || !take_ptr(a[17], &mask) || !take_i64(a[18], &mb) ||
+      !take_ptr(a[19], &sizes) || !take_ptr(a[21], &out) || !take_ptr(a[22], &ws) ||
+      !take_i64(a[23], &wsb) || !take_ptr(a[24], &stream))
+    return NULL;
+  return PyLong_FromLong(nibble_attention_tree(q, dt, B, T, nh, nkv, hd, kc, kb, kh, kr, vc, vb, vh,
+                                               vr, ms, len, mask, mb, sizes, (float)scale, out, ws,
+                                               (size_t)(wsb < 0 ? 0 : wsb), stream));
+}
+
+/* attention_tree_workspace_bytes(batch, tokens, n_heads, n_kv, head_dim, max_seq) */
+static PyObject* py_attention_tree_ws(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (!nargs_is(n, 6, "attention_tree_workspace_bytes")) return NULL;
+  long long B, T, nh, nkv, hd, ms;
+  if (!take_i64(a[0], &B) || !take_i64(a[1], &T) || !take_i64(a[2], &nh) ||
+      !take_i64(a[3], &nkv) || !take_i64(a[4], &hd) || !take_i64(a[5], &ms))
+    return NULL;
+  return PyLong_FromSize_t(nibble_attention_tree_workspace_bytes(B, T, nh, nkv, hd, ms));
+}
+
 /* dequant(Wq, wr, wc, S, sr, sc, g, fast, W, stream) */
 static PyObject* py_dequant(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   (void)self;
@@ -501,6 +559,12 @@ static PyMethodDef kMethods[] = {
      "nibble_attention_decode_f16"},
     {"attention_workspace_bytes", (PyCFunction)(void (*)(void))py_attention_ws, METH_FASTCALL,
      "(nibble_attention_decode_workspace_bytes, nibble_attention_decode_counter_bytes)"},
+    {"qk_norm_rope", (PyCFunction)(void (*)(void))py_qk_norm_rope, METH_FASTCALL,
+     "nibble_qk_norm_rope"},
+    {"attention_tree", (PyCFunction)(void (*)(void))py_attention_tree, METH_FASTCALL,
+     "nibble_attention_tree"},
+    {"attention_tree_workspace_bytes", (PyCFunction)(void (*)(void))py_attention_tree_ws,
+     METH_FASTCALL, "nibble_attention_tree_workspace_bytes"},
     {"chain_create", (PyCFunction)(void (*)(void))py_chain_create, METH_FASTCALL,
      "nibble_chain_create"},
     {"chain_run", (PyCFunction)(void (*)(void))py_chain_run, METH_FASTCALL, "nibble_chain_run"},

@@ -1,6 +1,9 @@
-"""Decode-step glue around the W4A16 projections: RMSNorm and grouped-query
-attention over a KV cache, as HIP kernels (``nibble_rmsnorm_f16`` and
-``nibble_attention_decode_f16`` of the C ABI).
+"""Decode-step glue around the projections: RMSNorm and grouped-query attention
+over a KV cache, as HIP kernels (``nibble_rmsnorm_f16`` and
+``nibble_attention_decode_f16`` of the C ABI), and the same step for several
+tokens of several sequences at once: head norms, rotary embedding and the cache
+append in one pass (``nibble_qk_norm_rope``) and attention of a tree of drafted
+tokens over the cache (``nibble_attention_tree``).
 
 The reference runs these as PyTorch / transformers ops of the model it
 decodes with QuantLinear layers swapped in (bench/bench_model.py:131-154,
@@ -18,7 +21,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native
-from .ops import _raise, _stream, _workspace, _ws_plan
+from .ops import _call, _check_no_backward, _raise, _stream, _workspace, _ws_plan
 
 HEAD_DIM = 128
 LLAMA3_ROPE_THETA = 500000.0
@@ -116,5 +119,209 @@ def attention_bytes(n_kv: int, pos: int) -> int:
     return 2 * n_kv * (pos + 1) * HEAD_DIM * 2
 
 
+_HALF_DTYPES = {torch.float16: 0, torch.bfloat16: 1}
+
+
+def _check_half(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
+    if t.dtype not in _HALF_DTYPES:
+        raise RuntimeError(f"{name} must be fp16 or bf16, got {t.dtype}")
+    if t.dtype != like.dtype:
+        raise RuntimeError(f"{name} must be {like.dtype}, got {t.dtype}")
+    _check_gpu(name, t, like)
+    _check_no_backward(name, t)
+    if t.is_neg():
+        raise RuntimeError(f"{name} must hold its values as they are (resolve_neg)")
+
+
+def _check_gpu(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must live on the GPU")
+    if t.device != like.device:
+        raise RuntimeError(f"{name} must live on {like.device}, got {t.device}")
+
+
+def _check_index(name: str, t: torch.Tensor, shape, like: torch.Tensor) -> None:
+    _check_gpu(name, t, like)
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+
+
+def _caches(x: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor):
+    """Checks the caches beside the tokens ``x`` ``[B, T, ..]`` or ``[T, ..]``
+    and returns both in the batched form."""
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _check_half(name, t, x)
+        if t.dim() != x.dim() + 1:
+            raise ValueError(f"{name} must have {x.dim() + 1} dimensions beside {x.dim()} of the "
+                             f"tokens, got {tuple(t.shape)}")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError(f"caches must have one shape, got {tuple(k_cache.shape)} and "
+                         f"{tuple(v_cache.shape)}")
+    if x.dim() == 2:
+        k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
+    elif k_cache.shape[0] != x.shape[0]:
+        raise ValueError(f"caches of {k_cache.shape[0]} sequences beside tokens of {x.shape[0]}")
+    if 0 in k_cache.shape[1:]:
+        raise ValueError(f"the caches are empty: {tuple(k_cache.shape)}")
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.stride(3) != 1:
+            raise RuntimeError(f"{name}: the elements of a row must be adjacent")
+    return k_cache, v_cache
+
+
+def qk_norm_rope(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 positions: torch.Tensor, slots: torch.Tensor,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                 eps: float = 1e-5,
+                 rope: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
+    """Norms of the query and key heads, their rotary embedding and the cache
+    append of ``T`` tokens of ``B`` sequences, in one pass.
+
+    qkv fp16 or bf16 [B, T, (n_heads + 2 n_kv) * D], the q|k|v projection's
+    output, D 64 or 128.  k_cache, v_cache [B, n_kv, max_seq, D] of its dtype,
+    of any strides that are multiples of 8 with a row's elements adjacent.
+    ``positions`` and ``slots`` int32 [B, T]: a token's rotary position and its
+    cache row.  Each q and k head is normalised, ``x / sqrt(mean(x^2) + eps) *
+    weight`` (weights [D] of qkv's dtype; None: no norm of those heads), then
+    rotated by the (cos, sin) of :func:`rope_tables` (None: no rotation), in
+    fp32 with one rounding.  k and v go to row ``slots`` of their sequence's
+    caches; q is returned as [B, T, n_heads * D].
+
+    A token whose slot is no row of the cache (-1, say) or whose position is
+    no row of the tables is padding: it writes no cache row and its q is zero.
+    The slots of one sequence's tokens must differ: of two tokens in one row
+    either may remain, in parts of 16 bytes.  One sequence may come without
+    its batch dimension: qkv [T, ..] (and q so), caches [n_kv, max_seq, D],
+    positions and slots [T].  Positions, slots and caches are read on the GPU,
+    so a captured call follows their contents.  There is no backward."""
+    _check_half("qkv", qkv, qkv)
+    if qkv.dim() not in (2, 3) or not qkv.is_contiguous():
+        raise RuntimeError("qkv must be a contiguous [B, T, ..] or [T, ..] tensor")
+    k4, v4 = _caches(qkv, k_cache, v_cache)
+    for name, t in (("k_cache", k4), ("v_cache", v4)):
+        if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+            raise RuntimeError(f"{name} is written and must not be an expanded view")
+    B, n_kv, max_seq, D = k4.shape
+    T, width = qkv.shape[-2:]
+    n_heads = width // D - 2 * n_kv
+    if width % D or n_heads < 1:
+        raise ValueError(f"qkv must be [.., (n_heads + 2 * {n_kv}) * {D}], got {tuple(qkv.shape)}")
+    for name, t in (("positions", positions), ("slots", slots)):
+        _check_index(name, t, qkv.shape[:-1], qkv)
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if t is not None:
+            _check_half(name, t, qkv)
+            if t.shape != (D,) or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous [{D}] tensor, got {tuple(t.shape)}")
+    cos_p = sin_p = None
+    rope_rows = 0
+    if rope is not None:
+        cos, sin = rope
+        for name, t in (("rope cos", cos), ("rope sin", sin)):
+            _check_gpu(name, t, qkv)
+            _check_no_backward(name, t)
+            if t.dtype != torch.float32 or not t.is_contiguous():
+                raise RuntimeError(f"{name} must be a contiguous fp32 GPU tensor")
+            if t.dim() != 2 or t.shape != (cos.shape[0], D // 2) or t.shape[0] < 1:
+                raise ValueError(f"{name} must be [rows, {D // 2}], got {tuple(t.shape)}")
+        cos_p, sin_p, rope_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+    ext = _native.binding()
+    out = torch.empty((*qkv.shape[:-1], n_heads * D), dtype=qkv.dtype, device=qkv.device)
+    _call(ext.qk_norm_rope, qkv.device, qkv.data_ptr(), _HALF_DTYPES[qkv.dtype], B, T, n_heads,
+          n_kv, D, k4.data_ptr(), *k4.stride()[:3], v4.data_ptr(), *v4.stride()[:3], max_seq,
+          positions.data_ptr(), slots.data_ptr(),
+          q_weight.data_ptr() if q_weight is not None else None,
+          k_weight.data_ptr() if k_weight is not None else None, float(eps), cos_p, sin_p,
+          rope_rows, out.data_ptr())
+    return out
+
+
+def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   lengths: torch.Tensor, mask: Optional[torch.Tensor] = None,
+                   sizes: Optional[torch.Tensor] = None,
+                   scale: Optional[float] = None) -> torch.Tensor:
+    """Attention of trees of drafted tokens over their sequences' caches.
+
+    q fp16 or bf16 [B, T, n_heads * D], as :func:`qk_norm_rope` returns it, D
+    64 or 128; k_cache, v_cache [B, n_kv, max_seq, D] as there.  ``lengths``
+    int32 [B]: the rows a sequence's cache held before its tree; the tree's
+    tokens lie in the rows behind them, in order.  ``mask`` bool [T, T] or
+    [B, T, T]: ``mask[i, j]`` is whether token i sees token j (:func:`tree_mask`
+    makes one from parents); None: the tokens up to itself, a run of tokens
+    such as a prompt's next part.  ``sizes`` int32 [B]: the tokens of each
+    sequence's tree, T where it is None.  Every token sees all ``lengths`` rows
+    before the tree.  Returns [B, T, n_heads * D]: per query head
+    ``softmax(scale q k^T) v`` over what the token sees, head i reading kv head
+    ``i // (n_heads // n_kv)``, scale ``1 / sqrt(D)`` by default, in fp32 with
+    the probabilities rounded to q's dtype.
+
+    Tokens behind a sequence's last, and tokens that see nothing, give zeros.
+    Rows that a token does not see have no part in its output, whatever they
+    hold; rows behind the tree are not read.  ``lengths`` and ``sizes`` count
+    as far as the cache goes.  One sequence may come without its batch
+    dimension: q [T, ..], caches [n_kv, max_seq, D], lengths [1], sizes [1].
+    Lengths, sizes and mask are read on the GPU, so a captured call follows
+    their contents.  There is no backward."""
+    _check_half("q", q, q)
+    if q.dim() not in (2, 3) or not q.is_contiguous():
+        raise RuntimeError("q must be a contiguous [B, T, ..] or [T, ..] tensor")
+    k4, v4 = _caches(q, k_cache, v_cache)
+    B, n_kv, max_seq, D = k4.shape
+    T, width = q.shape[-2:]
+    n_heads = width // D
+    if width % D:
+        raise ValueError(f"q must be [.., n_heads * {D}], got {tuple(q.shape)}")
+    _check_index("lengths", lengths, (B,), q)
+    if sizes is not None:
+        _check_index("sizes", sizes, (B,), q)
+    mask_p, mask_batches = None, 1
+    if mask is not None:
+        _check_gpu("mask", mask, q)
+        if mask.dtype != torch.bool or not mask.is_contiguous():
+            raise RuntimeError("mask must be a contiguous bool tensor")
+        if tuple(mask.shape) not in ((T, T), (B, T, T)):
+            raise ValueError(f"mask must be [{T}, {T}] or [{B}, {T}, {T}], got {list(mask.shape)}")
+        mask_p, mask_batches = mask.data_ptr(), B if mask.dim() == 3 else 1
+    ext = _native.binding()
+    dev = q.device
+    key = ("tree", B, T, n_heads, n_kv, D, max_seq)
+    nbytes = _ws_plan.get(key)
+    if nbytes is None:
+        nbytes = ext.attention_tree_workspace_bytes(B, T, n_heads, n_kv, D, max_seq)
+        _ws_plan[key] = nbytes
+    ws, ws_bytes = _workspace((nbytes, 0), dev, _stream(dev))
+    out = torch.empty_like(q)
+    _call(ext.attention_tree, dev, q.data_ptr(), _HALF_DTYPES[q.dtype], B, T, n_heads, n_kv, D,
+          k4.data_ptr(), *k4.stride()[:3], v4.data_ptr(), *v4.stride()[:3], max_seq,
+          lengths.data_ptr(), mask_p, mask_batches, sizes.data_ptr() if sizes is not None else None,
+          float(D ** -0.5 if scale is None else scale), out.data_ptr(),
+          ws.data_ptr() if ws is not None else None, ws_bytes)
+    return out
+
+
+def tree_mask(parents: torch.Tensor) -> torch.Tensor:
+    """The mask of :func:`attention_tree` for trees given by ``parents``, int
+    [T] or [B, T]: the index of a token's parent, which comes before it, or -1
+    for a token that follows the cached ones.  bool [T, T] or [B, T, T]: a
+    token sees itself and its ancestors."""
+    if parents.dim() not in (1, 2) or parents.is_floating_point():
+        raise ValueError(f"parents must be an integer [T] or [B, T] tensor, got {parents.dtype} "
+                         f"{tuple(parents.shape)}")
+    p = (parents if parents.dim() == 2 else parents[None]).long()
+    T = p.shape[-1]
+    i = torch.arange(T, device=p.device)
+    if bool((p >= i).any()) or bool((p < -1).any()):
+        raise ValueError("a parent must come before its token, or be -1")
+    seen = torch.eye(T, dtype=torch.bool, device=p.device).expand(p.shape[0], T, T).clone()
+    at = p  # the ancestor each token has reached
+    while bool((at >= 0).any()):
+        b, t = (at >= 0).nonzero(as_tuple=True)
+        seen[b, t, at[b, t]] = True
+        at = torch.where(at >= 0, p.gather(1, at.clamp(min=0)), -1)
+    return seen.reshape(*parents.shape, T)
+
+
 __all__ = ["HEAD_DIM", "LLAMA3_ROPE_THETA", "rmsnorm", "rope_tables", "attention_decode",
-           "attention_bytes"]
+           "attention_bytes", "qk_norm_rope", "attention_tree", "tree_mask"]

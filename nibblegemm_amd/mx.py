@@ -37,7 +37,7 @@ from typing import Optional, Union
 import torch
 
 from . import _native
-from .ops import _check_no_backward, _raise, _stream
+from .ops import _call, _check_no_backward
 
 #: Values that share a scale, and blocks whose scales share a word.
 MX_BLOCK = 32
@@ -106,19 +106,6 @@ def _check_values(name: str, x: torch.Tensor) -> None:
     _check_k(x.shape[1])
 
 
-def _launch(fn, device: torch.device, *args) -> None:
-    """``fn(*args, stream)`` on torch's current stream of ``device``.  Another
-    device is entered only where it is not the current one: a null stream is
-    the current device's."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, _stream(device))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _stream(device))
-    if rc:
-        _raise(rc, _native.binding())
-
-
 def mx_from_blocks(codes: torch.Tensor, scales: torch.Tensor) -> MXMatrix:
     """A matrix from ``codes`` uint8 ``[rows, K / 2]`` and one biased exponent a
     block, ``scales`` uint8 ``[rows, K / 32]``, on their device."""
@@ -154,7 +141,7 @@ def quantize_mx(x: torch.Tensor) -> MXMatrix:
     ext = _native.binding()
     codes = torch.empty((rows, K // 2), dtype=torch.uint8, device=x.device)
     scales = torch.empty((_groups(K), rows, 4), dtype=torch.uint8, device=x.device)
-    _launch(ext.mx_quantize, x.device, x.data_ptr(), rows, K, row_stride, k_stride,
+    _call(ext.mx_quantize, x.device, x.data_ptr(), rows, K, row_stride, k_stride,
             _DTYPES[x.dtype], codes.data_ptr(), scales.data_ptr())
     return MXMatrix(codes, scales, rows, K)
 
@@ -194,7 +181,7 @@ def dequantize_mx(m: MXMatrix, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
         return torch.where(e == 255, float("nan"), v).float().to(dtype)
     ext = _native.binding()
     out = torch.empty((m.rows, m.K), dtype=dtype, device=dev)
-    _launch(ext.mx_dequantize, dev, m.codes.data_ptr(), m.scales.data_ptr(), m.rows, m.K,
+    _call(ext.mx_dequantize, dev, m.codes.data_ptr(), m.scales.data_ptr(), m.rows, m.K,
             _DTYPES[dtype], out.data_ptr())
     return out
 
@@ -232,7 +219,7 @@ def matmul_mx(x: Union[torch.Tensor, MXMatrix], w: MXMatrix,
         x = quantize_mx(x)
     ext = _native.binding()
     y = torch.empty((M, w.rows), dtype=out_dtype, device=dev)
-    _launch(ext.mx_matmul, dev, x.codes.data_ptr(), x.scales.data_ptr(), M, w.codes.data_ptr(),
+    _call(ext.mx_matmul, dev, x.codes.data_ptr(), x.scales.data_ptr(), M, w.codes.data_ptr(),
             w.scales.data_ptr(), w.rows, K, _DTYPES[out_dtype], y.data_ptr())
     return y
 

@@ -105,6 +105,18 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _call(fn, device: torch.device, *args) -> None:
+    """``fn(*args, stream)`` on torch's current stream of ``device``, entered
+    where it is not the current one (a null stream is the current device's)."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _stream(device))
+    if rc:
+        _raise(rc, _native.binding())
+
+
 def _check_matmul_inputs(X: torch.Tensor, Wq: torch.Tensor, S: torch.Tensor) -> None:
     """The dtype/device/layout half of check_inputs (reference
     csrc/gemv_w4a16.cu:251-258, csrc/gemm_w4a16.cu:381-386)."""
