@@ -482,7 +482,7 @@ NIBBLE_API size_t nibble_attention_tree_workspace_bytes(int64_t batch, int64_t t
  *   scales  uint8 [ceil(K / 128), rows, 4], the power of two of each block of
  *           32 k, biased by 127 (255: the block is NaN), four neighbouring
  *           blocks to a word, zero behind the last; 4-byte aligned.
- * ceil(K / 128) * rows * 4 must be below 2^31, K at most 2^24.
+ * ceil(K / 128) * rows * 4 must be below 2^31, K at most 2^22.
  * dtype: 0 fp16, 1 bf16, 2 fp32.
  */
 
@@ -502,6 +502,15 @@ NIBBLE_API int nibble_mx_dequantize(const void* codes, const void* scales, int64
 NIBBLE_API int nibble_mx_matmul(const void* x_codes, const void* x_scales, int64_t M,
                                 const void* w_codes, const void* w_scales, int64_t N, int64_t K,
                                 int64_t dtype, void* Y, void* stream);
+/* The same with a dense X [M, K] (x_dtype; rows row_stride elements apart,
+ * every row on 16 bytes, the last one ending below 2^31 bytes), quantised on the
+ * way: nibble_mx_quantize's codes and nibble_mx_matmul's bits in one launch, where
+ * nibble_mx_matmul_takes_dense(M, N, K) is 1 (few rows); NIBBLE_ERR_UNSUPPORTED
+ * elsewhere. */
+NIBBLE_API int nibble_mx_matmul_dense(const void* X, int64_t M, int64_t row_stride, int64_t x_dtype,
+                                      const void* w_codes, const void* w_scales, int64_t N,
+                                      int64_t K, int64_t dtype, void* Y, void* stream);
+NIBBLE_API int nibble_mx_matmul_takes_dense(int64_t M, int64_t N, int64_t K);
 
 /*
  * Measurement: a streaming read of `bytes` (a positive multiple of 16) from

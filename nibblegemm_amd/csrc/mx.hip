@@ -265,6 +265,8 @@ struct MxArgs {
   const uint8_t* ws;  // w scales [groups, N, 4]
   void* y;            // [M, N]
   int M, N, K;
+  const void* x;      // dense x instead of codes: [M, K], rows ld elements apart
+  int ld;
 };
 
 constexpr int kMxChunk = 512;  // k of one step of a wave: a lane's four blocks
@@ -320,11 +322,63 @@ __device__ __forceinline__ f4_t mx_mfma16(const MxFrag& a, const MxFrag& b, f4_t
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, J, (int)a.s, J, (int)b.s);
 }
 
+// A lane's operand from dense values: the four blocks that MxRows::load would
+// read, quantised here (lane c of a 16-lane row holds row c of x).  Rows and
+// blocks that are not there read as zeros.
+template <int XD>
+struct MxDense {
+  static constexpr uint32_t kSize = XD == kMxF32 ? 4 : 2;
+  __amdgpu_buffer_rsrc_t x;
+  uint32_t off0;
+  int blocks;
+  __device__ __forceinline__ MxDense(const MxArgs& a, int lane) {
+    const int r = lane & 15, g = lane >> 4;
+    x = make_rsrc(a.x, (static_cast<uint32_t>(a.M - 1) * a.ld + a.K) * kSize);
+    off0 = r < a.M ? (static_cast<uint32_t>(r) * a.ld + g * 128u) * kSize : kOutOfRange;
+    blocks = a.K / kMxBlock - 4 * g;
+  }
+  __device__ __forceinline__ void load(MxFrag& f, int chunk) const {
+    constexpr int PIECES = 2 * kSize;  // of 16 bytes, a block
+    f.s = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t off = chunk * 16 + j < blocks
+                               ? off0 + (chunk * 512u + j * kMxBlock) * kSize : kOutOfRange;
+      u4_t v[PIECES];
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+        v[i] = __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(x, off + 16u * i, 0, 0));
+      uint32_t top = 0;
+      float b[4][8];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        float& t = b[i / 8][i % 8];
+        if constexpr (XD == kMxF32) {
+          const uint32_t w = v[i / 4][i % 4];
+          t = __builtin_bit_cast(float, w);
+        } else {
+          const uint32_t w = v[i / 8][i % 8 / 2];
+          t = MxElem<XD>::get(static_cast<unsigned short>(i % 2 ? w >> 16 : w));
+        }
+        top = max(top, mag_bits(t));
+      }
+      const uint32_t e = mx_scale(top);
+      f.s |= e << (8 * j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f.c[j][i] = mx_codes8(b[i], e);
+    }
+  }
+};
+
 // y = x w^T for few rows of x.  A workgroup takes 16 rows of w and 16 MT rows
 // of x; its eight waves share out the k in steps of 512 and meet in LDS, in
-// wave order.
-template <int MT, int DT>
+// wave order.  Codes come straight from memory into the matrix cores' operands;
+// a dense x (XD, at most 16 rows) is quantised by every workgroup on the way,
+// which costs less than a launch before this one.
+constexpr int kMxCodes = -1;
+template <int MT, int XD, int DT>
 __global__ __launch_bounds__(64 * kMxWaves) void mx_rows_kernel(MxArgs a) {
+  static_assert(XD == kMxCodes || MT == 1, "a dense x has at most 16 rows");
   __shared__ float part[kMxWaves][MT][16][17];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -337,9 +391,9 @@ __global__ __launch_bounds__(64 * kMxWaves) void mx_rows_kernel(MxArgs a) {
     w.load(fw, c);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const MxRows x(a.xc, a.xs, a.M, a.K, m0 + 16 * t, lane);
       MxFrag fx;
-      x.load(fx, c);
+      if constexpr (XD == kMxCodes) MxRows(a.xc, a.xs, a.M, a.K, m0 + 16 * t, lane).load(fx, c);
+      else MxDense<XD>(a, lane).load(fx, c);
       acc[t] = mx_mfma16<0>(fw, fx, acc[t]);
       acc[t] = mx_mfma16<1>(fw, fx, acc[t]);
       acc[t] = mx_mfma16<2>(fw, fx, acc[t]);
@@ -362,15 +416,79 @@ __global__ __launch_bounds__(64 * kMxWaves) void mx_rows_kernel(MxArgs a) {
   }
 }
 
+}  // namespace
+}  // namespace nibble
+
+#include "mx_tile.h"
+
+namespace nibble {
+namespace {
+
+template <int XT, int WT, int WM, int WN, int KU, int RING, int OCC, int DT>
+hipError_t launch_mx_tile(const MxArgs& a, hipStream_t stream) {
+  using S = MxTile<XT, WT, WM, WN, KU, RING>;
+  const int tm = static_cast<int>(ceil_div(a.M, S::BM)), tn = static_cast<int>(ceil_div(a.N, S::BN));
+  mx_tile_kernel<S, XT, WT, WM, WN, KU, DT, OCC><<<dim3(tm * tn), S::THREADS, 0, stream>>>(a, tm, tn);
+  return hipGetLastError();
+}
+
+// Which kernel a product runs on.  Few rows take the rows kernel while its
+// workgroups (16 rows of w by up to 64 of x) are few a CU; the tile kernel's
+// forms are priced by what a step of 128 k takes on a CU (ns; measured on
+// MI355X, N = 1024 .. 28672, K = 1024 .. 14336): `alone` where a CU has one tile,
+// `each` where it has many.  us, rows kernel / 64 x 64 / 64 x 128 / 128 x 128 /
+// 256 x 256 tiles: 64 x 4096 x 4096 7.8 / 8.4 / 11.7 / 15.3 / 28.5; 96 x 4096 x
+// 4096 11.2 / 8.5 / 11.7 / 15.2 / 28.6; 1 x 28672 x 4096 14.0 / 11.9 / 16.4 / 19.3
+// / 31.7; 1024 x 4096 x 4096 76 / 19.3 / 16.8 / 17.6 / 30.3; 2048 x 4096 x 4096
+// 147 / 33.4 / 32.6 / 25.1 / 35.5; 2048 x 14336 x 4096 537 / 112 / 97 / 85 / 77.
+enum MxForm { kMxRowsForm, kMx64x64, kMx64x128, kMx128x128, kMx256x256 };
+MxForm mx_form(int64_t M, int64_t N) {
+  const int64_t most = M <= 16 ? 768 : M <= 32 ? 384 : 256;
+  if (ceil_div(N, 16) * ceil_div(M, 64) <= most) return kMxRowsForm;
+  struct Price {
+    MxForm form;
+    int bm, bn, alone, each;
+  };
+  const Price prices[] = {{kMx64x64, 64, 64, 155, 122},
+                          {kMx64x128, 64, 128, 270, 210},
+                          {kMx128x128, 128, 128, 420, 345},
+                          {kMx256x256, 256, 256, 1050, 1150}};
+  MxForm best = kMx64x64;
+  int64_t least = INT64_MAX;
+  for (const Price& p : prices) {
+    const int64_t rounds = ceil_div(ceil_div(M, p.bm) * ceil_div(N, p.bn), 256);
+    const int64_t cost = std::max<int64_t>(p.alone, rounds * p.each);
+    if (cost < least) least = cost, best = p.form;
+  }
+  return best;
+}
+
 template <int DT>
 hipError_t launch_mx_matmul(const MxArgs& a, hipStream_t stream) {
+  switch (mx_form(a.M, a.N)) {
+    case kMx64x64: return launch_mx_tile<2, 2, 2, 2, 2, 3, 2, DT>(a, stream);
+    case kMx64x128: return launch_mx_tile<2, 4, 2, 2, 2, 2, 2, DT>(a, stream);
+    case kMx128x128: return launch_mx_tile<4, 4, 2, 2, 2, 2, 2, DT>(a, stream);
+    case kMx256x256: return launch_mx_tile<8, 4, 2, 4, 2, 2, 2, DT>(a, stream);
+    case kMxRowsForm: break;
+  }
   const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
   const dim3 grid(static_cast<unsigned>(ceil_div(a.N, 16)),
                   static_cast<unsigned>(ceil_div(a.M, 16 * mt)));
   const int threads = 64 * kMxWaves;
-  if (mt == 1) mx_rows_kernel<1, DT><<<grid, threads, 0, stream>>>(a);
-  else if (mt == 2) mx_rows_kernel<2, DT><<<grid, threads, 0, stream>>>(a);
-  else mx_rows_kernel<4, DT><<<grid, threads, 0, stream>>>(a);
+  if (mt == 1) mx_rows_kernel<1, kMxCodes, DT><<<grid, threads, 0, stream>>>(a);
+  else if (mt == 2) mx_rows_kernel<2, kMxCodes, DT><<<grid, threads, 0, stream>>>(a);
+  else mx_rows_kernel<4, kMxCodes, DT><<<grid, threads, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+template <int XD>
+hipError_t launch_mx_dense(const MxArgs& a, int dtype, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(ceil_div(a.N, 16)));
+  const int threads = 64 * kMxWaves;
+  if (dtype == kMxF16) mx_rows_kernel<1, XD, kMxF16><<<grid, threads, 0, stream>>>(a);
+  else if (dtype == kMxBF16) mx_rows_kernel<1, XD, kMxBF16><<<grid, threads, 0, stream>>>(a);
+  else mx_rows_kernel<1, XD, kMxF32><<<grid, threads, 0, stream>>>(a);
   return hipGetLastError();
 }
 
@@ -407,8 +525,8 @@ hipError_t launch_mx_quantize(const void* X, int64_t rows, int64_t K, int64_t ro
 int check_mx(int64_t rows, int64_t K, int64_t dtype) {
   NIBBLE_CHECK(rows >= 0 && K >= 0, "negative dimension");
   NIBBLE_CHECK(K % kMxBlock == 0, "K=%lld is not a multiple of %d", (long long)K, kMxBlock);
-  // 32-bit offsets within 16 rows of codes and within the scales
-  NIBBLE_CHECK(K <= (1 << 24), "K above %d", 1 << 24);
+  // 32-bit offsets within a tile's rows of codes and within the scales
+  NIBBLE_CHECK(K <= (1 << 22), "K above %d", 1 << 22);
   NIBBLE_CHECK(rows <= (1 << 28) && ceil_div(K, kMxGroup) * rows * 4 < (int64_t(1) << 31),
                "a matrix of %lld x %lld has 2^31 bytes of scales or more", (long long)rows,
                (long long)K);
@@ -496,10 +614,48 @@ extern "C" int nibble_mx_matmul(const void* x_codes, const void* x_scales, int64
   NIBBLE_HIP(guard.enter(stream, &dev));
   const MxArgs a{static_cast<const uint8_t*>(x_codes), static_cast<const uint8_t*>(x_scales),
                  static_cast<const uint8_t*>(w_codes), static_cast<const uint8_t*>(w_scales), Y,
-                 static_cast<int>(M), static_cast<int>(N), static_cast<int>(K)};
+                 static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), nullptr, 0};
   const hipError_t e = dtype == kMxF16    ? launch_mx_matmul<kMxF16>(a, stream)
                        : dtype == kMxBF16 ? launch_mx_matmul<kMxBF16>(a, stream)
                                           : launch_mx_matmul<kMxF32>(a, stream);
+  if (e != hipSuccess) return hip_fail(e, "mx matmul kernel launch");
+  return ok();
+}
+
+extern "C" int nibble_mx_matmul_takes_dense(int64_t M, int64_t N, int64_t K) {
+  return M >= 1 && M <= 16 && N >= 1 && K >= 1 && mx_form(M, N) == kMxRowsForm;
+}
+
+extern "C" int nibble_mx_matmul_dense(const void* X, int64_t M, int64_t row_stride, int64_t x_dtype,
+                                      const void* w_codes, const void* w_scales, int64_t N,
+                                      int64_t K, int64_t dtype, void* Y, void* stream_) {
+  int rc = check_mx(M, K, x_dtype);
+  if (rc != NIBBLE_OK) return rc;
+  rc = check_mx(N, K, dtype);
+  if (rc != NIBBLE_OK) return rc;
+  if (M == 0 || N == 0) return ok();
+  if (!nibble_mx_matmul_takes_dense(M, N, K))
+    return fail(NIBBLE_ERR_UNSUPPORTED,
+                "a dense x of %lld rows is quantised first for N=%lld, K=%lld", (long long)M,
+                (long long)N, (long long)K);
+  NIBBLE_CHECK(X != nullptr && Y != nullptr && w_codes != nullptr && w_scales != nullptr,
+               "null pointer");
+  const int64_t size = x_dtype == kMxF32 ? 4 : 2;
+  NIBBLE_CHECK(row_stride >= 0 && row_stride * size % 16 == 0 && aligned(X, 16),
+               "every row of x must start on 16 bytes");
+  NIBBLE_CHECK(((M - 1) * row_stride + K) * size < (int64_t(1) << 31), "rows of x beyond 2^31 bytes");
+  NIBBLE_CHECK(aligned(w_codes, 16) && aligned(w_scales, 4) && aligned(Y, 16), "misaligned pointer");
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  DeviceGuard guard;
+  int dev = 0;
+  NIBBLE_HIP(guard.enter(stream, &dev));
+  const MxArgs a{nullptr, nullptr, static_cast<const uint8_t*>(w_codes),
+                 static_cast<const uint8_t*>(w_scales), Y, static_cast<int>(M), static_cast<int>(N),
+                 static_cast<int>(K), X, static_cast<int>(row_stride)};
+  const int d = static_cast<int>(dtype);
+  const hipError_t e = x_dtype == kMxF16    ? launch_mx_dense<kMxF16>(a, d, stream)
+                       : x_dtype == kMxBF16 ? launch_mx_dense<kMxBF16>(a, d, stream)
+                                            : launch_mx_dense<kMxF32>(a, d, stream);
   if (e != hipSuccess) return hip_fail(e, "mx matmul kernel launch");
   return ok();
 }

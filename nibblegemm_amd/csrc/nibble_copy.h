@@ -5,20 +5,32 @@
 
 namespace nibble {
 
-// One LDS-DMA copy of 16 bytes a lane: lane l's bytes, from byte offset voff of
+// One LDS-DMA copy of 16 bytes a lane: lane l's bytes, at byte voff + soff of
 // [base, base + bytes) (beyond it: zeros), land at LDS byte address dst + 16 l;
-// dst is the same in every lane.  Written as assembly because the compiler,
-// knowing a pending copy, waits for it before every LDS read that it cannot
-// tell apart; the kernel's own waits (vmcnt) order the copies.  No register is
-// written; the addresses are read at issue.
+// dst and soff are the same in every lane.  (The range check takes soff in
+// without wrapping.)  Written as assembly because the compiler, knowing a
+// pending copy, waits for it before every LDS read that it cannot tell apart;
+// the kernel's own waits (vmcnt) order the copies.  No register is written; the
+// addresses are read at issue.
 __device__ __forceinline__ void lds_copy16(const void* base, uint32_t bytes, uint32_t dst,
-                                           uint32_t voff) {
+                                           uint32_t voff, uint32_t soff = 0) {
   const uint64_t b = reinterpret_cast<uint64_t>(base);
   const u4_t rsrc = {static_cast<uint32_t>(b), static_cast<uint32_t>(b >> 32) & 0xffffu, bytes,
                      0x00020000u};
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
-               : "s"(dst), "v"(voff), "s"(rsrc)
+               : "s"(dst), "v"(voff), "s"(rsrc), "s"(soff)
+               : "memory", "m0");
+}
+// The same with 4 bytes a lane, landing at dst + 4 l.
+__device__ __forceinline__ void lds_copy4(const void* base, uint32_t bytes, uint32_t dst,
+                                          uint32_t voff, uint32_t soff = 0) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  const u4_t rsrc = {static_cast<uint32_t>(b), static_cast<uint32_t>(b >> 32) & 0xffffu, bytes,
+                     0x00020000u};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+               :
+               : "s"(dst), "v"(voff), "s"(rsrc), "s"(soff)
                : "memory", "m0");
 }
 

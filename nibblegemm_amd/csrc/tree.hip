@@ -50,11 +50,11 @@ struct TreeArgs {
   float scale;  // times log2(e)
 };
 
-// Unit (16 bytes) u of LDS row r lies at unit u ^ tree_swizzle(r): the 16 rows
-// of a K read cover all banks once, and the 4-unit pieces of a V read do.
+// Unit (16 bytes) u of LDS row r lies at unit u ^ tree_swizzle(r): eight rows of
+// a K read, and four rows' 32-byte pieces of a V read, cover 32 banks once.
 template <int UNITS>
 __device__ __forceinline__ int tree_swizzle(int r) {
-  return UNITS == 16 ? ((r & 7) << 1) | (r >> 3 & 1) : ((r & 3) << 1) | (r >> 2 & 1);
+  return ((r & 3) << 1 | (r >> 2 & 1) | (r & 8)) & (UNITS - 1);
 }
 
 // A lane's value and the one of the lane 32 (16) away, in either order.

@@ -215,14 +215,27 @@ def matmul_mx(x: Union[torch.Tensor, MXMatrix], w: MXMatrix,
         out_dtype = x.dtype if dense else torch.float16
     if out_dtype not in _DTYPES:
         raise RuntimeError(f"out_dtype must be fp16, bf16 or fp32, got {out_dtype}")
+    ext = _native.binding()
+    N = w.rows
+    y = torch.empty((M, N), dtype=out_dtype, device=dev)
+    if dense and ext.mx_matmul_takes_dense(M, N, K) and _rows_on_16_bytes(x):
+        _call(ext.mx_matmul_dense, dev, x.data_ptr(), M, x.stride(0) if M > 1 else K,
+              _DTYPES[x.dtype], w.codes.data_ptr(), w.scales.data_ptr(), N, K, _DTYPES[out_dtype],
+              y.data_ptr())
+        return y
     if dense:
         x = quantize_mx(x)
-    ext = _native.binding()
-    y = torch.empty((M, w.rows), dtype=out_dtype, device=dev)
     _call(ext.mx_matmul, dev, x.codes.data_ptr(), x.scales.data_ptr(), M, w.codes.data_ptr(),
-            w.scales.data_ptr(), w.rows, K, _DTYPES[out_dtype], y.data_ptr())
+          w.scales.data_ptr(), N, K, _DTYPES[out_dtype], y.data_ptr())
     return y
 
+
+def _rows_on_16_bytes(x: torch.Tensor) -> bool:
+    """Whether a kernel may read the rows of ``x`` in pieces of 16 bytes."""
+    size = x.element_size()
+    return (x.stride(1) == 1 and x.data_ptr() % 16 == 0 and not x.is_neg()
+            and (x.shape[0] == 1 or x.stride(0) * size % 16 == 0)
+            and ((x.shape[0] - 1) * x.stride(0) + x.shape[1]) * size < 1 << 31)
 
 __all__ = ["MX_BLOCK", "MX_GROUP", "MX_VALUES", "MXMatrix", "dequantize_mx", "matmul_mx",
            "mx_from_blocks", "quantize_mx"]
