@@ -26,7 +26,7 @@ namespace nibble {
 namespace {
 
 constexpr int kTreeThreads = 256;
-constexpr int kTreeKeys = 128;  // keys a workgroup holds in LDS at a time
+constexpr int kTreeKeys = 64;  // keys of a tile
 constexpr int kTreeMaxSplits = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 // A query's reference maximum moves only when a score passes it by this much
@@ -47,7 +47,8 @@ struct TreeArgs {
   int64_t mask_batch;  // bytes between two sequences' masks
   int B, T, n_heads, n_kv, qpk, seq;
   int splits, row_tiles;
-  float scale;  // times log2(e)
+  float scale;  // its magnitude times log2(e); 1 for a scale of zero
+  float sign;   // its sign
 };
 
 // Unit (16 bytes) u of LDS row r lies at unit u ^ tree_swizzle(r): eight rows of
@@ -91,17 +92,24 @@ struct TreeSpan {
 };
 
 // One workgroup: 16 QT WQ query rows of one kv head (WQ = 4 / WK waves along
-// the rows, WK along the keys), one split of the cached rows.
+// the rows, WK along the keys), one split of the cached rows, in tiles of 64
+// keys.  A tile's rows of k and v are copied straight into one of two LDS
+// buffers while the tile before it is computed; two workgroups share a CU, so
+// one's softmax runs beside the other's products.
 template <class E, int D, int QT, int WK>
-__global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
+__global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   using T = typename E::type;
   using vec8 = typename E::vec8;
   constexpr int WQ = 4 / WK, KT = kTreeKeys, ROWS = 16 * QT * WQ;
-  constexpr int STEPS = KT / (32 * WK);  // 32-key steps of a wave in a tile
-  constexpr int UNITS = D / 8;           // 16-byte units of a row
-  constexpr int COPIES = KT * UNITS / kTreeThreads;  // of K or V, a wave and tile
+  constexpr int KPW = KT / WK < 32 ? KT / WK : 32;    // keys of a wave's step: 16 or 32
+  constexpr int KS = KPW / 16, STEPS = KT / (KPW * WK);
+  constexpr int UNITS = D / 8;                        // 16-byte units of a row
+  constexpr int COPIES = KT * UNITS / kTreeThreads;   // of K or V, a wave and tile
+  constexpr int CROWS = 64 / UNITS;                   // rows of a copy
   typedef short s4_t __attribute__((ext_vector_type(4)));
-  __shared__ __attribute__((aligned(16))) T kv[2][KT * D];
+  typedef short s8_t __attribute__((ext_vector_type(8)));
+  typedef __attribute__((address_space(3))) s4_t lds4_t;
+  __shared__ __attribute__((aligned(16))) T kv[2][2][KT * D];  // buffer, k or v
   __shared__ float stat[2][WK][WQ * QT * 16];
   static_assert(sizeof(kv) >= sizeof(float) * WK * WQ * 16 * D, "the sums fit");
 
@@ -109,9 +117,13 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int wq = wave / WK, wk = wave % WK;
   const int g = lane >> 4, c = lane & 15;
-  const int split = blockIdx.y;
-  const int row_tile = blockIdx.x % a.row_tiles;
-  const int unit = blockIdx.x / a.row_tiles;  // (b, kv head)
+  // Workgroup -> (sequence and kv head, split), row tile: the row tiles that
+  // read the same cache rows run on one XCD (id % 8) and share its L2.
+  const int slot = blockIdx.x >> 3;
+  const int pair = slot / a.row_tiles * 8 + (blockIdx.x & 7);
+  if (pair >= a.B * a.n_kv * a.splits) return;
+  const int row_tile = a.row_tiles - 1 - slot % a.row_tiles;  // the longest of a run first
+  const int unit = pair / a.splits, split = pair - unit * a.splits;
   const int b = unit / a.n_kv, h = unit - b * a.n_kv;
   const TreeSpan span(a, b);
   const int rows_all = a.T * a.qpk, rows = span.live * a.qpk;
@@ -125,6 +137,27 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
     end = min(end, span.len + (min(r0 + ROWS, rows) - 1) / a.qpk + 1);
   const int tiles = (end + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
   const int first = min(split * per, tiles) * KT, last = min(end, min((split + 1) * per, tiles) * KT);
+
+  const T* const kbase = static_cast<const T*>(a.k) + b * a.kb + h * a.kh;
+  const T* const vbase = static_cast<const T*>(a.v) + b * a.vb + h * a.vh;
+  const uint32_t lds0 = lds_address(kv) + wave * COPIES * 1024u;
+  const uint32_t kpitch = static_cast<uint32_t>(a.ks) * 2u, vpitch = static_cast<uint32_t>(a.vs) * 2u;
+  constexpr uint32_t kTile = KT * D * 2;  // bytes of a tile of k or v
+  auto copy = [&](int key0, int buf) {
+    // Rows behind the sequence's last read as zeros.
+    const int here = last - key0;
+    const T* const kt = kbase + key0 * a.ks;
+    const T* const vt = vbase + key0 * a.vs;
+#pragma unroll
+    for (int u = 0; u < COPIES; ++u) {
+      const int r = (wave * COPIES + u) * CROWS + lane / UNITS;
+      const uint32_t unit16 = ((lane % UNITS) ^ tree_swizzle<UNITS>(r)) * 16u;
+      const uint32_t dst = lds0 + buf * 2 * kTile + u * 1024u;
+      lds_copy16(kt, 0x7fffffffu, dst, r < here ? r * kpitch + unit16 : kOutOfRange);
+      lds_copy16(vt, 0x7fffffffu, dst + kTile, r < here ? r * vpitch + unit16 : kOutOfRange);
+    }
+  };
+  if (first < last) copy(first, 0);
 
   // Queries: lane (g, c) holds elements 32 s + 8 g .. + 7 of row c of a tile.
   vec8 q[QT][D / 32];
@@ -141,9 +174,18 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
       q[t][s] = in ? *reinterpret_cast<const vec8*>(static_cast<const T*>(a.q) + at + 32 * s)
                    : vec8{};
   }
+  if (a.sign != 1.0f) {  // a scale that is not positive: its sign goes into q, exactly
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          q[t][s][i] = static_cast<T>(static_cast<float>(q[t][s][i]) * a.sign);
+  }
 
   f4_t acc[QT][D / 16];
-  float top[QT], sum[QT];  // of query c; sum over this lane's keys
+  float top[QT], sum[QT];  // of query c, top times the scale; sum over this lane's keys
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     top[t] = -INFINITY;
@@ -152,74 +194,61 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
     for (int d = 0; d < D / 16; ++d) acc[t][d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  const T* const kbase = static_cast<const T*>(a.k) + b * a.kb + h * a.kh;
-  const T* const vbase = static_cast<const T*>(a.v) + b * a.vb + h * a.vh;
-  const uint32_t lds_k = lds_address(kv[0]), lds_v = lds_address(kv[1]);
-  for (int key0 = first; key0 < last; key0 += KT) {
-    // Rows behind the sequence's last read as zeros.
-    const int here = min(KT, last - key0);
-    const T* const kt = kbase + key0 * a.ks;
-    const T* const vt = vbase + key0 * a.vs;
-    const uint32_t kpitch = static_cast<uint32_t>(a.ks) * 2u, vpitch = static_cast<uint32_t>(a.vs) * 2u;
-#pragma unroll
-    for (int u = 0; u < COPIES; ++u) {
-      const int piece = (wave * COPIES + u) * 64 + lane;
-      const int r = piece / UNITS;
-      const uint32_t unit16 = ((piece % UNITS) ^ tree_swizzle<UNITS>(r)) * 16u;
-      const bool in = r < here;
-      const uint32_t at = (wave * COPIES + u) * 1024u;
-      lds_copy16(kt, 0x7fffffffu, lds_k + at, in ? r * kpitch + unit16 : kOutOfRange);
-      lds_copy16(vt, 0x7fffffffu, lds_v + at, in ? r * vpitch + unit16 : kOutOfRange);
-    }
+  // Byte offsets within a tile (rows 16 apart share the swizzle): of row c, k
+  // elements 8 g .. of each 32; of row 4 g + c / 4, v elements 4 (c % 4) .. of
+  // each 16.
+  const int krow = c * D * 2 + ((g ^ tree_swizzle<UNITS>(c)) * 16);
+  const int vr = 4 * g + (c >> 2);
+  const int vrow = vr * D * 2 + (((c >> 1 & 1) ^ tree_swizzle<UNITS>(vr)) * 16) + (c & 1) * 8;
+  int buf = 0;
+  for (int key0 = first; key0 < last; key0 += KT, buf ^= 1) {
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-    __syncthreads();
-#pragma unroll 1
-    for (int st = 0; st < STEPS; ++st) {
-      const int kb = (st * WK + wk) * 32;  // this step's first key in the tile
-      f4_t s[2][QT];
+    lds_barrier();
+    if (key0 + KT < last) copy(key0 + KT, buf ^ 1);
+    const char* const kt = reinterpret_cast<const char*>(kv[buf][0]);
+    const uint32_t vt = lds_address(kv[buf][1]);
 #pragma unroll
-      for (int kt16 = 0; kt16 < 2; ++kt16) {
+    for (int st = 0; st < STEPS; ++st) {
+      const int kb = (st * WK + wk) * KPW;  // this step's first key in the tile
+      f4_t s[KS][QT];
+#pragma unroll
+      for (int kt16 = 0; kt16 < KS; ++kt16) {
 #pragma unroll
         for (int t = 0; t < QT; ++t) s[kt16][t] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        const int r = kb + 16 * kt16 + c;
 #pragma unroll
         for (int ss = 0; ss < D / 32; ++ss) {
-          const vec8 ka = *reinterpret_cast<const vec8*>(
-              &kv[0][r * D + ((4 * ss + g) ^ tree_swizzle<UNITS>(r)) * 8]);
+          const vec8 ka = *reinterpret_cast<const vec8*>(kt + (kb + 16 * kt16) * D * 2 +
+                                                         (krow ^ (64 * ss)));
 #pragma unroll
           for (int t = 0; t < QT; ++t) s[kt16][t] = E::mfma(ka, q[t][ss], s[kt16][t]);
         }
       }
-      const int k0 = key0 + kb + 4 * g;  // key of s[0][.][0]
-      const bool tail = key0 + kb + 32 > span.len;
+      const bool tail = key0 + kb + KPW > span.len;
+      if (tail) {
+        const int k0 = key0 + kb + 4 * g;  // key of s[0][.][0]
 #pragma unroll
-      for (int t = 0; t < QT; ++t)
+        for (int t = 0; t < QT; ++t)
 #pragma unroll
-        for (int kt16 = 0; kt16 < 2; ++kt16)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float x = s[kt16][t][i] * a.scale;
-            if (tail) {
-              const int key = k0 + 16 * kt16 + i, other = key - span.len;
-              bool seen = key < last;
-              if (seen && other >= 0)
-                seen = a.mask == nullptr
-                           ? other <= node[t]
-                           : a.mask[b * a.mask_batch + static_cast<int64_t>(node[t]) * a.T + other] != 0;
-              x = seen ? x : -INFINITY;
-            }
-            s[kt16][t][i] = x;
+          for (int i = 0; i < 4 * KS; ++i) {
+            const int key = k0 + 16 * (i / 4) + i % 4, other = key - span.len;
+            bool seen = key < last;
+            if (seen && other >= 0)
+              seen = a.mask == nullptr
+                         ? other <= node[t]
+                         : a.mask[b * a.mask_batch + static_cast<int64_t>(node[t]) * a.T + other] != 0;
+            if (!seen) s[i / 4][t][i % 4] = -INFINITY;
           }
+      }
       vec8 p[QT];
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
         float m = s[0][t][0];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) m = fmaxf(m, s[i / 4][t][i % 4]);
-        m = swap_max(m);
+        for (int i = 1; i < 4 * KS; ++i) m = fmaxf(m, s[i / 4][t][i % 4]);
+        m = swap_max(m) * a.scale;
         if (__any(m > top[t] + kTreeSlack)) {
           const float up = fmaxf(m, top[t]);
-          const float keep = up == -INFINITY ? 1.0f : exp2f(top[t] - up);
+          const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - up);
           top[t] = up;
           sum[t] *= keep;
 #pragma unroll
@@ -230,7 +259,9 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
         const float base = top[t] == -INFINITY ? 0.0f : top[t];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float e = exp2f(s[i / 4][t][i % 4] - base);
+          const float e = i < 4 * KS
+                              ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4 % KS][t][i % 4], a.scale, -base))
+                              : 0.0f;
           sum[t] += e;
           p[t][i] = static_cast<T>(e);
         }
@@ -239,16 +270,11 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
       bool strange = false;
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
-        s4_t v2[2];
+        s4_t v2[2] = {};
 #pragma unroll
-        for (int kt16 = 0; kt16 < 2; ++kt16) {
-          const int r = kb + 16 * kt16 + 4 * g + (c >> 2);
-          const int u = (2 * d + (c >> 1 & 1)) ^ tree_swizzle<UNITS>(r);
-          typedef __attribute__((address_space(3))) s4_t lds4_t;
+        for (int kt16 = 0; kt16 < KS; ++kt16)
           v2[kt16] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds4_t*)(uintptr_t)(lds_v + (r * D + u * 8 + (c & 1) * 4) * 2u));
-        }
-        typedef short s8_t __attribute__((ext_vector_type(8)));
+              (lds4_t*)(uintptr_t)(vt + (kb + 16 * kt16) * D * 2 + (vrow ^ (32 * d))));
         s8_t vv = {v2[0][0], v2[0][1], v2[0][2], v2[0][3], v2[1][0], v2[1][1], v2[1][2], v2[1][3]};
         if (tail) {
 #pragma unroll
@@ -264,7 +290,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
       }
       if (tail && __any(strange)) {
         // Key by key, the rows that see the key only.
-        for (int kk = 0; kk < 32; ++kk) {
+        for (int kk = 0; kk < KPW; ++kk) {
           const int from = (kk % 16 / 4) * 16 + c, i = kk / 16 * 4 + kk % 4;
           const int r = kb + kk;
 #pragma unroll
@@ -279,7 +305,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int dim = 16 * d + 4 * g + e;
-                const T x = kv[1][r * D + ((dim / 8) ^ tree_swizzle<UNITS>(r)) * 8 + dim % 8];
+                const T x = kv[buf][1][r * D + ((dim / 8) ^ tree_swizzle<UNITS>(r)) * 8 + dim % 8];
                 const bool odd = (__builtin_bit_cast(unsigned short, x) & E::kExponent) == E::kExponent;
                 if (odd && w != 0.0f) acc[t][d][e] += w * static_cast<float>(x);
               }
@@ -287,8 +313,8 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
         }
       }
     }
-    __syncthreads();
   }
+  __syncthreads();
 
   // The waves along the keys meet: statistics first, then the sums on the
   // common maximum, 16 rows of each wave at a time through LDS.
@@ -302,45 +328,36 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
     }
   }
   __syncthreads();
-  float* const red = reinterpret_cast<float*>(&kv[0][0]);  // [WK][WQ 16][D]
-#pragma unroll 1
+  float* const red = reinterpret_cast<float*>(&kv[0][0][0]);  // [WK][WQ 16][D]
+#pragma unroll
   for (int t = 0; t < QT; ++t) {
-    float mine[QT], wmax[QT];
+    float m = stat[0][0][(wq * QT + t) * 16 + c];
 #pragma unroll
-    for (int u = 0; u < QT; ++u) {
-      float m = stat[0][0][(wq * QT + u) * 16 + c];
+    for (int w = 1; w < WK; ++w) m = fmaxf(m, stat[0][w][(wq * QT + t) * 16 + c]);
+    const float mine = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[t] - m);
 #pragma unroll
-      for (int w = 1; w < WK; ++w) m = fmaxf(m, stat[0][w][(wq * QT + u) * 16 + c]);
-      wmax[u] = m;
-      mine[u] = m == -INFINITY ? 0.0f : exp2f(top[u] - m);
-    }
-    (void)wmax;
+    for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-    for (int u = 0; u < QT; ++u)
-      if (u == t) {
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            red[(wk * WQ * 16 + wq * 16 + c) * D + 16 * d + 4 * g + i] = acc[u][d][i] * mine[u];
-      }
+      for (int i = 0; i < 4; ++i)
+        red[(wk * WQ * 16 + wq * 16 + c) * D + 16 * d + 4 * g + i] = acc[t][d][i] * mine;
     __syncthreads();
     for (int e = threadIdx.x; e < WQ * 16 * (D / 4); e += kTreeThreads) {
       const int rr = e / (D / 4), d = e % (D / 4) * 4;
-      const int slot = (rr / 16 * QT + t) * 16 + rr % 16;
+      const int slot16 = (rr / 16 * QT + t) * 16 + rr % 16;
       const int r = r0 + rr / 16 * 16 * QT + 16 * t + rr % 16;
       if (r >= rows_all) continue;
       f4_t o = *reinterpret_cast<const f4_t*>(&red[rr * D + d]);
-      float m = stat[0][0][slot];
+      float mr = stat[0][0][slot16];
 #pragma unroll
       for (int w = 1; w < WK; ++w) {
         o += *reinterpret_cast<const f4_t*>(&red[(w * WQ * 16 + rr) * D + d]);
-        m = fmaxf(m, stat[0][w][slot]);
+        mr = fmaxf(mr, stat[0][w][slot16]);
       }
       float l = 0.0f;
 #pragma unroll
       for (int w = 0; w < WK; ++w)
-        l += m == -INFINITY ? 0.0f : stat[1][w][slot] * exp2f(stat[0][w][slot] - m);
+        l += mr == -INFINITY ? 0.0f
+                             : stat[1][w][slot16] * __builtin_amdgcn_exp2f(stat[0][w][slot16] - mr);
       if (a.splits == 1) {
         const int i = r / a.qpk;
         T* out = static_cast<T*>(a.out) +
@@ -356,7 +373,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_kernel(TreeArgs a) {
         if (d == 0) {
           float* st = a.partial +
                       static_cast<int64_t>(a.B) * a.n_kv * a.splits * rows_all * D + rec * 2;
-          st[0] = m;
+          st[0] = mr;
           st[1] = l;
         }
       }
@@ -388,7 +405,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(TreeArgs a) {
     const int64_t rec = rec0 + static_cast<int64_t>(s) * rows_all;
     const float x = st[rec * 2];
     if (x == -INFINITY) continue;  // saw nothing: its sums are zeros
-    const float w = exp2f(x - m);
+    const float w = __builtin_amdgcn_exp2f(x - m);
     l += st[rec * 2 + 1] * w;
     const f4_t v = *reinterpret_cast<const f4_t*>(a.partial + rec * D + d);
 #pragma unroll
@@ -426,12 +443,11 @@ int plan_tree(int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv, int6
   if (batch == 0 || tokens == 0) return NIBBLE_OK;
   const int64_t rows = tokens * (n_heads / n_kv);
   NIBBLE_CHECK(rows * batch * n_kv <= (int64_t(1) << 30), "more than 2^30 query rows");
-  p->qt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  p->wk = rows <= 64 ? 4 : rows <= 128 ? 2 : 1;
+  p->qt = rows <= 16 ? 1 : 2;
+  p->wk = rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
   p->rows = 16 * p->qt * (4 / p->wk);
   p->row_tiles = static_cast<int>(ceil_div(rows, p->rows));
   const int64_t units = batch * n_kv * p->row_tiles;
-  NIBBLE_CHECK(units < (int64_t(1) << 31), "too many query rows");
   // As many splits as make two rounds of the CUs, each of two tiles at least.
   const int64_t tiles = ceil_div(std::max<int64_t>(max_seq, 1), kTreeKeys);
   int64_t splits = std::min<int64_t>({ceil_div(512, units), ceil_div(tiles, 2), kTreeMaxSplits});
@@ -443,12 +459,12 @@ int plan_tree(int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv, int6
 
 template <class E, int D>
 hipError_t launch_tree(const TreeArgs& a, const TreePlan& p, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(a.B * a.n_kv * p.row_tiles), static_cast<unsigned>(p.splits));
+  const int64_t pairs = static_cast<int64_t>(a.B) * a.n_kv * p.splits;
+  const dim3 grid(static_cast<unsigned>(ceil_div(pairs, 8) * 8 * p.row_tiles));
   if (p.qt == 1) tree_kernel<E, D, 1, 4><<<grid, kTreeThreads, 0, stream>>>(a);
-  else if (p.qt == 2) tree_kernel<E, D, 2, 4><<<grid, kTreeThreads, 0, stream>>>(a);
-  else if (p.wk == 4) tree_kernel<E, D, 4, 4><<<grid, kTreeThreads, 0, stream>>>(a);
-  else if (p.wk == 2) tree_kernel<E, D, 4, 2><<<grid, kTreeThreads, 0, stream>>>(a);
-  else tree_kernel<E, D, 4, 1><<<grid, kTreeThreads, 0, stream>>>(a);
+  else if (p.wk == 4) tree_kernel<E, D, 2, 4><<<grid, kTreeThreads, 0, stream>>>(a);
+  else if (p.wk == 2) tree_kernel<E, D, 2, 2><<<grid, kTreeThreads, 0, stream>>>(a);
+  else tree_kernel<E, D, 2, 1><<<grid, kTreeThreads, 0, stream>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
   const int64_t rows = static_cast<int64_t>(a.B) * a.n_kv * a.T * a.qpk;
@@ -533,7 +549,8 @@ extern "C" int nibble_attention_tree(const void* Q, int64_t dtype, int64_t batch
   a.seq = static_cast<int>(max_seq);
   a.splits = p.splits;
   a.row_tiles = p.row_tiles;
-  a.scale = scale * kLog2e;
+  a.scale = scale == 0.0f ? 1.0f : std::fabs(scale) * kLog2e;
+  a.sign = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;
   const hipError_t e = dtype == 0 ? (head_dim == 64 ? launch_tree<Half, 64>(a, p, stream)
                                                     : launch_tree<Half, 128>(a, p, stream))
                                   : (head_dim == 64 ? launch_tree<Bfloat, 64>(a, p, stream)
