@@ -17,6 +17,7 @@
 // of two tiles in turn.  V is read transposed from LDS (ds_read_b64_tr_b16).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "nibble_common.h"
 #include "nibble_copy.h"
@@ -26,8 +27,9 @@ namespace nibble {
 namespace {
 
 constexpr int kTreeThreads = 256;
-constexpr int kTreeKeys = 64;  // keys of a tile
-constexpr int kTreeMaxSplits = 64;
+constexpr int kTreeKeys = 64;        // keys of a tile
+constexpr int kTreeMaxSplits = 64;   // of one sequence
+constexpr int kTreeWorkgroups = 512;  // two a CU
 constexpr float kLog2e = 1.4426950408889634f;
 // A query's reference maximum moves only when a score passes it by this much
 // (in powers of two): until then its probabilities stay below 2^8, which the
@@ -42,11 +44,12 @@ struct TreeArgs {
   const int32_t* sizes;    // [B] or null: T each
   const uint8_t* mask;     // [B or 1, T, T] or null: causal
   void* out;               // [B, T, n_heads, D]
-  float* partial;          // [B n_kv][splits][rows][D], then [..][2] (top, sum), when splits > 1
+  float* partial;          // [n_kv][shares][rows][D], then [..][2] (top, sum), when shares > 0
   int64_t kb, kh, ks, vb, vh, vs;
   int64_t mask_batch;  // bytes between two sequences' masks
   int B, T, n_heads, n_kv, qpk, seq;
-  int splits, row_tiles;
+  int shares, row_tiles;  // shares: 0 where no sequence's rows are split
+  bool fold;              // row tiles from both ends to the middle
   float scale;  // its magnitude times log2(e); 1 for a scale of zero
   float sign;   // its sign
 };
@@ -75,12 +78,6 @@ __device__ __forceinline__ float swap_max(float v) {
   const Pair b = swap_pair<16>(fmaxf(a.a, a.b));
   return fmaxf(b.a, b.b);
 }
-__device__ __forceinline__ float swap_sum(float v) {
-  const Pair a = swap_pair<32>(v);
-  const Pair b = swap_pair<16>(a.a + a.b);
-  return b.a + b.b;
-}
-
 // What of sequence b there is: cached tokens and tree tokens within the cache.
 struct TreeSpan {
   int len, live, total;
@@ -91,8 +88,76 @@ struct TreeSpan {
   }
 };
 
+// How the cached rows are split when there are fewer (sequence, kv head, row
+// tile)s than room for workgroups.  The lengths are on the GPU, so every wave
+// works it out alike: a share is at most `per` tiles of one sequence, and per is
+// the least for which all sequences' shares together are at most a.shares (about
+// the least: it grows by a 32nd a try).  Shares are numbered in the order of the
+// sequences.
+struct TreeShares {
+  int per = 0, found = -1, first = 0, count = 0;
+  // Finds sequence `b`'s shares (want_b), or the sequence that share `w` is of.
+  __device__ __forceinline__ TreeShares(const TreeArgs& a, bool want_b, int want) {
+    if (a.B == 1) {
+      const int all = tiles(a, 0);
+      per = max(max((all + a.shares - 1) / a.shares, (all + kTreeMaxSplits - 1) / kTreeMaxSplits), 1);
+      count = shares_of(a, 0);
+      found = want_b || want < count ? 0 : -1;
+      return;
+    }
+    const int lane = threadIdx.x & 63;
+    int most = 0;
+    int64_t total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      const int t = b0 + lane < a.B ? tiles(a, b0 + lane) : 0;
+      most = max(most, t);
+      total += t;
+    }
+    for (int x = 32; x > 0; x /= 2) {
+      most = max(most, __shfl_xor(most, x));
+      total += __shfl_xor(total, x);
+    }
+    most = __builtin_amdgcn_readfirstlane(most);
+    per = __builtin_amdgcn_readfirstlane(static_cast<int>((total + a.shares - 1) / a.shares));
+    per = max(max(per, (most + kTreeMaxSplits - 1) / kTreeMaxSplits), 1);
+    for (; per < most; per += max(1, per / 32)) {
+      int n = 0;
+      for (int b0 = 0; b0 < a.B; b0 += 64)
+        n += b0 + lane < a.B ? shares_of(a, b0 + lane) : 0;
+      for (int x = 32; x > 0; x /= 2) n += __shfl_xor(n, x);
+      if (__builtin_amdgcn_readfirstlane(n) <= a.shares) break;
+    }
+    int before = 0;
+    for (int b0 = 0; b0 < a.B && found < 0; b0 += 64) {
+      const int n = b0 + lane < a.B ? shares_of(a, b0 + lane) : 0;
+      int upto = n;
+#pragma unroll
+      for (int x = 1; x < 64; x *= 2) {
+        const int y = __shfl_up(upto, x);
+        if (lane >= x) upto += y;
+      }
+      const int start = before + upto - n;
+      const uint64_t hit = __ballot(want_b ? b0 + lane == want : want >= start && want < start + n);
+      if (hit != 0) {
+        const int at = __builtin_ctzll(hit);
+        found = b0 + at;
+        first = __builtin_amdgcn_readfirstlane(__shfl(start, at));
+        count = __builtin_amdgcn_readfirstlane(__shfl(n, at));
+      }
+      before += __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
+    }
+  }
+  static __device__ __forceinline__ int tiles(const TreeArgs& a, int b) {
+    return (TreeSpan(a, b).total + kTreeKeys - 1) / kTreeKeys;
+  }
+  // (A sequence without rows keeps a share, which writes that it saw nothing.)
+  __device__ __forceinline__ int shares_of(const TreeArgs& a, int b) const {
+    return max(1, (tiles(a, b) + per - 1) / per);
+  }
+};
+
 // One workgroup: 16 QT WQ query rows of one kv head (WQ = 4 / WK waves along
-// the rows, WK along the keys), one split of the cached rows, in tiles of 64
+// the rows, WK along the keys), one share of the cached rows, in tiles of 64
 // keys.  A tile's rows of k and v are copied straight into one of two LDS
 // buffers while the tile before it is computed; two workgroups share a CU, so
 // one's softmax runs beside the other's products.
@@ -100,16 +165,17 @@ template <class E, int D, int QT, int WK>
 __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   using T = typename E::type;
   using vec8 = typename E::vec8;
-  constexpr int WQ = 4 / WK, KT = kTreeKeys, ROWS = 16 * QT * WQ;
-  constexpr int KPW = KT / WK < 32 ? KT / WK : 32;    // keys of a wave's step: 16 or 32
-  constexpr int KS = KPW / 16, STEPS = KT / (KPW * WK);
+  constexpr int WQ = 4 / WK, ROWS = 16 * QT * WQ;
+  constexpr int KT = kTreeKeys, KPW = KT / WK, KS = KPW / 16;  // a wave's keys of a tile
+  constexpr int PS = (KS + 1) / 2;                    // products of 32 keys (or 16 and zeros)
   constexpr int UNITS = D / 8;                        // 16-byte units of a row
   constexpr int COPIES = KT * UNITS / kTreeThreads;   // of K or V, a wave and tile
   constexpr int CROWS = 64 / UNITS;                   // rows of a copy
   typedef short s4_t __attribute__((ext_vector_type(4)));
-  typedef short s8_t __attribute__((ext_vector_type(8)));
+  typedef unsigned short us4_t __attribute__((ext_vector_type(4)));
+  typedef unsigned short us8_t __attribute__((ext_vector_type(8)));
   typedef __attribute__((address_space(3))) s4_t lds4_t;
-  __shared__ __attribute__((aligned(16))) T kv[2][2][KT * D];  // buffer, k or v
+  __shared__ __attribute__((aligned(16))) T kv[2][2][KT * D];  // buffer; k, v
   __shared__ float stat[2][WK][WQ * QT * 16];
   static_assert(sizeof(kv) >= sizeof(float) * WK * WQ * 16 * D, "the sums fit");
 
@@ -117,47 +183,38 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int wq = wave / WK, wk = wave % WK;
   const int g = lane >> 4, c = lane & 15;
-  // Workgroup -> (sequence and kv head, split), row tile: the row tiles that
-  // read the same cache rows run on one XCD (id % 8) and share its L2.
+  // Workgroup -> (share, kv head), row tile: the row tiles that read the same
+  // cache rows run on one XCD (id % 8) and share its L2.  Without a mask the
+  // later row tiles are longer: longest first, or, where all are on the CUs at
+  // once, two a CU, each with its counterpart.
   const int slot = blockIdx.x >> 3;
   const int pair = slot / a.row_tiles * 8 + (blockIdx.x & 7);
-  if (pair >= a.B * a.n_kv * a.splits) return;
-  const int row_tile = a.row_tiles - 1 - slot % a.row_tiles;  // the longest of a run first
-  const int unit = pair / a.splits, split = pair - unit * a.splits;
-  const int b = unit / a.n_kv, h = unit - b * a.n_kv;
+  const int rt = slot % a.row_tiles;
+  const int row_tile = a.fold && rt >= (a.row_tiles + 1) / 2 ? rt - (a.row_tiles + 1) / 2
+                                                             : a.row_tiles - 1 - rt;
+  const int w = pair / a.n_kv, h = pair - w * a.n_kv;
+  int b = w, share = 0, per = 0x3fffffff;  // the whole sequence
+  if (a.shares > 0) {
+    if (w >= a.shares) return;
+    const TreeShares shares(a, false, w);
+    if (shares.found < 0) return;
+    b = shares.found, share = w - shares.first, per = shares.per;
+  } else if (w >= a.B) {
+    return;
+  }
   const TreeSpan span(a, b);
   const int rows_all = a.T * a.qpk, rows = span.live * a.qpk;
   const int r0 = row_tile * ROWS;
   const int rw = r0 + wq * 16 * QT;  // this wave's first row
 
-  // Keys up to `end` matter to this workgroup, of which this split takes
-  // [first, last), whole tiles of them.
+  // Keys up to `end` matter to this workgroup, of which it takes [first, last).
   int end = r0 < rows ? span.total : 0;
   if (a.mask == nullptr && end > 0)
     end = min(end, span.len + (min(r0 + ROWS, rows) - 1) / a.qpk + 1);
-  const int tiles = (end + KT - 1) / KT, per = (tiles + a.splits - 1) / a.splits;
-  const int first = min(split * per, tiles) * KT, last = min(end, min((split + 1) * per, tiles) * KT);
-
-  const T* const kbase = static_cast<const T*>(a.k) + b * a.kb + h * a.kh;
-  const T* const vbase = static_cast<const T*>(a.v) + b * a.vb + h * a.vh;
-  const uint32_t lds0 = lds_address(kv) + wave * COPIES * 1024u;
-  const uint32_t kpitch = static_cast<uint32_t>(a.ks) * 2u, vpitch = static_cast<uint32_t>(a.vs) * 2u;
-  constexpr uint32_t kTile = KT * D * 2;  // bytes of a tile of k or v
-  auto copy = [&](int key0, int buf) {
-    // Rows behind the sequence's last read as zeros.
-    const int here = last - key0;
-    const T* const kt = kbase + key0 * a.ks;
-    const T* const vt = vbase + key0 * a.vs;
-#pragma unroll
-    for (int u = 0; u < COPIES; ++u) {
-      const int r = (wave * COPIES + u) * CROWS + lane / UNITS;
-      const uint32_t unit16 = ((lane % UNITS) ^ tree_swizzle<UNITS>(r)) * 16u;
-      const uint32_t dst = lds0 + buf * 2 * kTile + u * 1024u;
-      lds_copy16(kt, 0x7fffffffu, dst, r < here ? r * kpitch + unit16 : kOutOfRange);
-      lds_copy16(vt, 0x7fffffffu, dst + kTile, r < here ? r * vpitch + unit16 : kOutOfRange);
-    }
-  };
-  if (first < last) copy(first, 0);
+  const int tiles = (end + KT - 1) / KT;
+  const int first = min(share * per, tiles) * KT;
+  const int last = min(end, min(share * per + per, tiles) * KT);
+  const int count = (last - first + KT - 1) / KT;  // tiles
 
   // Queries: lane (g, c) holds elements 32 s + 8 g .. + 7 of row c of a tile.
   vec8 q[QT][D / 32];
@@ -184,12 +241,36 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
           q[t][s][i] = static_cast<T>(static_cast<float>(q[t][s][i]) * a.sign);
   }
 
+  const T* const kbase = static_cast<const T*>(a.k) + b * a.kb + h * a.kh;
+  const T* const vbase = static_cast<const T*>(a.v) + b * a.vb + h * a.vh;
+  constexpr uint32_t kTile = KT * D * 2;  // bytes of a tile of k or v
+  const uint32_t lds0 = lds_address(kv) + wave * COPIES * 1024u;
+  // This wave's copies of tile i; rows behind the share's last, and whole tiles
+  // there, read as zeros.
+  auto copy = [&](int i) {
+    const int key0 = first + i * KT, here = last - key0, from = here > 0 ? key0 : 0;
+    const T* const kt = kbase + from * a.ks;
+    const T* const vt = vbase + from * a.vs;
+    const uint32_t dst = lds0 + (i & 1) * 2 * kTile;
+#pragma unroll
+    for (int u = 0; u < COPIES; ++u) {
+      const int r = (wave * COPIES + u) * CROWS + lane / UNITS;
+      const uint32_t unit16 = ((lane % UNITS) ^ tree_swizzle<UNITS>(r)) * 16u;
+      lds_copy16(kt, 0x7fffffffu, dst + u * 1024u,
+                 r < here ? r * static_cast<uint32_t>(a.ks) * 2u + unit16 : kOutOfRange);
+      lds_copy16(vt, 0x7fffffffu, dst + kTile + u * 1024u,
+                 r < here ? r * static_cast<uint32_t>(a.vs) * 2u + unit16 : kOutOfRange);
+    }
+  };
+  copy(0);
+
   f4_t acc[QT][D / 16];
-  float top[QT], sum[QT];  // of query c, top times the scale; sum over this lane's keys
+  float top[QT];  // of query c, times the scale
+  f4_t sum[QT];   // of the probabilities: four copies
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     top[t] = -INFINITY;
-    sum[t] = 0.0f;
+    sum[t] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) acc[t][d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
@@ -200,141 +281,223 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   const int krow = c * D * 2 + ((g ^ tree_swizzle<UNITS>(c)) * 16);
   const int vr = 4 * g + (c >> 2);
   const int vrow = vr * D * 2 + (((c >> 1 & 1) ^ tree_swizzle<UNITS>(vr)) * 16) + (c & 1) * 8;
-  int buf = 0;
-  for (int key0 = first; key0 < last; key0 += KT, buf ^= 1) {
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-    lds_barrier();
-    if (key0 + KT < last) copy(key0 + KT, buf ^ 1);
-    const char* const kt = reinterpret_cast<const char*>(kv[buf][0]);
-    const uint32_t vt = lds_address(kv[buf][1]);
+  struct Scores {
+    f4_t s[KS][QT];
+  };
+  auto multiply = [&](Scores& x, int i) {
+    const char* const kt = reinterpret_cast<const char*>(kv[i & 1][0]) + wk * KPW * D * 2;
 #pragma unroll
-    for (int st = 0; st < STEPS; ++st) {
-      const int kb = (st * WK + wk) * KPW;  // this step's first key in the tile
-      f4_t s[KS][QT];
+    for (int j = 0; j < KS; ++j) {
 #pragma unroll
-      for (int kt16 = 0; kt16 < KS; ++kt16) {
+      for (int ss = 0; ss < D / 32; ++ss) {
+        const vec8 ka = *reinterpret_cast<const vec8*>(kt + j * 16 * D * 2 + (krow ^ (64 * ss)));
 #pragma unroll
-        for (int t = 0; t < QT; ++t) s[kt16][t] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int ss = 0; ss < D / 32; ++ss) {
-          const vec8 ka = *reinterpret_cast<const vec8*>(kt + (kb + 16 * kt16) * D * 2 +
-                                                         (krow ^ (64 * ss)));
-#pragma unroll
-          for (int t = 0; t < QT; ++t) s[kt16][t] = E::mfma(ka, q[t][ss], s[kt16][t]);
-        }
-      }
-      const bool tail = key0 + kb + KPW > span.len;
-      if (tail) {
-        const int k0 = key0 + kb + 4 * g;  // key of s[0][.][0]
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4 * KS; ++i) {
-            const int key = k0 + 16 * (i / 4) + i % 4, other = key - span.len;
-            bool seen = key < last;
-            if (seen && other >= 0)
-              seen = a.mask == nullptr
-                         ? other <= node[t]
-                         : a.mask[b * a.mask_batch + static_cast<int64_t>(node[t]) * a.T + other] != 0;
-            if (!seen) s[i / 4][t][i % 4] = -INFINITY;
-          }
-      }
-      vec8 p[QT];
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        float m = s[0][t][0];
-#pragma unroll
-        for (int i = 1; i < 4 * KS; ++i) m = fmaxf(m, s[i / 4][t][i % 4]);
-        m = swap_max(m) * a.scale;
-        if (__any(m > top[t] + kTreeSlack)) {
-          const float up = fmaxf(m, top[t]);
-          const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - up);
-          top[t] = up;
-          sum[t] *= keep;
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t][d][i] *= keep;
-        }
-        const float base = top[t] == -INFINITY ? 0.0f : top[t];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float e = i < 4 * KS
-                              ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[i / 4 % KS][t][i % 4], a.scale, -base))
-                              : 0.0f;
-          sum[t] += e;
-          p[t][i] = static_cast<T>(e);
-        }
-      }
-      // A masked row's infinity or NaN must not meet its zero probability.
-      bool strange = false;
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d) {
-        s4_t v2[2] = {};
-#pragma unroll
-        for (int kt16 = 0; kt16 < KS; ++kt16)
-          v2[kt16] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (lds4_t*)(uintptr_t)(vt + (kb + 16 * kt16) * D * 2 + (vrow ^ (32 * d))));
-        s8_t vv = {v2[0][0], v2[0][1], v2[0][2], v2[0][3], v2[1][0], v2[1][1], v2[1][2], v2[1][3]};
-        if (tail) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if ((vv[i] & E::kExponent) == E::kExponent) {
-              strange = true;
-              vv[i] = 0;
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-          acc[t][d] = E::mfma(__builtin_bit_cast(vec8, vv), p[t], acc[t][d]);
-      }
-      if (tail && __any(strange)) {
-        // Key by key, the rows that see the key only.
-        for (int kk = 0; kk < KPW; ++kk) {
-          const int from = (kk % 16 / 4) * 16 + c, i = kk / 16 * 4 + kk % 4;
-          const int r = kb + kk;
-#pragma unroll
-          for (int t = 0; t < QT; ++t) {
-            float w = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (e == i) w = static_cast<float>(p[t][e]);
-            w = __shfl(w, from);
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int dim = 16 * d + 4 * g + e;
-                const T x = kv[buf][1][r * D + ((dim / 8) ^ tree_swizzle<UNITS>(r)) * 8 + dim % 8];
-                const bool odd = (__builtin_bit_cast(unsigned short, x) & E::kExponent) == E::kExponent;
-                if (odd && w != 0.0f) acc[t][d][e] += w * static_cast<float>(x);
-              }
-          }
-        }
+        for (int t = 0; t < QT; ++t) x.s[j][t] = E::mfma(ka, q[t][ss], ss == 0 ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : x.s[j][t]);
       }
     }
-  }
+  };
+  auto hide = [&](Scores& x, int i) {  // what a query does not see
+    const int k0 = first + i * KT + wk * KPW + 4 * g;  // key of s[0][.][0]
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      bool seen[4 * KS];
+      if (a.mask != nullptr) {
+        // (Every byte is loaded, from a place in the mask, before any is used.)
+        const uint8_t* const row = a.mask + b * a.mask_batch + static_cast<int64_t>(node[t]) * a.T;
+        uint8_t byte[4 * KS];
+#pragma unroll
+        for (int e = 0; e < 4 * KS; ++e)
+          byte[e] = row[min(max(k0 + 16 * (e / 4) + e % 4 - span.len, 0), a.T - 1)];
+#pragma unroll
+        for (int e = 0; e < 4 * KS; ++e) seen[e] = byte[e] != 0;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4 * KS; ++e) seen[e] = k0 + 16 * (e / 4) + e % 4 - span.len <= node[t];
+      }
+#pragma unroll
+      for (int e = 0; e < 4 * KS; ++e) {
+        const int key = k0 + 16 * (e / 4) + e % 4;
+        if (!(key < last && (key < span.len || seen[e]))) x.s[e / 4][t][e % 4] = -INFINITY;
+      }
+    }
+  };
+  float m[QT];  // the largest score of a query, times the scale
+  auto largest = [&](const Scores& x) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      m[t] = x.s[0][t][0];
+#pragma unroll
+      for (int i = 1; i < 4 * KS; ++i) m[t] = fmaxf(m[t], x.s[i / 4][t][i % 4]);
+      m[t] = swap_max(m[t]) * a.scale;
+    }
+  };
+  auto move = [&]() {
+    bool moves = false;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) moves |= m[t] > top[t] + kTreeSlack;
+    if (!__any(moves)) return;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const float up = fmaxf(m[t], top[t]);
+      const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - up);
+      top[t] = up;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[t][i] *= keep;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][d][i] *= keep;
+    }
+  };
+  vec8 p[PS][QT], ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = static_cast<T>(1.0f);
+  auto weigh = [&](const Scores& x) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const float base = top[t] == -INFINITY ? 0.0f : top[t];
+#pragma unroll
+      for (int i = 0; i < 8 * PS; ++i) {
+        p[i / 8][t][i % 8] = static_cast<T>(
+            i < 4 * KS ? __builtin_amdgcn_exp2f(
+                             __builtin_fmaf(x.s[i / 4 % KS][t][i % 4], a.scale, -base))
+                       : 0.0f);
+      }
+      // The sum of the probabilities as they are multiplied, by the matrix cores
+      // too: ones times P^T, a tile's keys at once, in fp32.
+#pragma unroll
+      for (int j = 0; j < PS; ++j) sum[t] = E::mfma(ones, p[j][t], sum[t]);
+    }
+  };
+  // Whether this wave's v rows of a tile hold an infinity or a NaN.
+  auto strange = [&](int i) {
+    const u4_t* const vt = reinterpret_cast<const u4_t*>(kv[i & 1][1] + wk * KPW * D);
+    us8_t most = {};
+#pragma unroll
+    for (int e = 0; e < KPW * UNITS / 64; ++e) {
+      const u4_t bits = vt[e * 64 + lane] & 0x7fff7fffu;
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(us8_t, bits));
+    }
+    bool odd = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) odd |= most[e] >= E::kExponent;
+    return __any(odd) != 0;
+  };
+  // V^T of 32 keys (16 where a wave has no more) for 16 elements.
+  auto values = [&](uint32_t vt, int d, int j) {
+    s4_t v2[2] = {};
+#pragma unroll
+    for (int e = 0; e < (KS == 1 ? 1 : 2); ++e)
+      v2[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds4_t*)(uintptr_t)(vt + (2 * j + e) * 16 * D * 2 + (vrow ^ (32 * d))));
+    return us8_t(__builtin_shufflevector(__builtin_bit_cast(us4_t, v2[0]),
+                                         __builtin_bit_cast(us4_t, v2[1]), 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  // The sums.  A hidden row's infinity or NaN must not meet its zero
+  // probability: with `careful` they are left out of the products and counted,
+  // over the rows a query gives any weight, by products of their own: infinities
+  // of either sign, a NaN as both.  A query and element that met one gets that
+  // infinity added, and of both the NaN that they make.
+  auto add = [&](int i, auto careful) {
+    constexpr bool kCareful = decltype(careful)::value;
+    const uint32_t vt = lds_address(kv[i & 1][1]) + wk * KPW * D * 2;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+      for (int j = 0; j < PS; ++j) {
+        us8_t v = values(vt, d, j);
+        if constexpr (kCareful) v = (v & E::kExponent) == E::kExponent ? us8_t{} : v;
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+          acc[t][d] = E::mfma(__builtin_bit_cast(vec8, v), p[j][t], acc[t][d]);
+        if constexpr (kCareful) __builtin_amdgcn_sched_barrier(0);  // one at a time: registers
+      }
+    if constexpr (kCareful) {
+#pragma unroll
+      for (int j = 0; j < PS; ++j)
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            p[j][t][e] = static_cast<T>(static_cast<float>(p[j][t][e]) != 0.0f ? 1.0f : 0.0f);
+      const us8_t one = __builtin_bit_cast(us8_t, ones);
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int sign = 0; sign < 2; ++sign) {
+          f4_t n[QT] = {};
+#pragma unroll
+          for (int j = 0; j < PS; ++j) {
+            const us8_t v = values(vt, d, j);
+            const us8_t inf = us8_t{} + static_cast<unsigned short>(E::kExponent | sign << 15);
+            const us8_t is = v == inf || (v & 0x7fff) > E::kExponent ? one : us8_t{};
+#pragma unroll
+            for (int t = 0; t < QT; ++t) n[t] = E::mfma(__builtin_bit_cast(vec8, is), p[j][t], n[t]);
+          }
+          const float met = sign == 0 ? INFINITY : -INFINITY;
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[t][d][e] += n[t][e] != 0.0f ? met : 0.0f;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+  };
+  auto turn = [&](int i, auto tail) {
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    lds_barrier();
+    copy(i + 1);
+    Scores x;
+    multiply(x, i);
+    if constexpr (decltype(tail)::value) hide(x, i);
+    largest(x);
+    move();
+    weigh(x);
+    if constexpr (decltype(tail)::value) {
+      if (strange(i)) {
+        add(i, std::true_type{});
+        return;
+      }
+    }
+    add(i, std::false_type{});
+    // Eight reads of v, the exponentials, then each read two pairs of products
+    // ahead of its own.
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+    __builtin_amdgcn_sched_group_barrier(0x402, 64 * PS * QT, 0);
+#pragma unroll
+    for (int n = 0; n < PS * (D / 16 + 1); ++n) {
+      __builtin_amdgcn_sched_group_barrier(0x008, QT, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+  };
+  // A tile with rows that some query does not see, or behind the last, is a tail.
+  const int common = a.mask != nullptr ? span.len : span.len + r0 / a.qpk + 1;
+  const int plain = max(0, min(common, last) - first) / KT;
+  int i = 0;
+  for (; i < plain; ++i) turn(i, std::false_type{});
+  for (; i < count; ++i) turn(i, std::true_type{});
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // no copy may land in what follows
   __syncthreads();
 
   // The waves along the keys meet: statistics first, then the sums on the
   // common maximum, 16 rows of each wave at a time through LDS.
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    sum[t] = swap_sum(sum[t]);
-    if (rw + 16 * t + c >= rows) top[t] = -INFINITY, sum[t] = 0.0f;  // behind the last token
+    const bool behind = rw + 16 * t + c >= rows;  // the last token
+    if (behind) top[t] = -INFINITY;
     if (g == 0) {
       stat[0][wk][(wq * QT + t) * 16 + c] = top[t];
-      stat[1][wk][(wq * QT + t) * 16 + c] = sum[t];
+      stat[1][wk][(wq * QT + t) * 16 + c] = behind ? 0.0f : sum[t][0];
     }
   }
   __syncthreads();
   float* const red = reinterpret_cast<float*>(&kv[0][0][0]);  // [WK][WQ 16][D]
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    float m = stat[0][0][(wq * QT + t) * 16 + c];
+    float high = stat[0][0][(wq * QT + t) * 16 + c];
 #pragma unroll
-    for (int w = 1; w < WK; ++w) m = fmaxf(m, stat[0][w][(wq * QT + t) * 16 + c]);
-    const float mine = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[t] - m);
+    for (int w = 1; w < WK; ++w) high = fmaxf(high, stat[0][w][(wq * QT + t) * 16 + c]);
+    const float mine = high == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[t] - high);
 #pragma unroll
     for (int d = 0; d < D / 16; ++d)
 #pragma unroll
@@ -358,7 +521,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
       for (int w = 0; w < WK; ++w)
         l += mr == -INFINITY ? 0.0f
                              : stat[1][w][slot16] * __builtin_amdgcn_exp2f(stat[0][w][slot16] - mr);
-      if (a.splits == 1) {
+      if (a.shares == 0) {
         const int i = r / a.qpk;
         T* out = static_cast<T*>(a.out) +
                  ((static_cast<int64_t>(b) * a.T + i) * a.n_heads + h * a.qpk + (r - i * a.qpk)) * D + d;
@@ -368,11 +531,11 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
         for (int x = 0; x < 4; ++x) y[x] = static_cast<T>(l == 0.0f ? 0.0f : o[x] / l);
         *reinterpret_cast<vec4*>(out) = y;
       } else {
-        const int64_t rec = (static_cast<int64_t>(unit) * a.splits + split) * rows_all + r;
-        *reinterpret_cast<f4_t*>(a.partial + rec * D + d) = o;
+        const int64_t rec = (static_cast<int64_t>(h) * a.shares + w) * rows_all + r;
+        if (mr != -INFINITY) *reinterpret_cast<f4_t*>(a.partial + rec * D + d) = o;
         if (d == 0) {
           float* st = a.partial +
-                      static_cast<int64_t>(a.B) * a.n_kv * a.splits * rows_all * D + rec * 2;
+                      static_cast<int64_t>(a.n_kv) * a.shares * rows_all * D + rec * 2;
           st[0] = mr;
           st[1] = l;
         }
@@ -382,37 +545,65 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   }
 }
 
-// Joins the splits of a row: one group of D / 4 lanes a row.
+// Joins the shares of a row: D / 4 lanes a row, four outputs each, the rows of
+// one (sequence, kv head) in a workgroup.  The lanes read the shares' statistics
+// together; the sums are then loaded eight shares at a time, those of shares
+// that saw nothing not at all.
 template <class E, int D>
 __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(TreeArgs a) {
   using T = typename E::type;
+  constexpr int LANES = D / 4, PER = kTreeMaxSplits / LANES;  // splits a lane looks at
   const int rows_all = a.T * a.qpk;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kTreeThreads / (D / 4)) +
-                      threadIdx.x / (D / 4);
-  const int64_t units = static_cast<int64_t>(a.B) * a.n_kv;
-  if (row >= units * rows_all) return;
-  const int d = threadIdx.x % (D / 4) * 4;
-  const int64_t unit = row / rows_all;
-  const int r = static_cast<int>(row - unit * rows_all);
-  const float* st = a.partial + units * a.splits * rows_all * D;
-  const int64_t rec0 = unit * a.splits * rows_all + r;
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s)
-    m = fmaxf(m, st[(rec0 + static_cast<int64_t>(s) * rows_all) * 2]);
-  f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-  float l = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t rec = rec0 + static_cast<int64_t>(s) * rows_all;
-    const float x = st[rec * 2];
-    if (x == -INFINITY) continue;  // saw nothing: its sums are zeros
-    const float w = __builtin_amdgcn_exp2f(x - m);
-    l += st[rec * 2 + 1] * w;
-    const f4_t v = *reinterpret_cast<const f4_t*>(a.partial + rec * D + d);
+  const int parts = (rows_all + kTreeThreads / LANES - 1) / (kTreeThreads / LANES);
+  const int unit = blockIdx.x / parts;
+  const int b = unit / a.n_kv, h = unit - b * a.n_kv;
+  const int at = (blockIdx.x - unit * parts) * (kTreeThreads / LANES) + threadIdx.x / LANES;
+  const bool in = at < rows_all;
+  const int r = in ? at : 0;  // (lanes without a row shuffle along)
+  const int lane = threadIdx.x % LANES, d = lane * 4;
+  const TreeShares shares(a, true, b);
+  const float* const st = a.partial + static_cast<int64_t>(a.n_kv) * a.shares * rows_all * D;
+  const int64_t rec0 = (static_cast<int64_t>(h) * a.shares + shares.first) * rows_all + r;
+  float tops[PER], w[PER], m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] += v[i] * w;
+  for (int u = 0; u < PER; ++u) {
+    const int s = u * LANES + lane;
+    const float* p = st + (rec0 + static_cast<int64_t>(s) * rows_all) * 2;
+    tops[u] = s < shares.count ? p[0] : -INFINITY;
+    w[u] = s < shares.count ? p[1] : 0.0f;
+    m = fmaxf(m, tops[u]);
   }
+#pragma unroll
+  for (int x = LANES / 2; x > 0; x /= 2) m = fmaxf(m, __shfl_xor(m, x, LANES));
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    const float keep = tops[u] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(tops[u] - m);
+    l += w[u] * keep;
+    w[u] = keep;
+  }
+#pragma unroll
+  for (int x = LANES / 2; x > 0; x /= 2) l += __shfl_xor(l, x, LANES);
+  f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int u = 0; u < PER; ++u)
+    for (int s0 = 0; s0 < LANES && u * LANES + s0 < shares.count; s0 += 8) {
+      f4_t v[8];
+      float k[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        k[e] = __shfl(w[u], s0 + e, LANES);
+        v[e] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        if (k[e] != 0.0f)
+          v[e] = *reinterpret_cast<const f4_t*>(
+              a.partial + (rec0 + static_cast<int64_t>(u * LANES + s0 + e) * rows_all) * D + d);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] += v[e][i] * k[e];
+    }
+  if (!in) return;
   const int i = r / a.qpk;
-  const int b = static_cast<int>(unit / a.n_kv), h = static_cast<int>(unit - b * a.n_kv);
   typedef T vec4 __attribute__((ext_vector_type(4)));
   vec4 y;
 #pragma unroll
@@ -423,7 +614,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(TreeArgs a) {
 }
 
 struct TreePlan {
-  int qt = 1, wk = 4, rows = 16, row_tiles = 1, splits = 1;
+  int form = 0, rows = 16, row_tiles = 1, shares = 0;
   size_t workspace_bytes = 0;
 };
 
@@ -443,33 +634,32 @@ int plan_tree(int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv, int6
   if (batch == 0 || tokens == 0) return NIBBLE_OK;
   const int64_t rows = tokens * (n_heads / n_kv);
   NIBBLE_CHECK(rows * batch * n_kv <= (int64_t(1) << 30), "more than 2^30 query rows");
-  p->qt = rows <= 16 ? 1 : 2;
-  p->wk = rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
-  p->rows = 16 * p->qt * (4 / p->wk);
+  p->form = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
+  p->rows = 16 << p->form;
   p->row_tiles = static_cast<int>(ceil_div(rows, p->rows));
-  const int64_t units = batch * n_kv * p->row_tiles;
-  // As many splits as make two rounds of the CUs, each of two tiles at least.
-  const int64_t tiles = ceil_div(std::max<int64_t>(max_seq, 1), kTreeKeys);
-  int64_t splits = std::min<int64_t>({ceil_div(512, units), ceil_div(tiles, 2), kTreeMaxSplits});
-  p->splits = static_cast<int>(std::max<int64_t>(splits, 1));
-  if (p->splits > 1)
-    p->workspace_bytes = static_cast<size_t>(batch * n_kv * p->splits * rows) * (head_dim + 2) * 4;
+  // Room for more workgroups than there are (sequence, kv head, row tile)s: the
+  // cached rows are split, unless there are but a few tiles of them.
+  const int64_t room = kTreeWorkgroups / (n_kv * p->row_tiles);
+  if (room > batch && max_seq > 4 * kTreeKeys) {
+    p->shares = static_cast<int>(room);
+    p->workspace_bytes = static_cast<size_t>(n_kv * room * rows) * (head_dim + 2) * 4;
+  }
   return NIBBLE_OK;
 }
 
 template <class E, int D>
 hipError_t launch_tree(const TreeArgs& a, const TreePlan& p, hipStream_t stream) {
-  const int64_t pairs = static_cast<int64_t>(a.B) * a.n_kv * p.splits;
+  const int64_t pairs = static_cast<int64_t>(p.shares > 0 ? p.shares : a.B) * a.n_kv;
   const dim3 grid(static_cast<unsigned>(ceil_div(pairs, 8) * 8 * p.row_tiles));
-  if (p.qt == 1) tree_kernel<E, D, 1, 4><<<grid, kTreeThreads, 0, stream>>>(a);
-  else if (p.wk == 4) tree_kernel<E, D, 2, 4><<<grid, kTreeThreads, 0, stream>>>(a);
-  else if (p.wk == 2) tree_kernel<E, D, 2, 2><<<grid, kTreeThreads, 0, stream>>>(a);
+  if (p.form == 0) tree_kernel<E, D, 1, 4><<<grid, kTreeThreads, 0, stream>>>(a);
+  else if (p.form == 1) tree_kernel<E, D, 2, 4><<<grid, kTreeThreads, 0, stream>>>(a);
+  else if (p.form == 2) tree_kernel<E, D, 2, 2><<<grid, kTreeThreads, 0, stream>>>(a);
   else tree_kernel<E, D, 2, 1><<<grid, kTreeThreads, 0, stream>>>(a);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.splits == 1) return e;
-  const int64_t rows = static_cast<int64_t>(a.B) * a.n_kv * a.T * a.qpk;
-  tree_join_kernel<E, D><<<dim3(static_cast<unsigned>(ceil_div(rows, kTreeThreads / (D / 4)))),
-                           kTreeThreads, 0, stream>>>(a);
+  if (e != hipSuccess || p.shares == 0) return e;
+  const int64_t parts = ceil_div(static_cast<int64_t>(a.T) * a.qpk, kTreeThreads / (D / 4));
+  tree_join_kernel<E, D><<<dim3(static_cast<unsigned>(a.B * a.n_kv * parts)), kTreeThreads, 0,
+                           stream>>>(a);
   return hipGetLastError();
 }
 
@@ -547,8 +737,9 @@ extern "C" int nibble_attention_tree(const void* Q, int64_t dtype, int64_t batch
   a.n_kv = static_cast<int>(n_kv_heads);
   a.qpk = static_cast<int>(n_heads / n_kv_heads);
   a.seq = static_cast<int>(max_seq);
-  a.splits = p.splits;
+  a.shares = p.shares;
   a.row_tiles = p.row_tiles;
+  a.fold = mask == nullptr && batch * n_kv_heads * p.row_tiles <= kTreeWorkgroups;
   a.scale = scale == 0.0f ? 1.0f : std::fabs(scale) * kLog2e;
   a.sign = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;
   const hipError_t e = dtype == 0 ? (head_dim == 64 ? launch_tree<Half, 64>(a, p, stream)
