@@ -601,6 +601,8 @@ extern "C" int nibble_mx_matmul(const void* x_codes, const void* x_scales, int64
   if (rc != NIBBLE_OK) return rc;
   if (M == 0 || N == 0) return ok();
   NIBBLE_CHECK(M <= 65535 * 64, "more than %d rows of x", 65535 * 64);
+  NIBBLE_CHECK(ceil_div(M, 64) * ceil_div(N, 64) <= (1 << 30), "an output of %lld x %lld",
+               (long long)M, (long long)N);
   NIBBLE_CHECK(Y != nullptr, "null pointer");
   NIBBLE_CHECK(K == 0 || (x_codes != nullptr && x_scales != nullptr && w_codes != nullptr &&
                           w_scales != nullptr),

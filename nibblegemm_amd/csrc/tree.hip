@@ -45,6 +45,7 @@ struct TreeArgs {
   const uint8_t* mask;     // [B or 1, T, T] or null: causal
   void* out;               // [B, T, n_heads, D]
   float* partial;          // [n_kv][shares][rows][D], then [..][2] (top, sum), when shares > 0
+  int* runs;               // [B][2]: a sequence's first share and their number
   int64_t kb, kh, ks, vb, vh, vs;
   int64_t mask_batch;  // bytes between two sequences' masks
   int B, T, n_heads, n_kv, qpk, seq;
@@ -91,69 +92,74 @@ struct TreeSpan {
 // How the cached rows are split when there are fewer (sequence, kv head, row
 // tile)s than room for workgroups.  The lengths are on the GPU, so every wave
 // works it out alike: a share is at most `per` tiles of one sequence, and per is
-// the least for which all sequences' shares together are at most a.shares (about
-// the least: it grows by a 32nd a try).  Shares are numbered in the order of the
-// sequences.
+// (to a 16th) the least for which all sequences' shares together are at most
+// a.shares.  Shares are numbered in the order of the sequences, of which there
+// are fewer than a.shares; one without rows keeps a share, which writes that it
+// saw nothing.
 struct TreeShares {
+  static constexpr int kChunks = kTreeWorkgroups / 64;  // of sequences, one a lane
   int per = 0, found = -1, first = 0, count = 0;
-  // Finds sequence `b`'s shares (want_b), or the sequence that share `w` is of.
-  __device__ __forceinline__ TreeShares(const TreeArgs& a, bool want_b, int want) {
+  // Finds the sequence that share `want` is of, and that sequence's shares.
+  __device__ __forceinline__ TreeShares(const TreeArgs& a, int want) {
+    const int lane = threadIdx.x & 63;
+    int t[kChunks];  // tiles; 0 where there is no sequence
+    float most_f = 0.0f, total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      t[i] = 0;
+      if (64 * i < a.B) {
+        t[i] = 64 * i + lane < a.B ? tiles(a, 64 * i + lane) : 0;
+        most_f = fmaxf(most_f, static_cast<float>(t[i]));  // (below 2^24: exact)
+        total += static_cast<float>(t[i]);
+      }
+    }
+    const int most = static_cast<int>(wave_max(most_f));
+    per = static_cast<int>(ceilf(wave_sum(total) / static_cast<float>(a.shares)));
+    per = max(max(per, (most + kTreeMaxSplits - 1) / kTreeMaxSplits), 1);
+    per = __builtin_amdgcn_readfirstlane(per);
     if (a.B == 1) {
-      const int all = tiles(a, 0);
-      per = max(max((all + a.shares - 1) / a.shares, (all + kTreeMaxSplits - 1) / kTreeMaxSplits), 1);
-      count = shares_of(a, 0);
-      found = want_b || want < count ? 0 : -1;
+      count = shares_of(most);
+      found = want < count ? 0 : -1;
       return;
     }
-    const int lane = threadIdx.x & 63;
-    int most = 0;
-    int64_t total = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const int t = b0 + lane < a.B ? tiles(a, b0 + lane) : 0;
-      most = max(most, t);
-      total += t;
-    }
-    for (int x = 32; x > 0; x /= 2) {
-      most = max(most, __shfl_xor(most, x));
-      total += __shfl_xor(total, x);
-    }
-    most = __builtin_amdgcn_readfirstlane(most);
-    per = __builtin_amdgcn_readfirstlane(static_cast<int>((total + a.shares - 1) / a.shares));
-    per = max(max(per, (most + kTreeMaxSplits - 1) / kTreeMaxSplits), 1);
-    for (; per < most; per += max(1, per / 32)) {
+    int high = max(per, most);  // enough: one share each
+    for (int low = per; low < high;) {
+      const bool close = high - low <= low / 16;
+      const int mid = close ? low : low + (high - low) / 2;
       int n = 0;
-      for (int b0 = 0; b0 < a.B; b0 += 64)
-        n += b0 + lane < a.B ? shares_of(a, b0 + lane) : 0;
-      for (int x = 32; x > 0; x /= 2) n += __shfl_xor(n, x);
-      if (__builtin_amdgcn_readfirstlane(n) <= a.shares) break;
-    }
-    int before = 0;
-    for (int b0 = 0; b0 < a.B && found < 0; b0 += 64) {
-      const int n = b0 + lane < a.B ? shares_of(a, b0 + lane) : 0;
-      int upto = n;
 #pragma unroll
-      for (int x = 1; x < 64; x *= 2) {
-        const int y = __shfl_up(upto, x);
-        if (lane >= x) upto += y;
-      }
-      const int start = before + upto - n;
-      const uint64_t hit = __ballot(want_b ? b0 + lane == want : want >= start && want < start + n);
-      if (hit != 0) {
-        const int at = __builtin_ctzll(hit);
-        found = b0 + at;
-        first = __builtin_amdgcn_readfirstlane(__shfl(start, at));
-        count = __builtin_amdgcn_readfirstlane(__shfl(n, at));
-      }
-      before += __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
+      for (int i = 0; i < kChunks; ++i)
+        if (64 * i < a.B) n += 64 * i + lane < a.B ? max(1, (t[i] + mid - 1) / mid) : 0;
+      if (wave_sum(static_cast<float>(n)) <= static_cast<float>(a.shares)) high = mid;
+      else low = close ? high : mid + 1;
     }
+    per = high;
+    int before = 0;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i)
+      if (64 * i < a.B && found < 0) {
+        const int n = 64 * i + lane < a.B ? shares_of(t[i]) : 0;
+        int upto = n;
+#pragma unroll
+        for (int x = 1; x < 64; x *= 2) {
+          const int y = __shfl_up(upto, x);
+          if (lane >= x) upto += y;
+        }
+        const int start = before + upto - n;
+        const uint64_t hit = __ballot(want >= start && want < start + n);
+        if (hit != 0) {
+          const int at = __builtin_ctzll(hit);
+          found = 64 * i + at;
+          first = __builtin_amdgcn_readlane(start, at);
+          count = __builtin_amdgcn_readlane(n, at);
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+      }
   }
   static __device__ __forceinline__ int tiles(const TreeArgs& a, int b) {
     return (TreeSpan(a, b).total + kTreeKeys - 1) / kTreeKeys;
   }
-  // (A sequence without rows keeps a share, which writes that it saw nothing.)
-  __device__ __forceinline__ int shares_of(const TreeArgs& a, int b) const {
-    return max(1, (tiles(a, b) + per - 1) / per);
-  }
+  __device__ __forceinline__ int shares_of(int t) const { return max(1, (t + per - 1) / per); }
 };
 
 // One workgroup: 16 QT WQ query rows of one kv head (WQ = 4 / WK waves along
@@ -196,9 +202,12 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   int b = w, share = 0, per = 0x3fffffff;  // the whole sequence
   if (a.shares > 0) {
     if (w >= a.shares) return;
-    const TreeShares shares(a, false, w);
+    const TreeShares shares(a, w);
     if (shares.found < 0) return;
     b = shares.found, share = w - shares.first, per = shares.per;
+    // (for the kernel that joins them)
+    if (share == 0 && h == 0 && rt == 0 && threadIdx.x == 0)
+      a.runs[2 * b] = shares.first, a.runs[2 * b + 1] = shares.count;
   } else if (w >= a.B) {
     return;
   }
@@ -485,6 +494,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   for (int t = 0; t < QT; ++t) {
     const bool behind = rw + 16 * t + c >= rows;  // the last token
     if (behind) top[t] = -INFINITY;
+    else if (top[t] == -INFINITY && sum[t][0] != 0.0f) top[t] = 0.0f;  // NaN scores alone
     if (g == 0) {
       stat[0][wk][(wq * QT + t) * 16 + c] = top[t];
       stat[1][wk][(wq * QT + t) * 16 + c] = behind ? 0.0f : sum[t][0];
@@ -561,16 +571,16 @@ __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(TreeArgs a) {
   const bool in = at < rows_all;
   const int r = in ? at : 0;  // (lanes without a row shuffle along)
   const int lane = threadIdx.x % LANES, d = lane * 4;
-  const TreeShares shares(a, true, b);
+  const int first = a.runs[2 * b], count = a.runs[2 * b + 1];
   const float* const st = a.partial + static_cast<int64_t>(a.n_kv) * a.shares * rows_all * D;
-  const int64_t rec0 = (static_cast<int64_t>(h) * a.shares + shares.first) * rows_all + r;
+  const int64_t rec0 = (static_cast<int64_t>(h) * a.shares + first) * rows_all + r;
   float tops[PER], w[PER], m = -INFINITY, l = 0.0f;
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     const int s = u * LANES + lane;
     const float* p = st + (rec0 + static_cast<int64_t>(s) * rows_all) * 2;
-    tops[u] = s < shares.count ? p[0] : -INFINITY;
-    w[u] = s < shares.count ? p[1] : 0.0f;
+    tops[u] = s < count ? p[0] : -INFINITY;
+    w[u] = s < count ? p[1] : 0.0f;
     m = fmaxf(m, tops[u]);
   }
 #pragma unroll
@@ -586,7 +596,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(TreeArgs a) {
   f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int u = 0; u < PER; ++u)
-    for (int s0 = 0; s0 < LANES && u * LANES + s0 < shares.count; s0 += 8) {
+    for (int s0 = 0; s0 < LANES && u * LANES + s0 < count; s0 += 8) {
       f4_t v[8];
       float k[8];
 #pragma unroll
@@ -640,9 +650,10 @@ int plan_tree(int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv, int6
   // Room for more workgroups than there are (sequence, kv head, row tile)s: the
   // cached rows are split, unless there are but a few tiles of them.
   const int64_t room = kTreeWorkgroups / (n_kv * p->row_tiles);
-  if (room > batch && max_seq > 4 * kTreeKeys) {
+  if (room > batch && batch < 64 * TreeShares::kChunks && max_seq > 4 * kTreeKeys) {
     p->shares = static_cast<int>(room);
-    p->workspace_bytes = static_cast<size_t>(n_kv * room * rows) * (head_dim + 2) * 4;
+    p->workspace_bytes =
+        static_cast<size_t>(n_kv * room * rows) * (head_dim + 2) * 4 + static_cast<size_t>(batch) * 8;
   }
   return NIBBLE_OK;
 }
@@ -728,6 +739,8 @@ extern "C" int nibble_attention_tree(const void* Q, int64_t dtype, int64_t batch
   a.mask = static_cast<const uint8_t*>(mask);
   a.out = Out;
   a.partial = static_cast<float*>(workspace);
+  a.runs = reinterpret_cast<int*>(a.partial + static_cast<size_t>(n_kv_heads) * p.shares * tokens *
+                                              (n_heads / n_kv_heads) * (head_dim + 2));
   a.kb = k_batch_stride, a.kh = k_head_stride, a.ks = k_row_stride;
   a.vb = v_batch_stride, a.vh = v_head_stride, a.vs = v_row_stride;
   a.mask_batch = mask_batches == 1 ? 0 : tokens * tokens;

@@ -252,7 +252,8 @@ def test_tree_workspace():
     ext = ng.extension()
     assert ext.attention_tree_workspace_bytes(1, 16, 32, 8, 128, 128) == 0  # one tile of rows
     need = ext.attention_tree_workspace_bytes(1, 16, 32, 8, 128, 65536)
-    assert need > 0 and need % (8 * 64 * 130 * 4) == 0  # whole splits of (sums, top, sum)
+    # whole shares of (sums, top, sum), and where each sequence's begin
+    assert need > 0 and (need - 8) % (8 * 64 * 130 * 4) == 0
     assert ext.attention_tree_workspace_bytes(1, 16, 32, 8, 96, 65536) == 0  # a refused plan
     st = (8 * 65536 * 128, 65536 * 128, 128)
     big = dict(T=16, nh=32, nkv=8, S=65536, st=st)
@@ -423,6 +424,45 @@ def test_strange_values_in_rows_not_seen(T, n_heads, dtype):
         k[b, 0, n + T:], v[b, 0, n + T:] = nan, inf
     got = check_tree(q, k, v, lengths, mask, None)
     assert got.isnan().any() and got.isinf().any() and got.isfinite().all(-1).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths", [[3, 900], [700, 20]])
+def test_strange_values_seen_by_all(lengths, dtype):
+    """A NaN in a query is its own output's alone; infinities in cached rows
+    that every query sees come out where they belong."""
+    q, k, v, lengths, mask, _ = tree_case(2, 9, 4, 2, 128, 920, dtype, lengths, True)
+    q[0, 3, 1, 17] = float("nan")
+    q[1, 0, 2, 5] = float("nan")
+    v[1, 1, 2, 40], v[1, 1, 1, 41] = float("inf"), -float("inf")
+    k[0, 0, 1, 3] = float("nan")
+    got = check_tree(q, k, v, lengths, mask, None)
+    assert got[0, :, :2].isnan().all() and got[0, 2, 2:].isfinite().all()
+    assert got[1, 0, 2].isnan().all() and got[1, 1, 0].isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_kv,n_heads,B", [(1, 2, 70), (1, 1, 300), (2, 4, 33), (1, 3, 511)])
+def test_many_sequences_of_uneven_lengths(n_kv, n_heads, B):
+    """Shares of the cached rows by the lengths: one long sequence among many
+    short and empty ones, all alike, and all empty."""
+    S, T, D = 1500, 2, 64
+    g = torch.Generator().manual_seed(B)
+    q = torch.randn((B, T, n_heads, D), generator=g).to(F16)
+    k, v = (torch.randn((1, n_kv, S, D), generator=g).to(F16).expand(B, n_kv, S, D) for _ in range(2))
+    for kind in range(3):
+        lengths = torch.randint(0, 40, (B,), generator=g)
+        lengths[B // 2] = 1490
+        lengths[::7] = 0
+        if kind:
+            lengths[:] = 700 if kind == 1 else 0
+        sizes = torch.randint(0, T + 1, (B,), generator=g)
+        got = run_tree(q, k, v, lengths.int(), None, sizes.int()).cpu().double()
+        for b in sorted({0, 1, 6, 7, B // 2, B // 2 + 1, B - 1}):
+            want, bound = oracle_attention(q[b:b + 1], k[:1], v[:1], lengths[b:b + 1], None,
+                                           sizes[b:b + 1], D ** -0.5)
+            assert ((got[b:b + 1] - want).abs() <= bound).all(), (kind, b)
 
 
 @pytest.mark.gpu
