@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .ops import _call, _check_no_backward, _raise, _stream, _workspace, _ws_plan
@@ -133,6 +134,19 @@ def _check_half(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
         raise RuntimeError(f"{name} must hold its values as they are (resolve_neg)")
 
 
+def _in_order(dtype: torch.dtype, index: int, *tensors: Optional[torch.Tensor]) -> bool:
+    """Whether every tensor passes :func:`_check_half` beside one of this dtype
+    on this GPU, at a glance: the checks that name what is wrong take longer
+    than a small call's kernel."""
+    if index < 0 or dtype not in _HALF_DTYPES or getattr(forward_ad, "_current_level", -1) >= 0:
+        return False
+    for t in tensors:
+        if t is not None and (t.dtype is not dtype or t.get_device() != index or t.requires_grad
+                              or t.is_neg()):
+            return False
+    return True
+
+
 def _check_gpu(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
     if not t.is_cuda:
         raise RuntimeError(f"{name} must live on the GPU")
@@ -141,34 +155,35 @@ def _check_gpu(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
 
 
 def _check_index(name: str, t: torch.Tensor, shape, like: torch.Tensor) -> None:
+    if (t.dtype is torch.int32 and t.get_device() == like.get_device() and t.shape == shape
+            and t.is_contiguous()):
+        return
     _check_gpu(name, t, like)
     if t.dtype != torch.int32 or not t.is_contiguous():
         raise RuntimeError(f"{name} must be a contiguous int32 tensor")
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
 
 
-def _caches(x: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor):
-    """Checks the caches beside the tokens ``x`` ``[B, T, ..]`` or ``[T, ..]``
-    and returns both in the batched form."""
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _check_half(name, t, x)
-        if t.dim() != x.dim() + 1:
-            raise ValueError(f"{name} must have {x.dim() + 1} dimensions beside {x.dim()} of the "
-                             f"tokens, got {tuple(t.shape)}")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError(f"caches must have one shape, got {tuple(k_cache.shape)} and "
-                         f"{tuple(v_cache.shape)}")
-    if x.dim() == 2:
-        k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
-    elif k_cache.shape[0] != x.shape[0]:
-        raise ValueError(f"caches of {k_cache.shape[0]} sequences beside tokens of {x.shape[0]}")
-    if 0 in k_cache.shape[1:]:
-        raise ValueError(f"the caches are empty: {tuple(k_cache.shape)}")
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if t.stride(3) != 1:
-            raise RuntimeError(f"{name}: the elements of a row must be adjacent")
-    return k_cache, v_cache
+def _cache_strides(x: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor):
+    """Checks the caches' shapes beside the tokens ``x`` ``[B, T, ..]`` or
+    ``[T, ..]``: their batched shape, and the batch, head and row strides of
+    both."""
+    shape = k_cache.shape
+    if v_cache.shape != shape:
+        raise ValueError(f"caches must have one shape, got {tuple(shape)} and {tuple(v_cache.shape)}")
+    if len(shape) != x.dim() + 1:
+        raise ValueError(f"caches must have {x.dim() + 1} dimensions beside {x.dim()} of the tokens, "
+                         f"got {tuple(shape)}")
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if len(shape) == 3:
+        shape, ks, vs = (1, *shape), (0, *ks), (0, *vs)
+    elif shape[0] != x.shape[0]:
+        raise ValueError(f"caches of {shape[0]} sequences beside tokens of {x.shape[0]}")
+    if 0 in shape[1:]:
+        raise ValueError(f"the caches are empty: {tuple(shape)}")
+    if ks[3] != 1 or vs[3] != 1:
+        raise RuntimeError("the elements of a cache row must be adjacent")
+    return shape, ks, vs
 
 
 def qk_norm_rope(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -196,42 +211,45 @@ def qk_norm_rope(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     its batch dimension: qkv [T, ..] (and q so), caches [n_kv, max_seq, D],
     positions and slots [T].  Positions, slots and caches are read on the GPU,
     so a captured call follows their contents.  There is no backward."""
-    _check_half("qkv", qkv, qkv)
+    dtype, dev = qkv.dtype, qkv.device
+    if not _in_order(dtype, qkv.get_device(), qkv, k_cache, v_cache, q_weight, k_weight):
+        for name, t in (("qkv", qkv), ("k_cache", k_cache), ("v_cache", v_cache),
+                        ("q_weight", q_weight), ("k_weight", k_weight)):
+            if t is not None:
+                _check_half(name, t, qkv)
     if qkv.dim() not in (2, 3) or not qkv.is_contiguous():
         raise RuntimeError("qkv must be a contiguous [B, T, ..] or [T, ..] tensor")
-    k4, v4 = _caches(qkv, k_cache, v_cache)
-    for name, t in (("k_cache", k4), ("v_cache", v4)):
-        if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
-            raise RuntimeError(f"{name} is written and must not be an expanded view")
-    B, n_kv, max_seq, D = k4.shape
+    (B, n_kv, max_seq, D), ks, vs = _cache_strides(qkv, k_cache, v_cache)
+    for n, k, v in zip((B, n_kv, max_seq), ks, vs):
+        if n > 1 and (k == 0 or v == 0):
+            raise RuntimeError("the caches are written and must not be expanded views")
+    lead = qkv.shape[:-1]
     T, width = qkv.shape[-2:]
     n_heads = width // D - 2 * n_kv
     if width % D or n_heads < 1:
         raise ValueError(f"qkv must be [.., (n_heads + 2 * {n_kv}) * {D}], got {tuple(qkv.shape)}")
-    for name, t in (("positions", positions), ("slots", slots)):
-        _check_index(name, t, qkv.shape[:-1], qkv)
+    _check_index("positions", positions, lead, qkv)
+    _check_index("slots", slots, lead, qkv)
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if t is not None:
-            _check_half(name, t, qkv)
-            if t.shape != (D,) or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous [{D}] tensor, got {tuple(t.shape)}")
+        if t is not None and (t.shape != (D,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous [{D}] tensor, got {tuple(t.shape)}")
     cos_p = sin_p = None
     rope_rows = 0
     if rope is not None:
         cos, sin = rope
         for name, t in (("rope cos", cos), ("rope sin", sin)):
-            _check_gpu(name, t, qkv)
+            if t.get_device() != dev.index:
+                _check_gpu(name, t, qkv)
             _check_no_backward(name, t)
-            if t.dtype != torch.float32 or not t.is_contiguous():
+            if t.dtype is not torch.float32 or not t.is_contiguous():
                 raise RuntimeError(f"{name} must be a contiguous fp32 GPU tensor")
             if t.dim() != 2 or t.shape != (cos.shape[0], D // 2) or t.shape[0] < 1:
                 raise ValueError(f"{name} must be [rows, {D // 2}], got {tuple(t.shape)}")
         cos_p, sin_p, rope_rows = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-    ext = _native.binding()
-    out = torch.empty((*qkv.shape[:-1], n_heads * D), dtype=qkv.dtype, device=qkv.device)
-    _call(ext.qk_norm_rope, qkv.device, qkv.data_ptr(), _HALF_DTYPES[qkv.dtype], B, T, n_heads,
-          n_kv, D, k4.data_ptr(), *k4.stride()[:3], v4.data_ptr(), *v4.stride()[:3], max_seq,
-          positions.data_ptr(), slots.data_ptr(),
+    out = torch.empty((*lead, n_heads * D), dtype=dtype, device=dev)
+    _call(_native.binding().qk_norm_rope, dev, qkv.data_ptr(), _HALF_DTYPES[dtype], B, T, n_heads,
+          n_kv, D, k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
+          max_seq, positions.data_ptr(), slots.data_ptr(),
           q_weight.data_ptr() if q_weight is not None else None,
           k_weight.data_ptr() if k_weight is not None else None, float(eps), cos_p, sin_p,
           rope_rows, out.data_ptr())
@@ -264,11 +282,13 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     dimension: q [T, ..], caches [n_kv, max_seq, D], lengths [1], sizes [1].
     Lengths, sizes and mask are read on the GPU, so a captured call follows
     their contents.  There is no backward."""
-    _check_half("q", q, q)
+    dtype, dev = q.dtype, q.device
+    if not _in_order(dtype, q.get_device(), q, k_cache, v_cache):
+        for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache)):
+            _check_half(name, t, q)
     if q.dim() not in (2, 3) or not q.is_contiguous():
         raise RuntimeError("q must be a contiguous [B, T, ..] or [T, ..] tensor")
-    k4, v4 = _caches(q, k_cache, v_cache)
-    B, n_kv, max_seq, D = k4.shape
+    (B, n_kv, max_seq, D), ks, vs = _cache_strides(q, k_cache, v_cache)
     T, width = q.shape[-2:]
     n_heads = width // D
     if width % D:
@@ -278,23 +298,23 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         _check_index("sizes", sizes, (B,), q)
     mask_p, mask_batches = None, 1
     if mask is not None:
-        _check_gpu("mask", mask, q)
-        if mask.dtype != torch.bool or not mask.is_contiguous():
+        if mask.get_device() != dev.index:
+            _check_gpu("mask", mask, q)
+        if mask.dtype is not torch.bool or not mask.is_contiguous():
             raise RuntimeError("mask must be a contiguous bool tensor")
-        if tuple(mask.shape) not in ((T, T), (B, T, T)):
+        if mask.shape not in ((T, T), (B, T, T)):
             raise ValueError(f"mask must be [{T}, {T}] or [{B}, {T}, {T}], got {list(mask.shape)}")
         mask_p, mask_batches = mask.data_ptr(), B if mask.dim() == 3 else 1
     ext = _native.binding()
-    dev = q.device
     key = ("tree", B, T, n_heads, n_kv, D, max_seq)
-    nbytes = _ws_plan.get(key)
-    if nbytes is None:
-        nbytes = ext.attention_tree_workspace_bytes(B, T, n_heads, n_kv, D, max_seq)
-        _ws_plan[key] = nbytes
-    ws, ws_bytes = _workspace((nbytes, 0), dev, _stream(dev))
+    plan = _ws_plan.get(key)
+    if plan is None:
+        plan = (ext.attention_tree_workspace_bytes(B, T, n_heads, n_kv, D, max_seq), 0)
+        _ws_plan[key] = plan
+    ws, ws_bytes = _workspace(plan, dev, _stream(dev))
     out = torch.empty_like(q)
-    _call(ext.attention_tree, dev, q.data_ptr(), _HALF_DTYPES[q.dtype], B, T, n_heads, n_kv, D,
-          k4.data_ptr(), *k4.stride()[:3], v4.data_ptr(), *v4.stride()[:3], max_seq,
+    _call(ext.attention_tree, dev, q.data_ptr(), _HALF_DTYPES[dtype], B, T, n_heads, n_kv, D,
+          k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2], max_seq,
           lengths.data_ptr(), mask_p, mask_batches, sizes.data_ptr() if sizes is not None else None,
           float(D ** -0.5 if scale is None else scale), out.data_ptr(),
           ws.data_ptr() if ws is not None else None, ws_bytes)

@@ -85,6 +85,12 @@ def _check_k(K: int) -> None:
 
 def _check_mx(name: str, m: MXMatrix) -> None:
     _check_k(m.K)
+    codes, scales = m.codes, m.scales
+    if (codes.dtype is torch.uint8 and scales.dtype is torch.uint8
+            and codes.shape == (m.rows, m.K // 2) and scales.shape == (_groups(m.K), m.rows, 4)
+            and codes.is_contiguous() and scales.is_contiguous()
+            and codes.get_device() == scales.get_device()):
+        return
     for what, t, shape in (("codes", m.codes, (m.rows, m.K // 2)),
                            ("scales", m.scales, (_groups(m.K), m.rows, 4))):
         if t.dtype != torch.uint8:
@@ -193,22 +199,20 @@ def matmul_mx(x: Union[torch.Tensor, MXMatrix], w: MXMatrix,
     ``out_dtype`` (fp16, bf16 or fp32).  A dense ``x`` (fp16, bf16 or fp32) is
     quantised first, with :func:`quantize_mx`'s values, and gives its own dtype
     by default; an :class:`MXMatrix` fp16.  A NaN block makes the outputs of its
-    row NaN."""
+    row of ``x`` or of ``w`` NaN."""
     _check_mx("w", w)
     if not w.codes.is_cuda:
         raise RuntimeError("all tensors must live on the GPU")
-    dev = w.codes.device
     dense = isinstance(x, torch.Tensor)
     if dense:
         _check_values("x", x)
         M, K = x.shape
-        if x.device != dev:
-            raise RuntimeError("all tensors must live on the same device")
     else:
         _check_mx("x", x)
         M, K = x.rows, x.K
-        if x.codes.device != dev:
-            raise RuntimeError("all tensors must live on the same device")
+    if (x if dense else x.codes).get_device() != w.codes.get_device():
+        raise RuntimeError("all tensors must live on the same device")
+    dev = w.codes.device
     if K != w.K:
         raise RuntimeError(f"x has K={K}, the weight K={w.K}")
     if out_dtype is None:
