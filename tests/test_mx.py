@@ -219,8 +219,40 @@ def test_library_rejections(call, needle):
     assert needle in ext.last_error()
 
 
+def dense(ext, X=P, M=2, rs=128, xdt=0, wc=P, ws=P, N=64, K=128, dt=0, Y=P):
+    return ext.mx_matmul_dense(X, M, rs, xdt, wc, ws, N, K, dt, Y, None)
+
+
+@pytest.mark.parametrize("kwargs,needle,status", [
+    (dict(K=100), "multiple of 32", INVALID),
+    (dict(xdt=3), "dtype", INVALID),
+    (dict(dt=3), "dtype", INVALID),
+    (dict(M=-1), "negative", INVALID),
+    (dict(X=0), "null", INVALID),
+    (dict(ws=0), "null", INVALID),
+    (dict(rs=132), "16 bytes", INVALID),
+    (dict(X=P + 8), "16 bytes", INVALID),
+    (dict(rs=1 << 30), "2^31", INVALID),
+    (dict(wc=P + 8), "misaligned", INVALID),
+    (dict(M=17), "quantised first", 2),
+    (dict(N=1 << 20), "quantised first", 2),
+])
+def test_dense_rejections(kwargs, needle, status):
+    ext = ng.extension()
+    assert dense(ext, **kwargs) == status
+    assert needle in ext.last_error()
+
+
+def test_where_a_dense_x_is_taken():
+    takes = ng.extension().mx_matmul_takes_dense
+    assert takes(1, 1024, 4096) and takes(16, 4096, 4096) and takes(1, 12288, 32)
+    assert not takes(17, 1024, 4096) and not takes(1, 28672, 4096)
+    assert not takes(0, 1024, 4096) and not takes(1, 0, 4096) and not takes(1, 64, 0)
+
+
 def test_library_takes_empty_sizes():
     ext = ng.extension()
+    assert dense(ext, M=0, X=0) == 0 and dense(ext, N=0, wc=0) == 0
     assert quant(ext, rows=0, X=0) == 0 and quant(ext, K=0, X=0) == 0
     assert ext.mx_dequantize(0, 0, 0, 128, 0, 0, None) == 0
     assert prod(ext, M=0, xc=0) == 0 and prod(ext, N=0, wc=0) == 0
@@ -406,6 +438,36 @@ def test_nan_blocks_stay_in_their_rows(M, N):
     want[M // 2] = True
     want[:, N - 1] = True
     assert torch.equal(y.isnan(), want)
+
+
+@pytest.mark.gpu
+def test_matrices_beyond_32_bits():
+    """Weights of more than 2^31 bytes of codes, and values of more than 2^32
+    bytes quantised."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("not enough memory")
+    N, K = 600_000, 8192
+    g = torch.Generator(device=dev).manual_seed(0)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, device=dev, dtype=torch.uint8)
+    scales = torch.randint(120, 130, (K // 128, N, 4), generator=g, device=dev, dtype=torch.uint8)
+    w = mx.MXMatrix(codes, scales, N, K)
+    some = torch.tensor([0, 5, 262144, 599_000, N - 1], device=dev)
+    part = mx.MXMatrix(codes[some].contiguous(), scales[:, some].contiguous(), 5, K)
+    for M in (3, 70):
+        x = ng.quantize_mx(sample(M, K, F16, seed=M).to(dev))
+        y = ng.matmul_mx(x, w, F32)
+        check_product(y[:, some], values64(x), values64(part), F32)
+        del y
+    assert torch.equal(ng.dequantize_mx(w, F16)[some], ng.dequantize_mx(part, F16))
+    del w, codes, scales
+    v = torch.empty((300_000, K), dtype=F16, device=dev)  # 4.9 GB
+    v.normal_(generator=g)
+    rows = torch.tensor([0, 131072, 262143, 262144, 299_999], device=dev)
+    q = ng.quantize_mx(v)
+    want = ng.quantize_mx(v[rows].contiguous())
+    assert torch.equal(q.codes[rows], want.codes) and torch.equal(q.scales[:, rows], want.scales)
+    t = ng.quantize_mx(v[:, :4096].contiguous().t().contiguous().t())
+    assert torch.equal(t.codes[rows], want.codes[:, :2048])
 
 
 @pytest.mark.gpu
