@@ -35,7 +35,7 @@ struct MxElem {
                         : __builtin_bit_cast(float, static_cast<uint32_t>(v) << 16);
   }
   static __device__ __forceinline__ void load8(const type* p, float (&f)[8]) {
-    const us8_t v = __builtin_nontemporal_load(reinterpret_cast<const us8_t*>(p));
+    const us8_t v = *reinterpret_cast<const us8_t*>(p);
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = get(v[i]);
   }
@@ -45,8 +45,8 @@ struct MxElem<kMxF32> {
   using type = float;
   static __device__ __forceinline__ float get(float v) { return v; }
   static __device__ __forceinline__ void load8(const type* p, float (&f)[8]) {
-    const f4_t a = __builtin_nontemporal_load(reinterpret_cast<const f4_t*>(p));
-    const f4_t b = __builtin_nontemporal_load(reinterpret_cast<const f4_t*>(p) + 1);
+    const f4_t a = *reinterpret_cast<const f4_t*>(p);
+    const f4_t b = *(reinterpret_cast<const f4_t*>(p) + 1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = a[i], f[4 + i] = b[i];
   }
@@ -85,11 +85,14 @@ __device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
       __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false));
 }
 
-// Rows whose k are adjacent in memory.  A workgroup takes 32 rows of 512 k;
+// Rows whose k are adjacent in memory.  A workgroup takes 8 rows of 512 k;
 // wave w the k group w of them, 16 lanes a row: lane j holds k 8j .. 8j + 7,
 // four lanes a block.  The largest magnitude meets in the four lanes (DPP),
 // the four blocks' exponents in the row's first lane, which writes the word.
-constexpr int kMxRows = 32;
+// Memory bounds it: 28672 x 4096 in 53 us from fp16, 5.6 TB/s, and 91 from fp32
+// (54 and 95 with 16 rows, 57 and 90 with 4; 60 and 97 with 32 rows and loads
+// that pass by the caches, whose values the caches may hold).
+constexpr int kMxRows = 8;
 constexpr int kMxPasses = kMxRows / 4;
 
 template <int DT, bool VEC>
@@ -174,7 +177,7 @@ __global__ __launch_bounds__(256) void mx_quantize_t_kernel(const typename MxEle
     for (int i = 0; i < kMxBlock; ++i) {
       const typename E::type* x = X + (k0 + i) * ld + row;
       if (VEC) {
-        const pair_t v = row < rows ? __builtin_nontemporal_load(reinterpret_cast<const pair_t*>(x))
+        const pair_t v = row < rows ? *reinterpret_cast<const pair_t*>(x)
                                     : pair_t{};
         f[0][i] = E::get(v[0]);
         f[1][i] = E::get(v[1]);
@@ -226,36 +229,45 @@ __device__ __forceinline__ typename MxElem<DT>::type mx_out(float v) {
   }
 }
 
-// A code's value times the block's power of two, exact in 32 bits (down to
-// 2^-128; above 2^125 times 6 it overflows to infinity, as it should).
-__device__ __forceinline__ float mx_value(uint32_t code, uint32_t e) {
-  const uint32_t m = code & 7u;
-  // 2^(e2 - 1) (1 + m / 2), or m / 2 with a zero exponent
-  const float v = m < 2u ? 0.5f * static_cast<float>(m)
-                         : __builtin_bit_cast(float, ((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-  const float s = e == 255u ? __builtin_nanf("") : v * mx_power(e);
-  return code & 8u ? -s : s;
+// Two codes' values (byte B of a word) times the block's power of two: exact in
+// 32 bits (down to 2^-128; 2^126 times 4 or 6 is infinite, as it should be).
+typedef float f2_t __attribute__((ext_vector_type(2)));
+template <int B>
+__device__ __forceinline__ f2_t mx_values2(uint32_t codes, uint32_t e) {
+  const f2_t v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, mx_power(e), B);
+  return e == 255u ? f2_t{__builtin_nanf(""), __builtin_nanf("")} : v;
 }
 
-// Thread t expands eight codes: a word of them read, 16 or 32 bytes written.
+// A thread expands what 16 bytes of the output hold: eight codes, or four where
+// it has 32 bits.  Memory bounds it; what counts is that a wave's stores cover
+// 1 KiB without a gap and pass by the caches (28672 x 4096 in bf16: 43 us against
+// 60 with plain stores; in fp32 72 against 119, and 132 with 32 bytes a thread).
+// The grid has two dimensions because one ends at 2^32 threads.
+constexpr int64_t kMxDequantGrid = 1 << 20;
 template <int DT>
-__global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint32_t* codes,
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* codes,
                                                             const uint8_t* scales, int64_t rows,
                                                             int K, typename MxElem<DT>::type* out) {
-  const int per_row = K / 8;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= rows * per_row) return;
-  const int64_t row = i / per_row;
-  const int k = static_cast<int>(i - row * per_row) * 8;
-  const uint32_t c = codes[i];
+  typedef typename MxElem<DT>::type vec __attribute__((ext_vector_type(DT == kMxF32 ? 4 : 8)));
+  constexpr int PER = DT == kMxF32 ? 4 : 8;  // values of a thread
+  const uint32_t per_row = K / PER;
+  const int64_t first = (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * 256;
+  const int64_t row0 = first / per_row;  // (of the workgroup; in 32 bits from there)
+  const uint32_t at = static_cast<uint32_t>(first - row0 * per_row) + threadIdx.x;
+  const int64_t row = row0 + at / per_row, i = first + threadIdx.x;
+  const int k = static_cast<int>(at % per_row) * PER;
+  if (row >= rows) return;
+  uint32_t c;
+  if constexpr (DT == kMxF32) c = reinterpret_cast<const uint16_t*>(codes)[i];
+  else c = reinterpret_cast<const uint32_t*>(codes)[i];
   const uint32_t e = scales[((k / kMxGroup) * rows + row) * 4 + k / kMxBlock % 4];
-  typedef typename MxElem<DT>::type vec __attribute__((ext_vector_type(4)));
-  vec v[2];
+  f2_t f[4];
+  f[0] = mx_values2<0>(c, e), f[1] = mx_values2<1>(c, e);
+  if constexpr (DT != kMxF32) f[2] = mx_values2<2>(c, e), f[3] = mx_values2<3>(c, e);
+  vec v;
 #pragma unroll
-  for (int u = 0; u < 8; ++u) v[u / 4][u % 4] = mx_out<DT>(mx_value(c >> (4 * u) & 15u, e));
-  vec* o = reinterpret_cast<vec*>(out + i * 8);
-  o[0] = v[0];
-  o[1] = v[1];
+  for (int u = 0; u < PER; ++u) v[u] = mx_out<DT>(f[u / 2][u % 2]);
+  __builtin_nontemporal_store(v, reinterpret_cast<vec*>(out) + i);
 }
 
 struct MxArgs {
@@ -424,40 +436,48 @@ __global__ __launch_bounds__(64 * kMxWaves) void mx_rows_kernel(MxArgs a) {
 namespace nibble {
 namespace {
 
-template <int XT, int WT, int WM, int WN, int KU, int RING, int OCC, int DT>
+template <int XT, int WT, int WM, int WN, int RING, int OCC, int DT>
 hipError_t launch_mx_tile(const MxArgs& a, hipStream_t stream) {
-  using S = MxTile<XT, WT, WM, WN, KU, RING>;
+  using S = MxTile<XT, WT, WM, WN, RING>;
   const int tm = static_cast<int>(ceil_div(a.M, S::BM)), tn = static_cast<int>(ceil_div(a.N, S::BN));
-  mx_tile_kernel<S, XT, WT, WM, WN, KU, DT, OCC><<<dim3(tm * tn), S::THREADS, 0, stream>>>(a, tm, tn);
+  mx_tile_kernel<S, XT, WT, WM, WN, DT, OCC><<<dim3(tm * tn), S::THREADS, 0, stream>>>(a, tm, tn);
   return hipGetLastError();
 }
 
 // Which kernel a product runs on.  Few rows take the rows kernel while its
-// workgroups (16 rows of w by up to 64 of x) are few a CU; the tile kernel's
-// forms are priced by what a step of 128 k takes on a CU (ns; measured on
-// MI355X, N = 1024 .. 28672, K = 1024 .. 14336): `alone` where a CU has one tile,
-// `each` where it has many.  us, rows kernel / 64 x 64 / 64 x 128 / 128 x 128 /
-// 256 x 256 tiles: 64 x 4096 x 4096 7.8 / 8.4 / 11.7 / 15.3 / 28.5; 96 x 4096 x
-// 4096 11.2 / 8.5 / 11.7 / 15.2 / 28.6; 1 x 28672 x 4096 14.0 / 11.9 / 16.4 / 19.3
-// / 31.7; 1024 x 4096 x 4096 76 / 19.3 / 16.8 / 17.6 / 30.3; 2048 x 4096 x 4096
-// 147 / 33.4 / 32.6 / 25.1 / 35.5; 2048 x 14336 x 4096 537 / 112 / 97 / 85 / 77.
-enum MxForm { kMxRowsForm, kMx64x64, kMx64x128, kMx128x128, kMx256x256 };
-MxForm mx_form(int64_t M, int64_t N) {
+// workgroups (16 rows of w by up to 64 of x) are few a CU: 18 x 4136 x 5536 6.6 us
+// against 10.6 with the tile kernel, 26 x 9437 x 5536 13.1 against 11.5; 65 x 2770
+// x 5536 10.7 against 11.2, 128 x 4096 x 4096 12.6 against 8.6.  The tile kernel's
+// forms are priced (ns): `fixed` for filling and writing a CU's tiles, and a step
+// of 128 k, `alone` where a CU has one tile and `each` where it has more, the
+// larger of the two.  The prices are a fit to every form's time at 94 sizes (M 16
+// .. 4096, N 733 .. 28672, K 512 .. 14336), over which the form they name takes
+// 1.01 of the best one's time in the mean and 1.13 at most.  us, 64 x 64 / 64 x
+// 256 / 128 x 128 / 128 x 192 / 192 x 256 / 256 x 256: 512 x 4096 x 4096 10.6 /
+// 13.9 / 14.3 / 16.2 / 22.1 / 27.4; 1000 x 4102 x 4096 22.7 / 25 / 22.2 / 19.4 / 25.2
+// / 31.0; 2048 x 4096 x 4096 34.9 / 30 / 22.8 / 33.2 / 25.1 / 30.8; 1500 x 6144 x
+// 4096 36.8 / 38 / 33.0 / 32.8 / 25.8 / 30.1; 2048 x 14336 x 4096 120 / 101 / 77 /
+// 83 / 76 / 69.
+enum MxForm { kMxRowsForm, kMx64x64, kMx64x256, kMx128x128, kMx128x192, kMx192x256, kMx256x256 };
+MxForm mx_form(int64_t M, int64_t N, int64_t K) {
   const int64_t most = M <= 16 ? 768 : M <= 32 ? 384 : 256;
   if (ceil_div(N, 16) * ceil_div(M, 64) <= most) return kMxRowsForm;
   struct Price {
     MxForm form;
-    int bm, bn, alone, each;
+    int bm, bn, at_once;  // tiles a CU works on at once
+    int fixed, alone, each;
   };
-  const Price prices[] = {{kMx64x64, 64, 64, 155, 122},
-                          {kMx64x128, 64, 128, 270, 210},
-                          {kMx128x128, 128, 128, 420, 345},
-                          {kMx256x256, 256, 256, 1050, 1150}};
+  static constexpr Price prices[] = {
+      {kMx64x64, 64, 64, 2, 1400, 160, 110},     {kMx64x256, 64, 256, 1, 2630, 360, 360},
+      {kMx128x128, 128, 128, 2, 3900, 310, 270}, {kMx128x192, 128, 192, 1, 4100, 370, 370},
+      {kMx192x256, 192, 256, 1, 5950, 540, 540}, {kMx256x256, 256, 256, 1, 7500, 690, 690}};
+  const int64_t steps = 2 * ceil_div(K, 2 * kMxGroup);
   MxForm best = kMx64x64;
   int64_t least = INT64_MAX;
   for (const Price& p : prices) {
-    const int64_t rounds = ceil_div(ceil_div(M, p.bm) * ceil_div(N, p.bn), 256);
-    const int64_t cost = std::max<int64_t>(p.alone, rounds * p.each);
+    const int64_t tiles = ceil_div(M, p.bm) * ceil_div(N, p.bn);
+    const int64_t cost = ceil_div(tiles, 256 * p.at_once) * p.fixed +
+                         steps * std::max<int64_t>(p.alone, ceil_div(tiles, 256) * p.each);
     if (cost < least) least = cost, best = p.form;
   }
   return best;
@@ -465,11 +485,13 @@ MxForm mx_form(int64_t M, int64_t N) {
 
 template <int DT>
 hipError_t launch_mx_matmul(const MxArgs& a, hipStream_t stream) {
-  switch (mx_form(a.M, a.N)) {
-    case kMx64x64: return launch_mx_tile<2, 2, 2, 2, 2, 3, 2, DT>(a, stream);
-    case kMx64x128: return launch_mx_tile<2, 4, 2, 2, 2, 2, 2, DT>(a, stream);
-    case kMx128x128: return launch_mx_tile<4, 4, 2, 2, 2, 2, 2, DT>(a, stream);
-    case kMx256x256: return launch_mx_tile<8, 4, 2, 4, 2, 2, 2, DT>(a, stream);
+  switch (mx_form(a.M, a.N, a.K)) {
+    case kMx64x64: return launch_mx_tile<2, 2, 2, 2, 3, 2, DT>(a, stream);
+    case kMx64x256: return launch_mx_tile<2, 4, 2, 4, 2, 2, DT>(a, stream);
+    case kMx128x128: return launch_mx_tile<4, 4, 2, 2, 2, 2, DT>(a, stream);
+    case kMx128x192: return launch_mx_tile<4, 3, 2, 4, 2, 2, DT>(a, stream);
+    case kMx192x256: return launch_mx_tile<6, 4, 2, 4, 2, 2, DT>(a, stream);
+    case kMx256x256: return launch_mx_tile<8, 4, 2, 4, 2, 2, DT>(a, stream);
     case kMxRowsForm: break;
   }
   const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
@@ -576,9 +598,11 @@ extern "C" int nibble_mx_dequantize(const void* codes, const void* scales, int64
   DeviceGuard guard;
   int dev = 0;
   NIBBLE_HIP(guard.enter(stream, &dev));
-  const auto* c = static_cast<const uint32_t*>(codes);
+  const auto* c = static_cast<const uint8_t*>(codes);
   const auto* s = static_cast<const uint8_t*>(scales);
-  const dim3 grid(static_cast<unsigned>(ceil_div(rows * (K / 8), 256)));
+  const int64_t blocks = ceil_div(rows * (K / (dtype == kMxF32 ? 4 : 8)), 256);
+  const int64_t across = std::min(blocks, kMxDequantGrid);
+  const dim3 grid(static_cast<unsigned>(across), static_cast<unsigned>(ceil_div(blocks, across)));
   if (dtype == kMxF32)
     mx_dequantize_kernel<kMxF32><<<grid, 256, 0, stream>>>(c, s, rows, (int)K, static_cast<float*>(out));
   else if (dtype == kMxF16)
@@ -625,7 +649,7 @@ extern "C" int nibble_mx_matmul(const void* x_codes, const void* x_scales, int64
 }
 
 extern "C" int nibble_mx_matmul_takes_dense(int64_t M, int64_t N, int64_t K) {
-  return M >= 1 && M <= 16 && N >= 1 && K >= 1 && mx_form(M, N) == kMxRowsForm;
+  return M >= 1 && M <= 16 && N >= 1 && K >= 1 && mx_form(M, N, K) == kMxRowsForm;
 }
 
 extern "C" int nibble_mx_matmul_dense(const void* X, int64_t M, int64_t row_stride, int64_t x_dtype,
@@ -643,7 +667,8 @@ extern "C" int nibble_mx_matmul_dense(const void* X, int64_t M, int64_t row_stri
   NIBBLE_CHECK(X != nullptr && Y != nullptr && w_codes != nullptr && w_scales != nullptr,
                "null pointer");
   const int64_t size = x_dtype == kMxF32 ? 4 : 2;
-  NIBBLE_CHECK(row_stride >= 0 && row_stride * size % 16 == 0 && aligned(X, 16),
+  NIBBLE_CHECK(row_stride >= 0 && row_stride < (int64_t(1) << 40) && row_stride * size % 16 == 0 &&
+                   aligned(X, 16),
                "every row of x must start on 16 bytes");
   NIBBLE_CHECK(((M - 1) * row_stride + K) * size < (int64_t(1) << 31), "rows of x beyond 2^31 bytes");
   NIBBLE_CHECK(aligned(w_codes, 16) && aligned(w_scales, 4) && aligned(Y, 16), "misaligned pointer");

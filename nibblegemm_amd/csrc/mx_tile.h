@@ -9,11 +9,9 @@ namespace nibble {
 constexpr int kMxGroupM = 8;  // row tiles of x that share a column tile of w in turn
 
 // A tile of y = x w^T per workgroup of WM x WN waves, each XT 16-row tiles of x
-// by WT of w.  A step is KU k groups of 128: 64 KU bytes of codes and KU words of
-// scales a row, copied straight into an LDS ring; a step's copies are issued
-// between the products of the step RING - 1 before it.  A wave waits for its own
-// copies by count, then the barrier makes everybody's visible and the oldest
-// buffer free.  No other memory operation is in flight in the loop.
+// by WT of w.  A step is two k groups of 128: 128 bytes of codes (a whole line;
+// rows of 64 bytes came at half the rate) and two words of scales a row, copied
+// straight into a ring of RING buffers in LDS.
 //
 // v_mfma_scale_f32_16x16x128 takes from lane (g = l / 16, c = l % 16) block g of
 // row c and its scale, byte g of the row's word.  w is the row operand: a lane
@@ -21,10 +19,25 @@ constexpr int kMxGroupM = 8;  // row tiles of x that share a column tile of w in
 // moves the same bytes; on random codes, register to register, it ran at 5.9
 // PFLOP/s and this one at 6.8: the card's power sets both.)
 //
-// In LDS unit u (16 bytes) of row r lies at unit u ^ swizzle(r): eight rows of a
-// read cover 32 banks once.
-template <int XT, int WT, int WM, int WN, int KU, int RING_>
+// A register is read again from LDS as soon as its last product is issued, with
+// the next k group's codes, so reads run under products all the time and no
+// second set of registers is needed.  In a step's last k group, behind the first
+// column of products, a wave waits for its own copies of the next step, by count;
+// the barrier makes everybody's visible and this step's buffer free, and the
+// copies of the step RING later go out.  No other memory operation is in flight
+// in the loop.  2048 x 14336 x 16384 230 us against 240 with a k group's reads
+// before its products.
+//
+// In LDS unit u (16 bytes) of row r lies at unit u ^ (r % 8): eight rows of a read
+// cover 32 banks once.
+//
+// What bounds it: power, then the copies.  2048 x 14336 x 16384 takes 230 us, 4.2
+// PFLOP/s; with codes of zero, the same instructions, 190.  Without copies it took
+// 209 of then 273 us, without reads of LDS 254, without either 163, which is the
+// rate of the products alone over 448 tiles in two rounds of 256 CUs.
+template <int XT, int WT, int WM, int WN, int RING_>
 struct MxTile {
+  static constexpr int KU = 2;  // k groups of a step
   static constexpr int RING = RING_, WAVES = WM * WN, THREADS = 64 * WAVES;
   static constexpr int BM = 16 * XT * WM, BN = 16 * WT * WN;
   static constexpr int ROW = 64 * KU, UNITS = 4 * KU;   // bytes and 16-byte units of a row
@@ -38,14 +51,14 @@ struct MxTile {
   static constexpr bool SPARE = SCOPIES * WAVES > CHUNKS;  // copies that only keep the count
   static constexpr int LDS = RING * STEP + (SPARE ? 256 : 0);
   static constexpr int LOADS = XCOPIES + WCOPIES + SCOPIES;
-  static_assert(XCOPIES * WAVES * 1024 == BM * ROW && WCOPIES * WAVES * 1024 == BN * ROW, "shares");
+  static_assert(XCOPIES * WAVES * 1024 == BM * ROW && WCOPIES * WAVES * 1024 == BN * ROW &&
+                    BM % 64 == 0 && BN % 64 == 0, "shares");
   static_assert(LOADS * (RING - 1) <= 63, "vmcnt range");
-  static __device__ __forceinline__ int swizzle(int r) { return KU == 1 ? r >> 1 & 3 : r & 7; }
 };
 
-template <class S, int XT, int WT, int WM, int WN, int KU, int DT, int OCC>
+template <class S, int XT, int WT, int WM, int WN, int DT, int OCC>
 __global__ __launch_bounds__(S::THREADS, OCC) void mx_tile_kernel(MxArgs a, int tiles_m, int tiles_n) {
-  constexpr int BM = S::BM, BN = S::BN, WAVES = S::WAVES;
+  constexpr int BM = S::BM, BN = S::BN, KU = S::KU, WAVES = S::WAVES;
   __shared__ __attribute__((aligned(16))) uint8_t lds[S::LDS];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -77,7 +90,7 @@ __global__ __launch_bounds__(S::THREADS, OCC) void mx_tile_kernel(MxArgs a, int 
   // sent out of range lane by lane, so that the count of loads stays.
   constexpr int CROWS = 16 / KU;
   const int crow = lane / S::UNITS;
-  const int unit = (lane % S::UNITS) ^ S::swizzle(crow);  // (CROWS wave does not change it)
+  const int unit = (lane % S::UNITS) ^ crow;  // (crow < 8, and a copy starts on a multiple of 8)
   const uint32_t voff = static_cast<uint32_t>(crow) * half_k + unit * 16u;
   const uint32_t rows_step = static_cast<uint32_t>(CROWS * WAVES) * half_k;
   const uint32_t rows_wave = static_cast<uint32_t>(CROWS * wave) * half_k;
@@ -131,58 +144,68 @@ __global__ __launch_bounds__(S::THREADS, OCC) void mx_tile_kernel(MxArgs a, int 
     for (int j = 0; j < WT; ++j) acc[i][j] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
   const int c = lane & 15, g = lane >> 4;
-  const int xrow = wm * 16 * XT + c, wrow = BM + wn * 16 * WT + c;  // (rows 16 apart share
-  const int sw = S::swizzle(c);                                     // the swizzle)
+  const int xrow = wm * 16 * XT + c, wrow = BM + wn * 16 * WT + c;
+  const uint32_t at = (g ^ (c & 7)) * 16u;  // of a lane's block in k group 0; rows 16 apart agree
+  u4_t x[XT], w[WT];
+  uint32_t xs[XT], ws[WT];  // (a lane's block: byte g of its row's word)
+  auto read_x = [&](int i, int buf, int kg) {
+    const uint8_t* const p = lds + buf * S::STEP;
+    xs[i] = p[S::CODES + (kg * (BM + BN) + xrow + 16 * i) * 4 + g];
+    x[i] = *reinterpret_cast<const u4_t*>(p + (xrow + 16 * i) * S::ROW + (at ^ 64u * kg));
+  };
+  auto read_w = [&](int n, int buf, int kg) {
+    const uint8_t* const p = lds + buf * S::STEP;
+    ws[n] = p[S::CODES + (kg * (BM + BN) + wrow + 16 * n) * 4 + g];
+    w[n] = *reinterpret_cast<const u4_t*>(p + (wrow + 16 * n) * S::ROW + (at ^ 64u * kg));
+  };
 #pragma unroll
-  for (int t = 0; t < S::RING - 1; ++t) {
+  for (int t = 0; t < S::RING; ++t) {
     const Step s = prepare(t, t);
 #pragma unroll
     for (int u = 0; u < S::LOADS; ++u) load(u, s);
   }
-  int buf = 0, next = S::RING - 1;
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm((S::RING - 1) * S::LOADS));  // (step 0)
+  lds_barrier();
+#pragma unroll
+  for (int n = 0; n < WT; ++n) read_w(n, 0, 0);
+#pragma unroll
+  for (int i = 0; i < XT; ++i) read_x(i, 0, 0);
+  int buf = 0;
   for (int t = 0; t < steps; ++t) {
-    __builtin_amdgcn_s_waitcnt(waitcnt_vm((S::RING - 2) * S::LOADS));
-    lds_barrier();
-    const Step coming = prepare(t + S::RING - 1, next);
+    const int next = buf == S::RING - 1 ? 0 : buf + 1;
+    const Step coming = prepare(t + S::RING, buf);
 #pragma unroll
     for (int kg = 0; kg < KU; ++kg) {
-      const uint8_t* const p = lds + buf * S::STEP + ((4 * kg + g) ^ sw) * 16;
-      const uint8_t* const ps = lds + buf * S::STEP + S::CODES + kg * (BM + BN) * 4;
-      u4_t x[XT], w[WT];
-      uint32_t xs[XT], ws[WT];
-#pragma unroll
-      for (int i = 0; i < XT; ++i) {
-        xs[i] = *reinterpret_cast<const uint32_t*>(ps + (xrow + 16 * i) * 4);
-        x[i] = *reinterpret_cast<const u4_t*>(p + (xrow + 16 * i) * S::ROW);
-      }
-#pragma unroll
-      for (int i = 0; i < WT; ++i) {
-        ws[i] = *reinterpret_cast<const uint32_t*>(ps + (wrow + 16 * i) * 4);
-        w[i] = *reinterpret_cast<const u4_t*>(p + (wrow + 16 * i) * S::ROW);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+      const bool last = kg == KU - 1;
+      const int from = last ? next : buf, group = last ? 0 : kg + 1;
 #pragma unroll
       for (int n = 0; n < WT; ++n) {
-        const uint32_t wsn = ws[n] >> (8 * g);
         const i8_t vw = {(int)w[n][0], (int)w[n][1], (int)w[n][2], (int)w[n][3], 0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < XT; ++i) {
           const i8_t vx = {(int)x[i][0], (int)x[i][1], (int)x[i][2], (int)x[i][3], 0, 0, 0, 0};
           acc[i][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              vw, vx, acc[i][n], 4, 4, 0, (int)wsn, 0, (int)(xs[i] >> (8 * g)));
+              vw, vx, acc[i][n], 4, 4, 0, (int)ws[n], 0, (int)xs[i]);
+          if (n == WT - 1) {
+            __builtin_amdgcn_sched_barrier(0);
+            read_x(i, from, group);
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
         __builtin_amdgcn_sched_barrier(0);
-        // (all in the step's first group, so that the last ones have the others to
-        // arrive in: 2048 x 14336 x 4096 85 -> 82 us against the whole step)
-        constexpr int PARTS = WT;
-        const int part = kg * WT + n;
+        if (last && n == 0) {
+          __builtin_amdgcn_s_waitcnt(waitcnt_vm((S::RING - 2) * S::LOADS));
+          lds_barrier();
+        }
+        read_w(n, from, group);
+        if (last) {
 #pragma unroll
-        for (int u = min(part, PARTS) * S::LOADS / PARTS; u < min(part + 1, PARTS) * S::LOADS / PARTS; ++u) load(u, coming);
+          for (int u = n * S::LOADS / WT; u < (n + 1) * S::LOADS / WT; ++u) load(u, coming);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    buf = buf == S::RING - 1 ? 0 : buf + 1;
-    next = next == S::RING - 1 ? 0 : next + 1;
+    buf = next;
   }
   // No copy may land in LDS that holds something else by then.
   __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
@@ -190,7 +213,8 @@ __global__ __launch_bounds__(S::THREADS, OCC) void mx_tile_kernel(MxArgs a, int 
 
   // The outputs go through LDS, 16 rows of a wave at a time, so that a store
   // covers whole runs of a row: 16 bytes a lane where every row starts on 16,
-  // else 4 or single outputs.
+  // else 4 or single outputs.  They pass by the caches (512 x 14336 x 4096 21.8 us
+  // against 23.1).
   using T = typename MxElem<DT>::type;
   typedef T vec4 __attribute__((ext_vector_type(4)));
   constexpr int COLS = 16 * WT, PITCH = COLS + 16 / sizeof(T);
@@ -216,11 +240,12 @@ __global__ __launch_bounds__(S::THREADS, OCC) void mx_tile_kernel(MxArgs a, int 
       using P = decltype(piece);
       constexpr int E = sizeof(P) / sizeof(T), PER = COLS / E;  // outputs a store, stores a row
 #pragma unroll
-      for (int u = 0; u < 16 * PER / 64; ++u) {
+      for (int u = 0; u < (16 * PER + 63) / 64; ++u) {
         const int r = (u * 64 + lane) / PER, n = (u * 64 + lane) % PER * E;
-        if (m1 + r < a.M && n < cols)
-          *reinterpret_cast<P*>(y + static_cast<int64_t>(m1 + r) * a.N + n1 + n) =
-              *reinterpret_cast<const P*>(out + r * PITCH + n);
+        if (r < 16 && m1 + r < a.M && n < cols)
+          __builtin_nontemporal_store(
+              *reinterpret_cast<const P*>(out + r * PITCH + n),
+              reinterpret_cast<P*>(y + static_cast<int64_t>(m1 + r) * a.N + n1 + n));
       }
     };
     if (row_bytes == 0) store(u4_t{});

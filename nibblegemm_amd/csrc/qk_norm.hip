@@ -153,7 +153,9 @@ extern "C" int nibble_qk_norm_rope(const void* QKV, int64_t dtype, int64_t batch
   NIBBLE_CHECK(std::isfinite(eps) && eps >= 0.0f, "eps must be finite and >= 0");
   if (batch == 0 || tokens == 0) return ok();
   const int64_t vectors_per = n_heads + 2 * n_kv_heads;
-  NIBBLE_CHECK(batch * tokens <= (int64_t(1) << 34) / vectors_per, "too many tokens");
+  // (a launch ends at 2^32 threads, head_dim / 16 a vector)
+  NIBBLE_CHECK(batch * tokens <= ((int64_t(1) << 32) - kQkThreads) / (head_dim / 16) / vectors_per,
+               "too many tokens: %lld x %lld", (long long)batch, (long long)tokens);
   for (int64_t s : {k_batch_stride, k_head_stride, k_row_stride, v_batch_stride, v_head_stride,
                     v_row_stride})
     NIBBLE_CHECK(s >= 0 && s % 8 == 0, "cache strides must be multiples of 8 elements, got %lld",

@@ -231,6 +231,7 @@ def dense(ext, X=P, M=2, rs=128, xdt=0, wc=P, ws=P, N=64, K=128, dt=0, Y=P):
     (dict(X=0), "null", INVALID),
     (dict(ws=0), "null", INVALID),
     (dict(rs=132), "16 bytes", INVALID),
+    (dict(rs=1 << 62), "16 bytes", INVALID),
     (dict(X=P + 8), "16 bytes", INVALID),
     (dict(rs=1 << 30), "2^31", INVALID),
     (dict(wc=P + 8), "misaligned", INVALID),
@@ -376,7 +377,12 @@ SIZES = [(1, 64, 32), (1, 1024, 4096), (2, 17, 96), (5, 100, 512), (8, 48, 544),
          (16, 256, 1056), (17, 64, 4128), (27, 333, 2048), (32, 96, 5536), (33, 260, 640),
          (63, 1000, 992), (64, 64, 14336), (65, 129, 256), (100, 515, 1120), (128, 128, 512),
          (130, 257, 2080), (200, 1023, 128), (256, 256, 4096), (257, 300, 160), (333, 2050, 1024),
-         (513, 770, 1056), (1000, 1000, 544), (1024, 512, 2048), (2048, 1030, 64)]
+         (513, 770, 1056), (1000, 1000, 544), (1024, 512, 2048), (2048, 1030, 64),
+         # larger tiles of every form, whole and not
+         (70, 2113, 992), (1024, 4096, 256), (1000, 4090, 96), (132, 10937, 288), (2048, 4096, 128),
+         (2000, 4090, 352), (1921, 4033, 32), (1000, 4102, 544), (1674, 2370, 32), (261, 13148, 96),
+         (1500, 6144, 512), (2346, 3361, 32), (515, 13236, 288), (2048, 7168, 512), (1999, 7001, 288),
+         (1800, 7100, 1056)]
 
 
 @pytest.mark.gpu

@@ -225,6 +225,7 @@ def tree(ext, q=P, dt=0, B=1, T=2, nh=4, nkv=2, D=128, kc=P, st=(4096, 2048, 128
     (dict(qkv=0), "null"), (dict(kc=0), "null"), (dict(pos=0), "null"), (dict(slots=0), "null"),
     (dict(out=0), "null"), (dict(qkv=P + 8), "aligned"), (dict(qw=P + 8), "aligned"),
     (dict(vc=P + 2), "aligned"), (dict(pos=P + 2), "aligned"), (dict(B=1 << 30, T=1 << 30), "too many"),
+    (dict(B=1 << 20, T=1 << 10), "too many"),
 ])
 def test_qk_rejections(kwargs, needle):
     ext = ng.extension()
