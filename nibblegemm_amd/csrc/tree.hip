@@ -101,6 +101,13 @@ struct TreeShares {
   int per = 0, found = -1, first = 0, count = 0;
   // Finds the sequence that share `want` is of, and that sequence's shares.
   __device__ __forceinline__ TreeShares(const TreeArgs& a, int want) {
+    if (a.B == 1) {
+      const int all = tiles(a, 0);
+      per = max((all + a.shares - 1) / a.shares, max((all + kTreeMaxSplits - 1) / kTreeMaxSplits, 1));
+      count = shares_of(all);
+      found = want < count ? 0 : -1;
+      return;
+    }
     const int lane = threadIdx.x & 63;
     int t[kChunks];  // tiles; 0 where there is no sequence
     float most_f = 0.0f, total = 0.0f;
@@ -117,11 +124,6 @@ struct TreeShares {
     per = static_cast<int>(ceilf(wave_sum(total) / static_cast<float>(a.shares)));
     per = max(max(per, (most + kTreeMaxSplits - 1) / kTreeMaxSplits), 1);
     per = __builtin_amdgcn_readfirstlane(per);
-    if (a.B == 1) {
-      count = shares_of(most);
-      found = want < count ? 0 : -1;
-      return;
-    }
     int high = max(per, most);  // enough: one share each
     for (int low = per; low < high;) {
       const bool close = high - low <= low / 16;
@@ -183,7 +185,8 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   typedef __attribute__((address_space(3))) s4_t lds4_t;
   __shared__ __attribute__((aligned(16))) T kv[2][2][KT * D];  // buffer; k, v
   __shared__ float stat[2][WK][WQ * QT * 16];
-  static_assert(sizeof(kv) >= sizeof(float) * WK * WQ * 16 * D, "the sums fit");
+  __shared__ int place[WQ * QT * 16];  // of a row's output, in heads
+  static_assert(sizeof(kv) >= sizeof(float) * WK * WQ * QT * 16 * D, "the sums fit");
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -301,7 +304,8 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
       for (int ss = 0; ss < D / 32; ++ss) {
         const vec8 ka = *reinterpret_cast<const vec8*>(kt + j * 16 * D * 2 + (krow ^ (64 * ss)));
 #pragma unroll
-        for (int t = 0; t < QT; ++t) x.s[j][t] = E::mfma(ka, q[t][ss], ss == 0 ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : x.s[j][t]);
+        for (int t = 0; t < QT; ++t)
+          x.s[j][t] = E::mfma(ka, q[t][ss], ss == 0 ? f4_t{0.0f, 0.0f, 0.0f, 0.0f} : x.s[j][t]);
       }
     }
   };
@@ -486,72 +490,64 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   for (; i < plain; ++i) turn(i, std::false_type{});
   for (; i < count; ++i) turn(i, std::true_type{});
   __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // no copy may land in what follows
-  __syncthreads();
+  lds_barrier();
 
-  // The waves along the keys meet: statistics first, then the sums on the
-  // common maximum, 16 rows of each wave at a time through LDS.
+  // The waves along the keys meet: statistics and sums through LDS, then each
+  // wave's sums on the common maximum.  Unit (16 bytes) u of row c of 16 lies at
+  // unit u ^ (c % 8): eight rows of a write cover 32 banks once.
+  constexpr int QUADS = D / 4, ALL = QT * WQ * 16;
+  f4_t* const red = reinterpret_cast<f4_t*>(&kv[0][0][0]);  // [WK][ALL][QUADS]
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    const bool behind = rw + 16 * t + c >= rows;  // the last token
+    const int at = (wq * QT + t) * 16 + c, r = rw + 16 * t + c;
+    const bool behind = r >= rows;  // the last token
     if (behind) top[t] = -INFINITY;
     else if (top[t] == -INFINITY && sum[t][0] != 0.0f) top[t] = 0.0f;  // NaN scores alone
     if (g == 0) {
-      stat[0][wk][(wq * QT + t) * 16 + c] = top[t];
-      stat[1][wk][(wq * QT + t) * 16 + c] = behind ? 0.0f : sum[t][0];
+      stat[0][wk][at] = top[t];
+      stat[1][wk][at] = behind ? 0.0f : sum[t][0];
+      if (wk == 0) {
+        const int i = behind ? r / a.qpk : node[t];
+        place[at] = i * a.n_heads + r - i * a.qpk;
+      }
     }
-  }
-  __syncthreads();
-  float* const red = reinterpret_cast<float*>(&kv[0][0][0]);  // [WK][WQ 16][D]
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    float high = stat[0][0][(wq * QT + t) * 16 + c];
-#pragma unroll
-    for (int w = 1; w < WK; ++w) high = fmaxf(high, stat[0][w][(wq * QT + t) * 16 + c]);
-    const float mine = high == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[t] - high);
 #pragma unroll
     for (int d = 0; d < D / 16; ++d)
+      red[(wk * ALL + at) * QUADS + ((4 * d + g) ^ (c & 7))] = acc[t][d];
+  }
+  lds_barrier();
+  const int64_t rec0 = (static_cast<int64_t>(h) * a.shares + w) * rows_all + r0;
+  float* const sums = a.partial + rec0 * D;
+  float* const stats = a.partial + static_cast<int64_t>(a.n_kv) * a.shares * rows_all * D + rec0 * 2;
+  T* const out = static_cast<T*>(a.out) +
+                 (static_cast<int64_t>(b) * a.T * a.n_heads + h * a.qpk) * D;
+  const int u = threadIdx.x % QUADS;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        red[(wk * WQ * 16 + wq * 16 + c) * D + 16 * d + 4 * g + i] = acc[t][d][i] * mine;
-    __syncthreads();
-    for (int e = threadIdx.x; e < WQ * 16 * (D / 4); e += kTreeThreads) {
-      const int rr = e / (D / 4), d = e % (D / 4) * 4;
-      const int slot16 = (rr / 16 * QT + t) * 16 + rr % 16;
-      const int r = r0 + rr / 16 * 16 * QT + 16 * t + rr % 16;
-      if (r >= rows_all) continue;
-      f4_t o = *reinterpret_cast<const f4_t*>(&red[rr * D + d]);
-      float mr = stat[0][0][slot16];
+  for (int e = 0; e < ALL * QUADS / kTreeThreads; ++e) {
+    const int at = e * (kTreeThreads / QUADS) + threadIdx.x / QUADS;
+    if (r0 + at >= rows_all) break;
+    float mr = stat[0][0][at], l = 0.0f;
 #pragma unroll
-      for (int w = 1; w < WK; ++w) {
-        o += *reinterpret_cast<const f4_t*>(&red[(w * WQ * 16 + rr) * D + d]);
-        mr = fmaxf(mr, stat[0][w][slot16]);
-      }
-      float l = 0.0f;
+    for (int x = 1; x < WK; ++x) mr = fmaxf(mr, stat[0][x][at]);
+    f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int w = 0; w < WK; ++w)
-        l += mr == -INFINITY ? 0.0f
-                             : stat[1][w][slot16] * __builtin_amdgcn_exp2f(stat[0][w][slot16] - mr);
-      if (a.shares == 0) {
-        const int i = r / a.qpk;
-        T* out = static_cast<T*>(a.out) +
-                 ((static_cast<int64_t>(b) * a.T + i) * a.n_heads + h * a.qpk + (r - i * a.qpk)) * D + d;
-        typedef T vec4 __attribute__((ext_vector_type(4)));
-        vec4 y;
+    for (int x = 0; x < WK; ++x) {
+      const float keep = mr == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(stat[0][x][at] - mr);
+      l += stat[1][x][at] * keep;
+      const f4_t v = red[(x * ALL + at) * QUADS + (u ^ (at & 7))];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) y[x] = static_cast<T>(l == 0.0f ? 0.0f : o[x] / l);
-        *reinterpret_cast<vec4*>(out) = y;
-      } else {
-        const int64_t rec = (static_cast<int64_t>(h) * a.shares + w) * rows_all + r;
-        if (mr != -INFINITY) *reinterpret_cast<f4_t*>(a.partial + rec * D + d) = o;
-        if (d == 0) {
-          float* st = a.partial +
-                      static_cast<int64_t>(a.n_kv) * a.shares * rows_all * D + rec * 2;
-          st[0] = mr;
-          st[1] = l;
-        }
-      }
+      for (int i = 0; i < 4; ++i) o[i] += v[i] * keep;
     }
-    __syncthreads();
+    if (a.shares == 0) {
+      typedef T vec4 __attribute__((ext_vector_type(4)));
+      vec4 y;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) y[x] = static_cast<T>(l == 0.0f ? 0.0f : o[x] / l);
+      *reinterpret_cast<vec4*>(out + static_cast<int64_t>(place[at]) * D + 4 * u) = y;
+    } else {
+      if (mr != -INFINITY) *reinterpret_cast<f4_t*>(sums + static_cast<int64_t>(at) * D + 4 * u) = o;
+      if (u == 0) stats[2 * at] = mr, stats[2 * at + 1] = l;
+    }
   }
 }
 
