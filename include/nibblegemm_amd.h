@@ -505,7 +505,7 @@ NIBBLE_API int nibble_mx_matmul(const void* x_codes, const void* x_scales, int64
 /* The same with a dense X [M, K] (x_dtype; rows row_stride elements apart,
  * every row on 16 bytes, the last one ending below 2^31 bytes), quantised on the
  * way: nibble_mx_quantize's codes and nibble_mx_matmul's bits in one launch, where
- * nibble_mx_matmul_takes_dense(M, N, K) is 1 (few rows); NIBBLE_ERR_UNSUPPORTED
+ * nibble_mx_matmul_takes_dense(M, N, K) is 1 (few rows, a small w); NIBBLE_ERR_UNSUPPORTED
  * elsewhere. */
 NIBBLE_API int nibble_mx_matmul_dense(const void* X, int64_t M, int64_t row_stride, int64_t x_dtype,
                                       const void* w_codes, const void* w_scales, int64_t N,

@@ -151,7 +151,9 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const typename MxElem<
 // Rows that are adjacent in memory (a transposed view: element (row, k) at
 // k ld + row).  A workgroup takes 128 rows of one k group; wave w its block w,
 // lane l rows 2l and 2l + 1, whose 32 values it holds; the codes go through
-// LDS so that a row's 64 bytes are written together.
+// LDS so that a row's 64 bytes are written together.  Memory bounds it: 14336 rows
+// of 4096 k from fp32 in 42 us, 6.4 TB/s, from fp16 24 us; 4102 rows of 5536 k
+// from fp32 in 21 (23 with loads that pass by the caches).
 constexpr int kMxCols = 128;
 
 template <int DT, bool VEC>
@@ -386,7 +388,9 @@ struct MxDense {
 // of x; its eight waves share out the k in steps of 512 and meet in LDS, in
 // wave order.  Codes come straight from memory into the matrix cores' operands;
 // a dense x (XD, at most 16 rows) is quantised by every workgroup on the way,
-// which costs less than a launch before this one.
+// which costs less than a launch before this one where w is small.  Latency
+// bounds it: a wave's loads for a step of 512 k, the products, the meeting in LDS
+// (1 x 1024 x 4096 4.0 us of kernel for 2.2 MB).
 constexpr int kMxCodes = -1;
 template <int MT, int XD, int DT>
 __global__ __launch_bounds__(64 * kMxWaves) void mx_rows_kernel(MxArgs a) {
@@ -648,8 +652,15 @@ extern "C" int nibble_mx_matmul(const void* x_codes, const void* x_scales, int64
   return ok();
 }
 
+// Every workgroup quantises the whole of a dense x, so it is taken while that is
+// little: at most 4096 k a CU.  us, one launch / quantised before, in a graph and
+// as calls: 1 x 4096 x 1024 3.7 / 4.6, 7.5 / 15.1; 16 x 4096 x 4096 7.5 / 6.3, 7.8 /
+// 15.3; 16 x 12288 x 1024 7.7 / 5.8, 7.9 / 15.3; beyond it 1 x 12288 x 4096 10.5 /
+// 7.8, 10.0 / 14.7; 16 x 12288 x 4096 18.7 / 10.0, 17.8 / 15.0; 1 x 4096 x 14336
+// 14.2 / 8.8, 13.6 / 14.8; 16 x 12288 x 14336 64 / 28, 64 / 27.
 extern "C" int nibble_mx_matmul_takes_dense(int64_t M, int64_t N, int64_t K) {
-  return M >= 1 && M <= 16 && N >= 1 && K >= 1 && mx_form(M, N, K) == kMxRowsForm;
+  return M >= 1 && M <= 16 && N >= 1 && N <= 12288 && K >= 1 &&
+         ceil_div(N, 4096) * K <= 4096;  // (the rows kernel's sizes: one workgroup for 16 rows of w)
 }
 
 extern "C" int nibble_mx_matmul_dense(const void* X, int64_t M, int64_t row_stride, int64_t x_dtype,

@@ -15,6 +15,10 @@
 // its probabilities are already where the second product (V^T P^T, queries as
 // columns again) wants them, if that product's k index runs over a lane's keys
 // of two tiles in turn.  V is read transposed from LDS (ds_read_b64_tr_b16).
+//
+// What it reads, writes and computes: the cached rows once a kv head and 128
+// query rows, 4 rows keys D operations, and, where the rows are split, D + 2
+// floats a query row and share.  Times are of 32 heads on 8, head_dim 128.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -167,8 +171,21 @@ struct TreeShares {
 // One workgroup: 16 QT WQ query rows of one kv head (WQ = 4 / WK waves along
 // the rows, WK along the keys), one share of the cached rows, in tiles of 64
 // keys.  A tile's rows of k and v are copied straight into one of two LDS
-// buffers while the tile before it is computed; two workgroups share a CU, so
-// one's softmax runs beside the other's products.
+// buffers while the tile before it is computed; two workgroups share a CU.
+//
+// What bounds it: 64 tokens over 65000 take 89 us of this kernel (16 sequences of
+// 27 over up to 8100 86, 4.2 TB/s; 2048 over 2048 120 to 127, 0.83 PFLOP/s).  A tile of
+// a wave is 68 products of 16 cycles and 32 exponentials of 16 beside some 130
+// plain vector operations of 4; for the two waves of a SIMD that adds up to 4300
+// cycles, and a tile takes 4375: the two hardly overlap.  Neither a priority for
+// the products or the softmax, a fixed one by workgroup, nor a late start of one
+// of the two changed that (1 to 10% slower).  LDS is busy for 40% of the time.
+// Three workgroups a CU (smaller tiles) took 283 us for the last of those, 64
+// queries a wave, which would halve the reads of LDS, 519 (registers spilt).
+//
+// One call of 16 tokens over 1000 is latency: 7.7 us, of which finding its share
+// and loading the queries take 2.3, the copies 0.9, one tile 1.4, the meeting of
+// the waves and the stores 2.9 (4.5 with a barrier for each 16 rows).
 template <class E, int D, int QT, int WK>
 __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   using T = typename E::type;
@@ -376,6 +393,8 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
                              __builtin_fmaf(x.s[i / 4 % KS][t][i % 4], a.scale, -base))
                        : 0.0f);
       }
+      // (The probabilities are rounded to 16 bits because the matrix cores take
+      // them so: each is off by half a step at most, and the sum is of the rounded.)
       // The sum of the probabilities as they are multiplied, by the matrix cores
       // too: ones times P^T, a tile's keys at once, in fp32.
 #pragma unroll
@@ -554,7 +573,9 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
 // Joins the shares of a row: D / 4 lanes a row, four outputs each, the rows of
 // one (sequence, kv head) in a workgroup.  The lanes read the shares' statistics
 // together; the sums are then loaded eight shares at a time, those of shares
-// that saw nothing not at all.
+// that saw nothing not at all.  Memory and latency bound it: 64 rows of 16 shares
+// and 8 kv heads 3.9 us, 256 rows of 32 shares 8 us, 34 MB (loads begun before
+// the statistics are there gained 0.6 us on the first, lost 2 on ragged trees).
 template <class E, int D>
 __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(TreeArgs a) {
   using T = typename E::type;

@@ -248,6 +248,8 @@ def test_where_a_dense_x_is_taken():
     takes = ng.extension().mx_matmul_takes_dense
     assert takes(1, 1024, 4096) and takes(16, 4096, 4096) and takes(1, 12288, 32)
     assert not takes(17, 1024, 4096) and not takes(1, 28672, 4096)
+    assert not takes(1, 4097, 4096) and not takes(1, 4096, 4128) and not takes(1, 12289, 1024)
+    assert takes(16, 12288, 1024) and takes(5, 8192, 2048)
     assert not takes(0, 1024, 4096) and not takes(1, 0, 4096) and not takes(1, 64, 0)
 
 
@@ -397,6 +399,7 @@ def test_product(M, N, K):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M,N,K", [(1, 1024, 4096), (3, 100, 96), (7, 516, 2080), (16, 64, 544),
+                                   (2, 4100, 2048), (9, 4100, 2080), (1, 70, 4128), (16, 12288, 96),
                                    (27, 515, 1024), (64, 130, 4096), (150, 200, 672)])
 def test_product_of_dense_rows(M, N, K, dtype):
     """Quantising within the call gives the values of quantising before it."""
