@@ -407,6 +407,23 @@ def test_tokens_that_see_nothing(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("qpk", [1, 8])
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 6, 9, 66, 131])
+def test_masks_of_any_pattern(T, qpk):
+    """Trees that begin at every place of a group of four keys and of a tile,
+    masks without the token itself and with later ones, and bytes other than 1."""
+    lengths = [0, 1, 2, 3, 61, 64, 126]
+    q, k, v, lengths, _, _ = tree_case(len(lengths), T, qpk, 1, 64, 126 + T + 1, F16, lengths, False,
+                                       seed=T)
+    g = torch.Generator().manual_seed(T)
+    mask = torch.rand((len(lengths), T, T), generator=g) < 0.3
+    mask[:, T // 2] = False
+    got = check_tree(q, k, v, lengths, mask, None)
+    odd = torch.randint(1, 256, mask.shape, generator=g, dtype=torch.uint8) * mask
+    assert torch.equal(run_tree(q, k, v, lengths, odd.view(torch.bool)).cpu().double(), got)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,n_heads", [(6, 2), (6, 8), (24, 8), (40, 8), (90, 8)])
 def test_strange_values_in_rows_not_seen(T, n_heads, dtype):
