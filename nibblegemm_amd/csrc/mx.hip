@@ -454,7 +454,7 @@ hipError_t launch_mx_tile(const MxArgs& a, hipStream_t stream) {
 // x 5536 10.7 against 11.2, 128 x 4096 x 4096 12.6 against 8.6.  The tile kernel's
 // forms are priced (ns): `fixed` for filling and writing a CU's tiles, and a step
 // of 128 k, `alone` where a CU has one tile and `each` where it has more, the
-// larger of the two.  The prices are a fit to every form's time at 94 sizes (M 16
+// larger of the two.  The prices are a fit to every form's time at 94 sizes (M 17
 // .. 4096, N 733 .. 28672, K 512 .. 14336), over which the form they name takes
 // 1.01 of the best one's time in the mean and 1.13 at most.  us, 64 x 64 / 64 x
 // 256 / 128 x 128 / 128 x 192 / 192 x 256 / 256 x 256: 512 x 4096 x 4096 10.6 /
