@@ -502,15 +502,19 @@ NIBBLE_API int nibble_mx_dequantize(const void* codes, const void* scales, int64
 NIBBLE_API int nibble_mx_matmul(const void* x_codes, const void* x_scales, int64_t M,
                                 const void* w_codes, const void* w_scales, int64_t N, int64_t K,
                                 int64_t dtype, void* Y, void* stream);
-/* The same with a dense X [M, K] (x_dtype; rows row_stride elements apart,
- * every row on 16 bytes, the last one ending below 2^31 bytes), quantised on the
- * way: nibble_mx_quantize's codes and nibble_mx_matmul's bits in one launch, where
- * nibble_mx_matmul_takes_dense(M, N, K) is 1 (few rows, a small w); NIBBLE_ERR_UNSUPPORTED
- * elsewhere. */
+/* The same with a dense X [M, K] (x_dtype; rows row_stride elements apart):
+ * nibble_mx_quantize's codes and nibble_mx_matmul's bits.  Few rows by a small w
+ * are quantised on the way, in one launch, if every row starts on 16 bytes and
+ * the last one ends below 2^31 bytes; else X is quantised into the workspace
+ * first.  The workspace (nibble_mx_matmul_dense_workspace_bytes, `aligned`: whether
+ * X's rows are as said; 16-byte aligned, NULL when that is 0) needs no initial
+ * contents. */
 NIBBLE_API int nibble_mx_matmul_dense(const void* X, int64_t M, int64_t row_stride, int64_t x_dtype,
                                       const void* w_codes, const void* w_scales, int64_t N,
-                                      int64_t K, int64_t dtype, void* Y, void* stream);
-NIBBLE_API int nibble_mx_matmul_takes_dense(int64_t M, int64_t N, int64_t K);
+                                      int64_t K, int64_t dtype, void* Y, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+NIBBLE_API size_t nibble_mx_matmul_dense_workspace_bytes(int64_t M, int64_t N, int64_t K,
+                                                         int aligned);
 
 /*
  * Measurement: a streaming read of `bytes` (a positive multiple of 16) from

@@ -404,26 +404,30 @@ static PyObject* py_mx_matmul(PyObject* self, PyObject* const* a, Py_ssize_t n) 
   return PyLong_FromLong(nibble_mx_matmul(xc, xs, M, wc, ws, N, K, dt, Y, stream));
 }
 
-/* mx_matmul_dense(X, M, row_stride, x_dtype, w_codes, w_scales, N, K, dtype, Y, stream) */
+/* mx_matmul_dense(X, M, row_stride, x_dtype, w_codes, w_scales, N, K, dtype, Y, ws, ws_bytes,
+ * stream) */
 static PyObject* py_mx_matmul_dense(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   (void)self;
-  if (!nargs_is(n, 11, "mx_matmul_dense")) return NULL;
-  void *X, *wc, *ws, *Y, *stream;
-  long long M, rs, xdt, N, K, dt;
+  if (!nargs_is(n, 13, "mx_matmul_dense")) return NULL;
+  void *X, *wc, *ws, *Y, *work, *stream;
+  long long M, rs, xdt, N, K, dt, bytes;
   if (!take_ptr(a[0], &X) || !take_i64(a[1], &M) || !take_i64(a[2], &rs) || !take_i64(a[3], &xdt) ||
       !take_ptr(a[4], &wc) || !take_ptr(a[5], &ws) || !take_i64(a[6], &N) || !take_i64(a[7], &K) ||
-      !take_i64(a[8], &dt) || !take_ptr(a[9], &Y) || !take_ptr(a[10], &stream))
+      !take_i64(a[8], &dt) || !take_ptr(a[9], &Y) || !take_ptr(a[10], &work) ||
+      !take_i64(a[11], &bytes) || !take_ptr(a[12], &stream))
     return NULL;
-  return PyLong_FromLong(nibble_mx_matmul_dense(X, M, rs, xdt, wc, ws, N, K, dt, Y, stream));
+  return PyLong_FromLong(nibble_mx_matmul_dense(X, M, rs, xdt, wc, ws, N, K, dt, Y, work,
+                                                (size_t)(bytes < 0 ? 0 : bytes), stream));
 }
 
-/* mx_matmul_takes_dense(M, N, K) */
-static PyObject* py_mx_takes_dense(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+/* mx_matmul_dense_workspace_bytes(M, N, K, aligned) */
+static PyObject* py_mx_dense_ws(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   (void)self;
-  if (!nargs_is(n, 3, "mx_matmul_takes_dense")) return NULL;
+  if (!nargs_is(n, 4, "mx_matmul_dense_workspace_bytes")) return NULL;
   long long M, N, K;
-  if (!take_i64(a[0], &M) || !take_i64(a[1], &N) || !take_i64(a[2], &K)) return NULL;
-  return PyBool_FromLong(nibble_mx_matmul_takes_dense(M, N, K));
+  const int aligned = PyObject_IsTrue(a[3]);
+  if (aligned < 0 || !take_i64(a[0], &M) || !take_i64(a[1], &N) || !take_i64(a[2], &K)) return NULL;
+  return PyLong_FromSize_t(nibble_mx_matmul_dense_workspace_bytes(M, N, K, aligned));
 }
 
 /* gemm_strip_major(X, xr, xc, Wt, St, K, N, g, sw, version, Y, ws, ws_bytes, stream) */
@@ -574,8 +578,8 @@ static PyMethodDef kMethods[] = {
     {"mx_matmul", (PyCFunction)(void (*)(void))py_mx_matmul, METH_FASTCALL, "nibble_mx_matmul"},
     {"mx_matmul_dense", (PyCFunction)(void (*)(void))py_mx_matmul_dense, METH_FASTCALL,
      "nibble_mx_matmul_dense"},
-    {"mx_matmul_takes_dense", (PyCFunction)(void (*)(void))py_mx_takes_dense, METH_FASTCALL,
-     "nibble_mx_matmul_takes_dense"},
+    {"mx_matmul_dense_workspace_bytes", (PyCFunction)(void (*)(void))py_mx_dense_ws, METH_FASTCALL,
+     "nibble_mx_matmul_dense_workspace_bytes"},
     {"gemm_strip_major", (PyCFunction)(void (*)(void))py_sm_gemm, METH_FASTCALL,
      "nibble_gemm_w4a16_strip_major"},
     {"dequant_strip_major", (PyCFunction)(void (*)(void))py_sm_dequant, METH_FASTCALL,

@@ -620,14 +620,14 @@ extern "C" int nibble_mx_dequantize(const void* codes, const void* scales, int64
   return ok();
 }
 
-extern "C" int nibble_mx_matmul(const void* x_codes, const void* x_scales, int64_t M,
-                                const void* w_codes, const void* w_scales, int64_t N, int64_t K,
-                                int64_t dtype, void* Y, void* stream_) {
+static int check_mx_matmul(const void* x_codes, const void* x_scales, int64_t M,
+                           const void* w_codes, const void* w_scales, int64_t N, int64_t K,
+                           int64_t dtype, const void* Y) {
   int rc = check_mx(M, K, dtype);
   if (rc != NIBBLE_OK) return rc;
   rc = check_mx(N, K, dtype);
   if (rc != NIBBLE_OK) return rc;
-  if (M == 0 || N == 0) return ok();
+  if (M == 0 || N == 0) return NIBBLE_OK;
   NIBBLE_CHECK(M <= 65535 * 64, "more than %d rows of x", 65535 * 64);
   NIBBLE_CHECK(ceil_div(M, 64) * ceil_div(N, 64) <= (1 << 30), "an output of %lld x %lld",
                (long long)M, (long long)N);
@@ -638,6 +638,15 @@ extern "C" int nibble_mx_matmul(const void* x_codes, const void* x_scales, int64
   NIBBLE_CHECK(aligned(x_codes, 16) && aligned(w_codes, 16) && aligned(x_scales, 4) &&
                    aligned(w_scales, 4) && aligned(Y, 16),
                "misaligned pointer");
+  return NIBBLE_OK;
+}
+
+extern "C" int nibble_mx_matmul(const void* x_codes, const void* x_scales, int64_t M,
+                                const void* w_codes, const void* w_scales, int64_t N, int64_t K,
+                                int64_t dtype, void* Y, void* stream_) {
+  const int rc = check_mx_matmul(x_codes, x_scales, M, w_codes, w_scales, N, K, dtype, Y);
+  if (rc != NIBBLE_OK) return rc;
+  if (M == 0 || N == 0) return ok();
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   DeviceGuard guard;
   int dev = 0;
@@ -654,34 +663,54 @@ extern "C" int nibble_mx_matmul(const void* x_codes, const void* x_scales, int64
 
 // Every workgroup quantises the whole of a dense x, so it is taken while that is
 // little: at most 4096 k a CU.  us, one launch / quantised before, in a graph and
-// as calls: 1 x 4096 x 1024 3.7 / 4.6, 7.5 / 15.1; 16 x 4096 x 4096 7.5 / 6.3, 7.8 /
-// 15.3; 16 x 12288 x 1024 7.7 / 5.8, 7.9 / 15.3; beyond it 1 x 12288 x 4096 10.5 /
-// 7.8, 10.0 / 14.7; 16 x 12288 x 4096 18.7 / 10.0, 17.8 / 15.0; 1 x 4096 x 14336
-// 14.2 / 8.8, 13.6 / 14.8; 16 x 12288 x 14336 64 / 28, 64 / 27.
-extern "C" int nibble_mx_matmul_takes_dense(int64_t M, int64_t N, int64_t K) {
+// as calls (of two launches in one call since, 11): 1 x 4096 x 1024 3.7 / 4.6, 7.5
+// / 15.1; 16 x 4096 x 4096 7.5 / 6.3, 7.8 / 15.3; 16 x 12288 x 1024 7.7 / 5.8, 7.9 /
+// 15.3; beyond it 1 x 12288 x 4096 10.5 / 7.8, 10.0 / 14.7; 16 x 12288 x 4096 18.7 /
+// 10.0, 17.8 / 15.0; 1 x 4096 x 14336 14.2 / 8.8, 13.6 / 14.8; 16 x 12288 x 14336 64
+// / 28, 64 / 27.
+static bool mx_takes_dense(int64_t M, int64_t N, int64_t K) {
   return M >= 1 && M <= 16 && N >= 1 && N <= 12288 && K >= 1 &&
          ceil_div(N, 4096) * K <= 4096;  // (the rows kernel's sizes: one workgroup for 16 rows of w)
 }
 
+extern "C" size_t nibble_mx_matmul_dense_workspace_bytes(int64_t M, int64_t N, int64_t K,
+                                                         int aligned) {
+  if (check_mx(M, K, 0) != NIBBLE_OK || check_mx(N, K, 0) != NIBBLE_OK || M == 0 || N == 0) return 0;
+  if (aligned != 0 && mx_takes_dense(M, N, K)) return 0;
+  return static_cast<size_t>(M) * (K / 2) + static_cast<size_t>(ceil_div(K, kMxGroup)) * M * 4;
+}
+
 extern "C" int nibble_mx_matmul_dense(const void* X, int64_t M, int64_t row_stride, int64_t x_dtype,
                                       const void* w_codes, const void* w_scales, int64_t N,
-                                      int64_t K, int64_t dtype, void* Y, void* stream_) {
+                                      int64_t K, int64_t dtype, void* Y, void* workspace,
+                                      size_t workspace_bytes, void* stream_) {
   int rc = check_mx(M, K, x_dtype);
   if (rc != NIBBLE_OK) return rc;
   rc = check_mx(N, K, dtype);
   if (rc != NIBBLE_OK) return rc;
   if (M == 0 || N == 0) return ok();
-  if (!nibble_mx_matmul_takes_dense(M, N, K))
-    return fail(NIBBLE_ERR_UNSUPPORTED,
-                "a dense x of %lld rows is quantised first for N=%lld, K=%lld", (long long)M,
-                (long long)N, (long long)K);
+  NIBBLE_CHECK(row_stride >= 0 && row_stride < (int64_t(1) << 40), "row_stride out of range");
+  const int64_t size = x_dtype == kMxF32 ? 4 : 2;
+  const bool rows16 = row_stride * size % 16 == 0 && aligned(X, 16) &&
+                      (M - 1) * row_stride + K < (int64_t(1) << 31) / size;
+  if (!rows16 || !mx_takes_dense(M, N, K)) {
+    const size_t need = nibble_mx_matmul_dense_workspace_bytes(M, N, K, 0);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+      return fail(NIBBLE_ERR_WORKSPACE, "a dense x needs %zu bytes of workspace, got %zu", need,
+                  workspace == nullptr ? size_t(0) : workspace_bytes);
+    if (!aligned(workspace, 16))
+      return fail(NIBBLE_ERR_WORKSPACE, "workspace must be 16-byte aligned");
+    uint8_t* const codes = need > 0 ? static_cast<uint8_t*>(workspace) : nullptr;
+    uint8_t* const scales = need > 0 ? codes + M * (K / 2) : nullptr;
+    // (the product's arguments are looked at before anything is launched)
+    rc = check_mx_matmul(codes, scales, M, w_codes, w_scales, N, K, dtype, Y);
+    if (rc != NIBBLE_OK) return rc;
+    rc = nibble_mx_quantize(X, M, K, row_stride, 1, x_dtype, codes, scales, stream_);
+    if (rc != NIBBLE_OK) return rc;
+    return nibble_mx_matmul(codes, scales, M, w_codes, w_scales, N, K, dtype, Y, stream_);
+  }
   NIBBLE_CHECK(X != nullptr && Y != nullptr && w_codes != nullptr && w_scales != nullptr,
                "null pointer");
-  const int64_t size = x_dtype == kMxF32 ? 4 : 2;
-  NIBBLE_CHECK(row_stride >= 0 && row_stride < (int64_t(1) << 40) && row_stride * size % 16 == 0 &&
-                   aligned(X, 16),
-               "every row of x must start on 16 bytes");
-  NIBBLE_CHECK(((M - 1) * row_stride + K) * size < (int64_t(1) << 31), "rows of x beyond 2^31 bytes");
   NIBBLE_CHECK(aligned(w_codes, 16) && aligned(w_scales, 4) && aligned(Y, 16), "misaligned pointer");
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   DeviceGuard guard;

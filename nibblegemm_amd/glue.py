@@ -309,7 +309,7 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     key = ("tree", B, T, n_heads, n_kv, D, max_seq)
     plan = _ws_plan.get(key)
     if plan is None:
-        plan = (ext.attention_tree_workspace_bytes(B, T, n_heads, n_kv, D, max_seq), 0)
+        plan = (ext.attention_tree_workspace_bytes(B, T, n_heads, n_kv, D, max_seq), -1)
         _ws_plan[key] = plan
     ws, ws_bytes = _workspace(plan, dev, _stream(dev))
     out = torch.empty_like(q)

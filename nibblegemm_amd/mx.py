@@ -37,7 +37,7 @@ from typing import Optional, Union
 import torch
 
 from . import _native
-from .ops import _call, _check_no_backward
+from .ops import _call, _check_no_backward, _stream, _workspace
 
 #: Values that share a scale, and blocks whose scales share a word.
 MX_BLOCK = 32
@@ -45,6 +45,10 @@ MX_GROUP = 128
 
 #: The values of the 16 codes.
 MX_VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0)
+
+#: Bytes of quantised activations that a stream's calls keep between them; a
+#: larger x gets a buffer of its own.
+_KEPT_BYTES = 16 << 20
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
@@ -222,13 +226,18 @@ def matmul_mx(x: Union[torch.Tensor, MXMatrix], w: MXMatrix,
     ext = _native.binding()
     N = w.rows
     y = torch.empty((M, N), dtype=out_dtype, device=dev)
-    if dense and ext.mx_matmul_takes_dense(M, N, K) and _rows_on_16_bytes(x):
+    if dense and (x.stride(1) != 1 or x.is_neg() or (M > 1 and x.stride(0) < 1)):
+        x, dense = quantize_mx(x), False
+    if dense:
+        need = ext.mx_matmul_dense_workspace_bytes(M, N, K, M <= 16 and _rows_on_16_bytes(x))
+        if need <= _KEPT_BYTES:
+            ws, ws_bytes = _workspace((need, -1), dev, _stream(dev))
+        else:
+            ws, ws_bytes = torch.empty(need, dtype=torch.uint8, device=dev), need
         _call(ext.mx_matmul_dense, dev, x.data_ptr(), M, x.stride(0) if M > 1 else K,
               _DTYPES[x.dtype], w.codes.data_ptr(), w.scales.data_ptr(), N, K, _DTYPES[out_dtype],
-              y.data_ptr())
+              y.data_ptr(), ws.data_ptr() if ws is not None else None, ws_bytes)
         return y
-    if dense:
-        x = quantize_mx(x)
     _call(ext.mx_matmul, dev, x.codes.data_ptr(), x.scales.data_ptr(), M, w.codes.data_ptr(),
           w.scales.data_ptr(), N, K, _DTYPES[out_dtype], y.data_ptr())
     return y
@@ -237,9 +246,9 @@ def matmul_mx(x: Union[torch.Tensor, MXMatrix], w: MXMatrix,
 def _rows_on_16_bytes(x: torch.Tensor) -> bool:
     """Whether a kernel may read the rows of ``x`` in pieces of 16 bytes."""
     size = x.element_size()
-    return (x.stride(1) == 1 and x.data_ptr() % 16 == 0 and not x.is_neg()
-            and (x.shape[0] == 1 or x.stride(0) * size % 16 == 0)
+    return (x.data_ptr() % 16 == 0 and (x.shape[0] == 1 or x.stride(0) * size % 16 == 0)
             and ((x.shape[0] - 1) * x.stride(0) + x.shape[1]) * size < 1 << 31)
+
 
 __all__ = ["MX_BLOCK", "MX_GROUP", "MX_VALUES", "MXMatrix", "dequantize_mx", "matmul_mx",
            "mx_from_blocks", "quantize_mx"]

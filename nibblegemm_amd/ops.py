@@ -160,7 +160,9 @@ def _capture_id(stream: int) -> int:
 def _workspace(plan: Tuple[int, int], device: torch.device,
                stream: int) -> Tuple[Optional[torch.Tensor], int]:
     """A zeroed buffer of at least ``plan[0]`` bytes whose leading
-    ``plan[1]`` bytes (split-K counters) are zero; None if no bytes needed."""
+    ``plan[1]`` bytes (split-K counters) are zero; None if no bytes needed.
+    Where ``plan[1]`` is -1 the contents do not matter and nothing is zeroed
+    (in a capture that would be a node of every replay)."""
     global _capture_entries
     nbytes, counter_bytes = plan
     if nbytes == 0:
@@ -177,7 +179,8 @@ def _workspace(plan: Tuple[int, int], device: torch.device,
             buf = _workspaces.get(wkey)
             if buf is None or buf.numel() < nbytes:
                 size = max(nbytes, 1 << 20)
-                buf = torch.zeros(size, dtype=torch.uint8, device=device)
+                make = torch.empty if counter_bytes < 0 else torch.zeros
+                buf = make(size, dtype=torch.uint8, device=device)
                 _workspaces[wkey] = buf
                 if capture != 0:
                     _capture_entries += 1

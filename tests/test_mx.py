@@ -13,7 +13,7 @@ import torch
 import nibblegemm_amd as ng
 from nibblegemm_amd import mx
 
-INVALID = 1
+INVALID, WORKSPACE = 1, 3
 P = 1 << 20  # aligned, never dereferenced
 dev = "cuda"
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
@@ -219,8 +219,8 @@ def test_library_rejections(call, needle):
     assert needle in ext.last_error()
 
 
-def dense(ext, X=P, M=2, rs=128, xdt=0, wc=P, ws=P, N=64, K=128, dt=0, Y=P):
-    return ext.mx_matmul_dense(X, M, rs, xdt, wc, ws, N, K, dt, Y, None)
+def dense(ext, X=P, M=2, rs=128, xdt=0, wc=P, ws=P, N=64, K=128, dt=0, Y=P, work=0, size=0):
+    return ext.mx_matmul_dense(X, M, rs, xdt, wc, ws, N, K, dt, Y, work, size, None)
 
 
 @pytest.mark.parametrize("kwargs,needle,status", [
@@ -230,13 +230,23 @@ def dense(ext, X=P, M=2, rs=128, xdt=0, wc=P, ws=P, N=64, K=128, dt=0, Y=P):
     (dict(M=-1), "negative", INVALID),
     (dict(X=0), "null", INVALID),
     (dict(ws=0), "null", INVALID),
-    (dict(rs=132), "16 bytes", INVALID),
-    (dict(rs=1 << 62), "16 bytes", INVALID),
-    (dict(X=P + 8), "16 bytes", INVALID),
-    (dict(rs=1 << 30), "2^31", INVALID),
+    (dict(rs=-1), "row_stride", INVALID),
+    (dict(rs=1 << 62), "row_stride", INVALID),
     (dict(wc=P + 8), "misaligned", INVALID),
-    (dict(M=17), "quantised first", 2),
-    (dict(N=1 << 20), "quantised first", 2),
+    # quantised into a workspace first
+    (dict(rs=132), "workspace, got 0", WORKSPACE),
+    (dict(X=P + 8), "workspace, got 0", WORKSPACE),
+    (dict(rs=1 << 30), "workspace, got 0", WORKSPACE),
+    (dict(M=17), "workspace, got 0", WORKSPACE),
+    (dict(M=17, size=1 << 20), "workspace, got 0", WORKSPACE),
+    (dict(M=17, work=P, size=17 * 68 - 1), "needs 1156 bytes", WORKSPACE),
+    (dict(N=1 << 20, work=P, size=100), "workspace, got 100", WORKSPACE),
+    (dict(M=17, work=P + 8, size=1 << 20), "16-byte", WORKSPACE),
+    (dict(M=17, work=P, size=1 << 20, X=0), "null", INVALID),
+    (dict(M=17, work=P, size=1 << 20, X=P + 1), "misaligned", INVALID),
+    (dict(M=17, work=P, size=1 << 20, Y=P + 8), "misaligned", INVALID),
+    (dict(M=17, work=P, size=1 << 20, ws=0), "null", INVALID),
+    (dict(M=17, work=P, size=1 << 20, rs=0), "strides", INVALID),
 ])
 def test_dense_rejections(kwargs, needle, status):
     ext = ng.extension()
@@ -244,13 +254,15 @@ def test_dense_rejections(kwargs, needle, status):
     assert needle in ext.last_error()
 
 
-def test_where_a_dense_x_is_taken():
-    takes = ng.extension().mx_matmul_takes_dense
-    assert takes(1, 1024, 4096) and takes(16, 4096, 4096) and takes(1, 12288, 32)
-    assert not takes(17, 1024, 4096) and not takes(1, 28672, 4096)
-    assert not takes(1, 4097, 4096) and not takes(1, 4096, 4128) and not takes(1, 12289, 1024)
-    assert takes(16, 12288, 1024) and takes(5, 8192, 2048)
-    assert not takes(0, 1024, 4096) and not takes(1, 0, 4096) and not takes(1, 64, 0)
+def test_dense_workspace():
+    need = ng.extension().mx_matmul_dense_workspace_bytes
+    for M, N, K in [(1, 1024, 4096), (16, 4096, 4096), (1, 12288, 32), (16, 12288, 1024), (5, 8192, 2048)]:
+        assert need(M, N, K, True) == 0  # one launch
+        assert need(M, N, K, False) == M * (K // 2 + -(-K // 128) * 4)
+    for M, N, K in [(17, 1024, 4096), (1, 28672, 4096), (1, 4097, 4096), (1, 4096, 4128), (1, 12289, 1024)]:
+        assert need(M, N, K, True) == need(M, N, K, False) == M * (K // 2 + -(-K // 128) * 4)
+    assert need(0, 64, 128, True) == need(64, 0, 128, True) == need(64, 64, 0, False) == 0
+    assert need(17, 64, 100, True) == 0  # a refused product
 
 
 def test_library_takes_empty_sizes():
@@ -492,6 +504,39 @@ def test_product_refusals_on_the_gpu():
         ng.matmul_mx(torch.zeros((2, 128), device=dev, requires_grad=True), w)
     with pytest.raises(RuntimeError, match="out_dtype"):
         ng.matmul_mx(x, w, torch.float64)
+
+
+@pytest.mark.gpu
+def test_quantised_activations_are_not_mixed_up():
+    """Calls of different sizes on one stream share a workspace; calls on two
+    streams, two graphs and one beyond what is kept do not."""
+    w = ng.quantize_mx((sample(256, 512, F32, seed=4) * 0.02).to(dev))
+    big = torch.zeros((70_000, 512), dtype=F16, device=dev)  # 19 MB of codes and scales
+    big[:300] = sample(300, 512, F16, seed=3).to(dev)
+    xs = [big[:300].clone(), big[:40].clone(), big[:18] * 2]
+    want = [ng.matmul_mx(ng.quantize_mx(x), w) for x in xs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        got = [ng.matmul_mx(x, w) for x in xs]
+        with torch.cuda.stream(side):
+            other = [ng.matmul_mx(x, w) for x in reversed(xs)]
+    torch.cuda.synchronize()
+    for g, o, y in zip(got, reversed(other), want):
+        assert torch.equal(g, y) and torch.equal(o, y)
+    assert torch.equal(ng.matmul_mx(big, w)[:300], want[0])
+    graphs, ys = [], []
+    for x in xs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            ys.append(ng.matmul_mx(x, w))
+    for _ in range(3):
+        for graph in graphs:
+            graph.replay()
+        assert torch.equal(ng.matmul_mx(xs[1], w), want[1])
+        torch.cuda.synchronize()
+        for y, z in zip(ys, want):
+            assert torch.equal(y, z)
 
 
 @pytest.mark.gpu
