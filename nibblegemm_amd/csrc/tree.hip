@@ -34,6 +34,13 @@ constexpr int kTreeThreads = 256;
 constexpr int kTreeKeys = 64;        // keys of a tile
 constexpr int kTreeMaxSplits = 64;   // of one sequence
 constexpr int kTreeWorkgroups = 512;  // two a CU
+// What a share more costs, in the time of a tile: the join's turn, and a query
+// row's sums written and read again.  us with these / with as many shares as there
+// is room for: 1 x 100 tokens (32 heads on 8) over 1000 21.8 / 27.7, 1 x 64 over 4000
+// 27 / 30, 1 x 16 over 8000 20 / 25.5, 4 x 30 over 1000 23.8 / 29.4, 1 x 1 over 4000
+// 10.6 / 13.9 (13.8 with half the first); half the second -7 to +19%, twice it 2 to
+// 14% slower.
+constexpr float kTreeShareCost = 0.08f, kTreeRowCost = 4.8e-4f;
 constexpr float kLog2e = 1.4426950408889634f;
 // A query's reference maximum moves only when a score passes it by this much
 // (in powers of two): until then its probabilities stay below 2^8, which the
@@ -54,6 +61,7 @@ struct TreeArgs {
   int64_t mask_batch;  // bytes between two sequences' masks
   int B, T, n_heads, n_kv, qpk, seq;
   int shares, row_tiles;  // shares: 0 where no sequence's rows are split
+  float join_cost;        // of one share, in tiles
   bool fold;              // row tiles from both ends to the middle
   float scale;  // its magnitude times log2(e); 1 for a scale of zero
   float sign;   // its sign
@@ -107,7 +115,8 @@ struct TreeShares {
   __device__ __forceinline__ TreeShares(const TreeArgs& a, int want) {
     if (a.B == 1) {
       const int all = tiles(a, 0);
-      per = max((all + a.shares - 1) / a.shares, max((all + kTreeMaxSplits - 1) / kTreeMaxSplits, 1));
+      per = max((all + a.shares - 1) / a.shares,
+                max((all + kTreeMaxSplits - 1) / kTreeMaxSplits, worth(a, static_cast<float>(all))));
       count = shares_of(all);
       found = want < count ? 0 : -1;
       return;
@@ -125,8 +134,9 @@ struct TreeShares {
       }
     }
     const int most = static_cast<int>(wave_max(most_f));
-    per = static_cast<int>(ceilf(wave_sum(total) / static_cast<float>(a.shares)));
-    per = max(max(per, (most + kTreeMaxSplits - 1) / kTreeMaxSplits), 1);
+    total = wave_sum(total);
+    per = static_cast<int>(ceilf(total / static_cast<float>(a.shares)));
+    per = max(max(per, (most + kTreeMaxSplits - 1) / kTreeMaxSplits), worth(a, total));
     per = __builtin_amdgcn_readfirstlane(per);
     int high = max(per, most);  // enough: one share each
     for (int low = per; low < high;) {
@@ -161,6 +171,11 @@ struct TreeShares {
         }
         before += __builtin_amdgcn_readlane(upto, 63);
       }
+  }
+  // per tiles in turn, and total / per shares whose sums are written and joined:
+  // the least of per + join_cost total / per.
+  static __device__ __forceinline__ int worth(const TreeArgs& a, float total) {
+    return max(static_cast<int>(__builtin_amdgcn_sqrtf(a.join_cost * total)), 1);
   }
   static __device__ __forceinline__ int tiles(const TreeArgs& a, int b) {
     return (TreeSpan(a, b).total + kTreeKeys - 1) / kTreeKeys;
@@ -809,6 +824,7 @@ extern "C" int nibble_attention_tree(const void* Q, int64_t dtype, int64_t batch
   a.seq = static_cast<int>(max_seq);
   a.shares = p.shares;
   a.row_tiles = p.row_tiles;
+  a.join_cost = kTreeShareCost + kTreeRowCost * static_cast<float>(tokens * n_heads);
   a.fold = mask == nullptr && batch * n_kv_heads * p.row_tiles <= kTreeWorkgroups;
   a.scale = scale == 0.0f ? 1.0f : std::fabs(scale) * kLog2e;
   a.sign = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;

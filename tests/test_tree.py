@@ -365,6 +365,8 @@ def test_qk_one_sequence_and_refusals():
     (1, 70, 8, 1, 64, [40], 64),          # 560 rows: three workgroups
     (1, 65, 8, 2, 128, [600], 0),         # 260 rows: four of them in a second one
     (1, 2, 7, 1, 128, [3000], 30),        # an odd group of heads, several splits
+    (1, 2, 4, 2, 64, [20000], 0),         # 63 splits
+    (2, 3, 2, 1, 64, [20000, 0], 0),
 ])
 def test_tree_attention(B, T, n_heads, n_kv, D, lengths, extra, masked, dtype):
     check_tree(*tree_case(B, T, n_heads, n_kv, D, max(lengths) + T + extra, dtype, lengths, masked,
