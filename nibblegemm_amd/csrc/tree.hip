@@ -188,8 +188,8 @@ struct TreeShares {
 // keys.  A tile's rows of k and v are copied straight into one of two LDS
 // buffers while the tile before it is computed; two workgroups share a CU.
 //
-// What bounds it: 64 tokens over 65000 take 89 us of this kernel (16 sequences of
-// 27 over up to 8100 86, 4.2 TB/s; 2048 over 2048 120 to 127, 0.83 PFLOP/s).  A tile of
+// What bounds it: 64 tokens over 65000 take 85 us of this kernel (16 sequences of
+// 27 over up to 8100 86, 4.2 TB/s; 2048 over 2048 112, 0.92 PFLOP/s).  A tile of
 // a wave is 68 products of 16 cycles and 32 exponentials of 16 beside some 130
 // plain vector operations of 4; for the two waves of a SIMD that adds up to 4300
 // cycles, and a tile takes 4375: the two hardly overlap.  Neither a priority for
@@ -201,9 +201,9 @@ struct TreeShares {
 // Three workgroups a CU (smaller tiles) took 283 us for the last of those, 64
 // queries a wave, which would halve the reads of LDS, 519 (registers spilt).
 //
-// One call of 16 tokens over 1000 is latency: 7.7 us, of which finding its share
-// and loading the queries take 2.3, the copies 0.9, one tile 1.4, the meeting of
-// the waves and the stores 2.9 (4.5 with a barrier for each 16 rows).
+// One call of 16 tokens over 1000 is latency: 8.4 us, of which finding its share
+// and loading the queries take 2.3, the copies 0.9, each of two tiles 1.2, the
+// meeting of the waves and the stores 2.9 (4.5 with a barrier for each 16 rows).
 template <class E, int D, int QT, int WK>
 __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   using T = typename E::type;
@@ -628,8 +628,8 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
 // Joins the shares of a row: D / 4 lanes a row, four outputs each, the rows of
 // one (sequence, kv head) in a workgroup.  The lanes read the shares' statistics
 // together; the sums are then loaded eight shares at a time, those of shares
-// that saw nothing not at all.  Memory and latency bound it: 64 rows of 16 shares
-// and 8 kv heads 3.9 us, 256 rows of 32 shares 8 us, 34 MB (loads begun before
+// that saw nothing not at all.  Memory and latency bound it: 64 rows of 8 shares
+// and 8 kv heads 2.8 us, 256 rows of 32 shares 8 us, 34 MB (loads begun before
 // the statistics are there gained 0.6 us on the first, lost 2 on ragged trees).
 template <class E, int D>
 __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(TreeArgs a) {
