@@ -42,10 +42,18 @@ constexpr int kTreeWorkgroups = 512;  // two a CU
 // 14% slower.
 constexpr float kTreeShareCost = 0.08f, kTreeRowCost = 4.8e-4f;
 constexpr float kLog2e = 1.4426950408889634f;
-// A query's reference maximum moves only when a score passes it by this much
-// (in powers of two): until then its probabilities stay below 2^8, which the
-// 16-bit types hold, and its sums need no rescaling.
+// Probabilities are relative to a query's reference, 2^lift below a maximum.  It
+// moves only when a score passes that maximum by more than the slack (in powers of
+// two): until then they are at most 2^(slack + lift), and the sums need no
+// rescaling.  fp16 ends at 2^16 and has steps of 2^-24 at least, so its reference
+// lies as low as it can: weights down to 2^-21 of the largest keep all their bits,
+// and thousands of 2^-25, which a sink leaves to the rest, are not lost.  (A slack
+// of 4 and a lift of 11: 4 x 8 tokens over 3000, 32 heads of 64 on 4, 16.2 us in
+// place of 15.7; 16 x 27 over 8100 105.8 in place of 103.)  bf16 has the range of
+// fp32.
 constexpr float kTreeSlack = 8.0f;
+template <class E>
+constexpr float kTreeLift = std::is_same_v<E, Half> ? 7.0f : 0.0f;
 
 struct TreeArgs {
   const void* q;  // [B, T, n_heads, D]
@@ -312,7 +320,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   copy(0);
 
   f4_t acc[QT][D / 16];
-  float top[QT];  // of query c, times the scale
+  float top[QT];  // the reference of query c, in powers of two
   f4_t sum[QT];   // of the probabilities: four copies
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -409,11 +417,11 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   auto move = [&]() {
     bool moves = false;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) moves |= m[t] > top[t] + kTreeSlack;
+    for (int t = 0; t < QT; ++t) moves |= m[t] > top[t] + (kTreeSlack + kTreeLift<E>);
     if (!__any(moves)) return;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      const float up = fmaxf(swap_max(m[t]), top[t]);
+      const float up = fmaxf(swap_max(m[t]) - kTreeLift<E>, top[t]);
       const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - up);
       top[t] = up;
 #pragma unroll
@@ -439,7 +447,8 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
                        : 0.0f);
       }
       // (The probabilities are rounded to 16 bits because the matrix cores take
-      // them so: each is off by half a step at most, and the sum is of the rounded.)
+      // them so: each is off by half a step at most, in fp16 of 2^-24 at least, and the
+      // sum is of the rounded.)
       // The sum of the probabilities as they are multiplied, by the matrix cores
       // too: ones times P^T, a tile's keys at once, in fp32.
 #pragma unroll

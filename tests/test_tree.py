@@ -672,3 +672,52 @@ def test_a_layer_verifies_a_tree(dtype):
         want = layer(xs, k2, v2, pos, slots, mask, lengths)
         torch.cuda.synchronize()
         assert torch.equal(out[3], want[3]) and torch.equal(kg, k2) and torch.equal(vg, v2)
+
+
+# ---------------------------------------------------------------------------
+# rows of very different weight
+# ---------------------------------------------------------------------------
+def far_case(T, n_heads, D, S, n, dtype, nats, at, seed=0):
+    """Scores of 0 but for row ``at``, the sink, whose score is ``nats``; its
+    values are zero and the others' near one."""
+    g = torch.Generator().manual_seed(seed)
+    q = torch.zeros((1, T, n_heads, D), dtype=dtype)
+    q[..., 3] = 4.0
+    k = torch.randn((1, 1, S, D), generator=g).to(dtype)
+    k[..., 3] = 0.0
+    k[0, 0, at, 3] = nats / 4
+    assert k[0, 0, at, 3].item() == nats / 4
+    v = (1 + 0.25 * torch.randn((1, 1, S, D), generator=g)).to(dtype)
+    v[0, 0, at] = 0.0
+    return q, k, v, torch.tensor([n], dtype=torch.int32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nats", [10, 14, 17, 17.5, 19])
+@pytest.mark.parametrize("T,n_heads,n,at", [
+    (1, 1, 200, 0), (1, 4, 8192, 0), (1, 4, 8192, 8000), (6, 4, 8192, 70), (12, 4, 8000, 7990),
+    (40, 4, 8192, 100), (40, 4, 250, 5), (3, 4, 60000, 1), (40, 2, 60000, 59990)])
+def test_small_weights_of_many_rows_add_up(T, n_heads, n, at, nats, dtype):
+    """One row outweighs each of thousands by far, and they are what is left of
+    the output.  A probability is rounded in its type, fp16's in steps of 2^-24
+    at least, where the largest is 2^7 or more: each row's weight is off by half
+    a step of its own, or by 2^-25 of 2^7.  An error d of a row's weight moves
+    the output by d (v - out).  (bf16's least step is below all of this.)"""
+    D = 128
+    q, k, v, lengths = far_case(T, n_heads, D, n + T, n, dtype, nats, at)
+    got = run_tree(q, k, v, lengths, scale=1.0).cpu().double()
+    info = torch.finfo(dtype)
+    for i in range(T):
+        s = torch.zeros(n + i + 1, dtype=torch.float64)
+        s[at] = nats
+        w, vv = torch.softmax(s, 0), v[0, 0, :n + i + 1].double()
+        want = w @ vv
+        apart = (vv - want).abs()
+        # rounded weights; fp32 scores (exact but for the factor log2 e), exponentials, sums
+        off = w @ apart * (info.eps / 2 + (nats + 2) * 2.0 ** -22 + 2.0 ** -20)
+        if dtype == F16:
+            off = off + 2.0 ** -32 * apart.sum(0)
+        off = off + (want.abs() + off) * info.eps / 2 + info.smallest_normal * info.eps
+        for h in range(n_heads):
+            assert ((got[0, i, h] - want).abs() <= off).all(), (i, h)
