@@ -481,9 +481,10 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   };
   // The sums.  A hidden row's infinity or NaN must not meet its zero
   // probability: with `careful` they are left out of the products and counted,
-  // over the rows a query gives any weight, by products of their own: infinities
-  // of either sign, a NaN as both.  A query and element that met one gets that
-  // infinity added, and of both the NaN that they make.
+  // over the rows a query sees, by products of their own: infinities of either
+  // sign, a NaN as both.  A query and element that met one gets that infinity
+  // added, and of both the NaN that they make; a weight that rounds to zero takes
+  // neither away (in a tile that all see it makes NaN of an infinity).
   auto add = [&](int buf, auto careful) {
     constexpr bool kCareful = decltype(careful)::value;
     const uint32_t vt = lds_address(kv[buf][1]) + wk * KPW * D * 2;
@@ -505,7 +506,8 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
         for (int t = 0; t < QT; ++t)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            p[j][t][e] = static_cast<T>(static_cast<float>(p[j][t][e]) != 0.0f ? 1.0f : 0.0f);
+            p[j][t][e] = static_cast<T>(
+                8 * j + e < 4 * KS && (seen[t] >> (8 * j + e) & 1u) != 0 ? 1.0f : 0.0f);
       const us8_t one = __builtin_bit_cast(us8_t, ones);
 #pragma unroll
       for (int d = 0; d < D / 16; ++d)
@@ -547,6 +549,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
     weigh(x);
     if constexpr (decltype(tail)::value) {
       if (strange(i)) {
+        look(i);  // (again, so that its bits need no registers meanwhile: 15 x 444 -2.5%)
         add(buf, std::true_type{});
         return;
       }
@@ -637,7 +640,8 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
 // Joins the shares of a row: D / 4 lanes a row, four outputs each, the rows of
 // one (sequence, kv head) in a workgroup.  The lanes read the shares' statistics
 // together; the sums are then loaded eight shares at a time, those of shares
-// that saw nothing not at all.  Memory and latency bound it: 64 rows of 8 shares
+// that saw nothing not at all (a share of no weight counts: an infinity or a NaN in
+// its sums must not be lost).  Memory and latency bound it: 64 rows of 8 shares
 // and 8 kv heads 2.8 us, 256 rows of 32 shares 8 us, 34 MB (loads begun before
 // the statistics are there gained 0.6 us on the first, lost 2 on ragged trees).
 template <class E, int D>
@@ -670,7 +674,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(TreeArgs a) {
   for (int u = 0; u < PER; ++u) {
     const float keep = tops[u] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(tops[u] - m);
     l += w[u] * keep;
-    w[u] = keep;
+    w[u] = tops[u] == -INFINITY ? -1.0f : keep;  // (negative: no sums)
   }
 #pragma unroll
   for (int x = LANES / 2; x > 0; x /= 2) l += __shfl_xor(l, x, LANES);
@@ -684,7 +688,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(TreeArgs a) {
       for (int e = 0; e < 8; ++e) {
         k[e] = __shfl(w[u], s0 + e, LANES);
         v[e] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        if (k[e] != 0.0f)
+        if (!(k[e] < 0.0f))
           v[e] = *reinterpret_cast<const f4_t*>(
               a.partial + (rec0 + static_cast<int64_t>(u * LANES + s0 + e) * rows_all) * D + d);
       }

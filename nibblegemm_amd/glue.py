@@ -278,7 +278,9 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 
     Tokens behind a sequence's last, and tokens that see nothing, give zeros.
     Rows that a token does not see have no part in its output, whatever they
-    hold; rows behind the tree are not read.  ``lengths`` and ``sizes`` count
+    hold; rows behind the tree are not read.  An infinity in the values of a row
+    that it sees comes out as it is, or as NaN where the row's weight rounds to
+    zero; a NaN as NaN.  ``lengths`` and ``sizes`` count
     as far as the cache goes.  One sequence may come without its batch
     dimension: q [T, ..], caches [n_kv, max_seq, D], lengths [1], sizes [1].
     Lengths, sizes and mask are read on the GPU, so a captured call follows

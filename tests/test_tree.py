@@ -721,3 +721,27 @@ def test_small_weights_of_many_rows_add_up(T, n_heads, n, at, nats, dtype):
         off = off + (want.abs() + off) * info.eps / 2 + info.smallest_normal * info.eps
         for h in range(n_heads):
             assert ((got[0, i, h] - want).abs() <= off).all(), (i, h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nats", [40, 120])
+@pytest.mark.parametrize("T,n_heads", [(3, 1), (3, 4), (8, 4), (16, 4), (40, 4)])
+def test_strange_values_of_no_weight(T, n_heads, nats, dtype):
+    """An infinity or a NaN in a row that a token sees is not lost where the
+    row's weight rounds to zero, wherever the row lies: among other cached rows,
+    in the last tile of them, or in the tree; and it reaches nobody else."""
+    D, inf, nan = 64, float("inf"), float("nan")
+    mask = torch.ones((1, T, T)).tril().bool()
+    mask[0, :, 1] = torch.arange(T) % 2 == 1
+    for n, at in ((60, 3), (199, 3), (199, 197), (3000, 2), (3000, 2990)):
+        q, k, v, lengths = far_case(T, n_heads, D, n + T, n, dtype, nats, at)
+        v[0, 0, 10, 5], v[0, 0, 11, 6], v[0, 0, n - 1, 7], v[0, 0, n - 1, 8] = inf, nan, -inf, nan
+        v[0, 0, n + 1, 9], v[0, 0, n + 1, 10] = inf, nan
+        got = run_tree(q, k, v, lengths, mask, scale=1.0).cpu()
+        bad = ~got.isfinite()
+        want = torch.zeros((1, T, n_heads, D), dtype=torch.bool)
+        want[..., 5:9] = True
+        want[:, 1::2, :, 9:11] = True
+        assert torch.equal(bad, want), (n, at)
+        assert got[..., [6, 8]].isnan().all() and got[:, 1::2, :, 10].isnan().all()
