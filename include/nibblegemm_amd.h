@@ -457,7 +457,9 @@ NIBBLE_API int nibble_qk_norm_rope(const void* QKV, int64_t dtype, int64_t batch
  * rows and the tree tokens j with mask[b][i][j] != 0 (uint8 [mask_batches,
  * tokens, tokens], mask_batches 1 or batch; NULL: j <= i).  Out [batch, tokens,
  * n_heads head_dim] = softmax(scale q k^T) v, zeros for tokens that see nothing
- * and behind a tree's last.  Row strides are at most 2^22 elements.  The
+ * and behind a tree's last.  Row strides are at most 2^22 elements; batch and
+ * heads at most 65535, tokens 2^20, batch tokens n_heads 2^30, and a launch ends at
+ * 2^24 - 1 workgroups, one a sequence, kv head and up to 128 of its query rows.  The
  * workspace (nibble_attention_tree_workspace_bytes, 256-byte aligned; NULL when
  * that is 0) needs no initial contents. */
 NIBBLE_API int nibble_attention_tree(const void* Q, int64_t dtype, int64_t batch, int64_t tokens,

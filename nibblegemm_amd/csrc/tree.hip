@@ -732,6 +732,9 @@ int plan_tree(int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv, int6
   p->form = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
   p->rows = 16 << p->form;
   p->row_tiles = static_cast<int>(ceil_div(rows, p->rows));
+  NIBBLE_CHECK(ceil_div(batch * n_kv, 8) * 8 * p->row_tiles * kTreeThreads < (int64_t(1) << 32),
+               "%lld sequences of %lld kv heads: a launch ends at 2^32 threads", (long long)batch,
+               (long long)n_kv);
   // Room for more workgroups than there are (sequence, kv head, row tile)s: the
   // cached rows are split, unless there are but a few tiles of them.
   const int64_t room = kTreeWorkgroups / (n_kv * p->row_tiles);

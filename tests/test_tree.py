@@ -745,3 +745,14 @@ def test_strange_values_of_no_weight(T, n_heads, nats, dtype):
         want[:, 1::2, :, 9:11] = True
         assert torch.equal(bad, want), (n, at)
         assert got[..., [6, 8]].isnan().all() and got[:, 1::2, :, 10].isnan().all()
+
+
+@pytest.mark.parametrize("kwargs,needle", [
+    (dict(B=65535, T=1, nh=512, nkv=512, D=64), "2^32 threads"),
+    (dict(B=65535, T=3, nh=65535, nkv=257, D=64), "2^30 query rows"),
+])
+def test_tree_rejects_what_no_launch_holds(kwargs, needle):
+    ext = ng.extension()
+    assert tree(ext, **kwargs) == INVALID
+    assert needle in ext.last_error()
+    assert ext.attention_tree_workspace_bytes(65535, 1, 512, 512, 64, 16) == 0
