@@ -457,11 +457,12 @@ NIBBLE_API int nibble_qk_norm_rope(const void* QKV, int64_t dtype, int64_t batch
  * rows and the tree tokens j with mask[b][i][j] != 0 (uint8 [mask_batches,
  * tokens, tokens], mask_batches 1 or batch; NULL: j <= i).  Out [batch, tokens,
  * n_heads head_dim] = softmax(scale q k^T) v, zeros for tokens that see nothing
- * and behind a tree's last.  Row strides are at most 2^22 elements; batch and
- * heads at most 65535, tokens 2^20, batch tokens n_heads 2^30, and a launch ends at
- * 2^24 - 1 workgroups, one a sequence, kv head and up to 128 of its query rows.  The
- * workspace (nibble_attention_tree_workspace_bytes, 256-byte aligned; NULL when
- * that is 0) needs no initial contents. */
+ * and behind a tree's last.  scale is finite, also times log2(e).  Row strides
+ * are at most 2^22 elements; batch and heads at most 65535, tokens 2^20, batch
+ * tokens n_heads 2^30, and a launch ends at 2^24 - 1 workgroups, one a sequence,
+ * kv head and up to 128 of its query rows.  The workspace
+ * (nibble_attention_tree_workspace_bytes, 256-byte aligned; NULL when that is 0)
+ * needs no initial contents. */
 NIBBLE_API int nibble_attention_tree(const void* Q, int64_t dtype, int64_t batch, int64_t tokens,
                                      int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
                                      const void* K_cache, int64_t k_batch_stride,

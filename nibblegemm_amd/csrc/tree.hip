@@ -789,7 +789,7 @@ extern "C" int nibble_attention_tree(const void* Q, int64_t dtype, int64_t batch
   TreePlan p;
   const int rc = plan_tree(batch, tokens, n_heads, n_kv_heads, head_dim, max_seq, &p);
   if (rc != NIBBLE_OK) return rc;
-  NIBBLE_CHECK(std::isfinite(scale), "scale must be finite");
+  NIBBLE_CHECK(std::isfinite(scale * kLog2e), "scale must be finite, also times log2(e)");
   if (batch == 0 || tokens == 0) return ok();
   for (int64_t s : {k_batch_stride, k_head_stride, k_row_stride, v_batch_stride, v_head_stride,
                     v_row_stride})

@@ -756,3 +756,10 @@ def test_tree_rejects_what_no_launch_holds(kwargs, needle):
     assert tree(ext, **kwargs) == INVALID
     assert needle in ext.last_error()
     assert ext.attention_tree_workspace_bytes(65535, 1, 512, 512, 64, 16) == 0
+
+
+@pytest.mark.parametrize("scale", [3e38, -3e38, float("nan"), 1e39])
+def test_tree_rejects_a_scale_beyond_fp32(scale):
+    ext = ng.extension()
+    assert tree(ext, scale=scale) == INVALID
+    assert "scale" in ext.last_error()
