@@ -23,6 +23,9 @@ namespace {
 constexpr int kMxF16 = 0, kMxBF16 = 1, kMxF32 = 2;
 constexpr int kMxBlock = 32;   // k of one scale
 constexpr int kMxGroup = 128;  // k of one word of scales
+// Workgroups along a grid's first dimension, where there may be many: one dimension
+// ends at 2^32 threads.
+constexpr int64_t kMxGrid = 1 << 20;
 
 typedef int i8_t __attribute__((ext_vector_type(8)));
 typedef unsigned short us8_t __attribute__((ext_vector_type(8)));
@@ -102,8 +105,9 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const typename MxElem<
                                                           int col_tiles) {
   using E = MxElem<DT>;
   const int lane = threadIdx.x & 63;
-  const int64_t tile = blockIdx.x / col_tiles;
-  const int group = static_cast<int>(blockIdx.x % col_tiles) * 4 + (threadIdx.x >> 6);
+  const uint32_t block = blockIdx.y * static_cast<uint32_t>(kMxGrid) + blockIdx.x;
+  const int64_t tile = block / col_tiles;
+  const int group = static_cast<int>(block % col_tiles) * 4 + (threadIdx.x >> 6);
   const int j = lane & 15;
   const int k = group * kMxGroup + 8 * j;
   const int64_t row0 = tile * kMxRows + (lane >> 4);
@@ -244,8 +248,6 @@ __device__ __forceinline__ f2_t mx_values2(uint32_t codes, uint32_t e) {
 // it has 32 bits.  Memory bounds it; what counts is that a wave's stores cover
 // 1 KiB without a gap and pass by the caches (28672 x 4096 in bf16: 43 us against
 // 60 with plain stores; in fp32 72 against 119, and 132 with 32 bytes a thread).
-// The grid has two dimensions because one ends at 2^32 threads.
-constexpr int64_t kMxDequantGrid = 1 << 20;
 template <int DT>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(const uint8_t* codes,
                                                             const uint8_t* scales, int64_t rows,
@@ -527,7 +529,9 @@ hipError_t launch_mx_quantize(const void* X, int64_t rows, int64_t K, int64_t ro
   const int k = static_cast<int>(K);
   if (k_stride == 1) {
     const int64_t tiles = ceil_div(K, 4 * kMxGroup);
-    const dim3 grid(static_cast<unsigned>(tiles * ceil_div(rows, kMxRows)));
+    const int64_t blocks = tiles * ceil_div(rows, kMxRows);
+    const int64_t across = std::min(blocks, kMxGrid);  // (behind the last block: rows that are not there)
+    const dim3 grid(static_cast<unsigned>(across), static_cast<unsigned>(ceil_div(blocks, across)));
     auto* c = static_cast<uint32_t*>(codes);
     auto* s = static_cast<uint32_t*>(scales);
     // 16-byte loads where every row starts on 16 bytes
@@ -605,7 +609,7 @@ extern "C" int nibble_mx_dequantize(const void* codes, const void* scales, int64
   const auto* c = static_cast<const uint8_t*>(codes);
   const auto* s = static_cast<const uint8_t*>(scales);
   const int64_t blocks = ceil_div(rows * (K / (dtype == kMxF32 ? 4 : 8)), 256);
-  const int64_t across = std::min(blocks, kMxDequantGrid);
+  const int64_t across = std::min(blocks, kMxGrid);
   const dim3 grid(static_cast<unsigned>(across), static_cast<unsigned>(ceil_div(blocks, across)));
   if (dtype == kMxF32)
     mx_dequantize_kernel<kMxF32><<<grid, 256, 0, stream>>>(c, s, rows, (int)K, static_cast<float*>(out));

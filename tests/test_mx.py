@@ -561,3 +561,20 @@ def test_product_on_another_stream_and_in_a_graph(M):
         torch.cuda.synchronize()
         assert torch.equal(y, want[i])
         assert torch.equal(ng.matmul_mx(xs[2], w), want[2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,K", [((1 << 27) + 9, 32), ((1 << 26) + 3, 544)])
+def test_quantize_more_than_a_grid_dimension_holds(rows, K):
+    """Rows whose workgroups have 2^32 threads and more together."""
+    if torch.cuda.mem_get_info()[0] < 4 * rows * K:
+        pytest.skip("not enough memory")
+    some = torch.tensor([0, 7, 8, 8388607, 8388608, (1 << 26) - 1, 1 << 26, rows - 2, rows - 1],
+                        device=dev)
+    x = torch.zeros((rows, K), dtype=BF16, device=dev)
+    x[some] = sample(len(some), K, BF16, seed=8).to(dev)
+    m = ng.quantize_mx(x)
+    want = ng.quantize_mx(x[some].contiguous())
+    assert torch.equal(m.codes[some], want.codes) and torch.equal(m.scales[:, some], want.scales)
+    other = torch.tensor([1, 8388609, 67108800, rows - 5], device=dev)
+    assert not m.codes[other].any() and not m.scales[:, other].any()
