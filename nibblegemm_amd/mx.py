@@ -145,6 +145,8 @@ def quantize_mx(x: torch.Tensor) -> MXMatrix:
     if x.is_neg():  # a view whose values are its memory's, negated
         x = x.resolve_neg()
     row_stride, k_stride = x.stride()
+    if rows == 1 and k_stride == 1:  # (whatever a single row's stride is)
+        row_stride = K
     if not (row_stride == 1 and k_stride > 1 or k_stride == 1 and row_stride > 0):
         x = x.contiguous()
         row_stride, k_stride = x.stride()

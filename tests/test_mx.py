@@ -578,3 +578,21 @@ def test_quantize_more_than_a_grid_dimension_holds(rows, K):
     assert torch.equal(m.codes[some], want.codes) and torch.equal(m.scales[:, some], want.scales)
     other = torch.tensor([1, 8388609, 67108800, rows - 5], device=dev)
     assert not m.codes[other].any() and not m.scales[:, other].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_one_row_of_any_stride(dtype):
+    """The stride over a single row does not matter, whatever it is."""
+    x = sample(5, 192, dtype, seed=6)
+    xd = x.to(dev)
+    w = ng.quantize_mx(sample(40, 192, F32, seed=7).to(dev))
+    want = ng.matmul_mx(ng.quantize_mx(xd[:1].clone()), w, F32)
+    for one in (xd[0].expand(5, 192)[:1], xd[0].expand(1, 192), xd[:1], xd.t().contiguous().t()[:1],
+                xd.as_strided((1, 192), (3, 1)), xd.as_strided((1, 192), (0, 1)),
+                xd.as_strided((1, 192), (1, 1))):
+        check_quantized(ng.quantize_mx(one), x[:1])
+        assert torch.equal(ng.matmul_mx(one, w, F32), want)
+    both = torch.zeros((5, 384), dtype=dtype, device=dev)
+    both[:, ::2] = xd
+    check_quantized(ng.quantize_mx(both[:1, ::2]), x[:1])
