@@ -20,6 +20,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _native
 from .ops import _call, _check_no_backward, _raise, _stream, _workspace, _ws_plan
@@ -112,6 +113,7 @@ def attention_decode(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
                        ws.data_ptr() if ws is not None else None, ws_bytes, stream)
     if rc:
         _raise(rc, ext)
+    increment_version((k_cache, v_cache))
     return out
 
 
@@ -253,6 +255,7 @@ def qk_norm_rope(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
           q_weight.data_ptr() if q_weight is not None else None,
           k_weight.data_ptr() if k_weight is not None else None, float(eps), cos_p, sin_p,
           rope_rows, out.data_ptr())
+    increment_version((k_cache, v_cache))  # (autograd may have saved one before)
     return out
 
 

@@ -763,3 +763,33 @@ def test_tree_rejects_a_scale_beyond_fp32(scale):
     ext = ng.extension()
     assert tree(ext, scale=scale) == INVALID
     assert "scale" in ext.last_error()
+
+
+@pytest.mark.gpu
+def test_written_caches_are_marked_as_changed():
+    """Autograd notices that a cache it has saved was written since."""
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn((1, 2, 4 * 128), generator=g).to(F16).to(dev)
+    at = torch.arange(2, dtype=torch.int32, device=dev)[None]
+    for which in range(2):
+        caches = [torch.ones((1, 1, 8, 128), dtype=F16, device=dev) for _ in range(2)]
+        before = [c._version for c in caches]
+        w = torch.ones(1, dtype=F16, device=dev, requires_grad=True)
+        y = (w * caches[which]).sum()
+        glue.qk_norm_rope(x, *caches, at, at)
+        assert [c._version > b for c, b in zip(caches, before)] == [True, True]
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    caches = [torch.ones((1, 1, 8, 128), dtype=F16, device=dev) for _ in range(2)]
+    before = [c._version for c in caches]
+    glue.attention_tree(x, *caches, at[0, :1])  # only reads
+    assert [c._version for c in caches] == before
+    caches = [torch.ones((1, 8, 128), dtype=F16, device=dev) for _ in range(2)]
+    before = [c._version for c in caches]
+    glue.attention_decode(x[0, :1], *caches, 3)
+    assert [c._version > b for c, b in zip(caches, before)] == [True, True]
+    with torch.inference_mode():
+        caches = [torch.ones((1, 1, 8, 128), dtype=F16, device=dev) for _ in range(2)]
+        glue.qk_norm_rope(x, *caches, at, at)
+    glue.qk_norm_rope(x, *caches, at, at)  # (such tensors count no versions)
+    glue.attention_decode(x[0, :1], caches[0][0], caches[1][0], 3)
