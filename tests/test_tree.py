@@ -793,3 +793,16 @@ def test_written_caches_are_marked_as_changed():
         glue.qk_norm_rope(x, *caches, at, at)
     glue.qk_norm_rope(x, *caches, at, at)  # (such tensors count no versions)
     glue.attention_decode(x[0, :1], caches[0][0], caches[1][0], 3)
+
+
+@pytest.mark.gpu
+def test_a_batch_of_none():
+    for T in (0, 3):
+        q = torch.zeros((0, T, 256), dtype=F16, device=dev)
+        c = torch.zeros((0, 1, 8, 64), dtype=F16, device=dev)
+        n = torch.zeros(0, dtype=torch.int32, device=dev)
+        i = torch.zeros((0, T), dtype=torch.int32, device=dev)
+        mask = torch.zeros((0, T, T), dtype=torch.bool, device=dev)
+        assert glue.attention_tree(q, c, c.clone(), n).shape == (0, T, 256)
+        assert glue.attention_tree(q, c, c.clone(), n, mask, n).shape == (0, T, 256)
+        assert glue.qk_norm_rope(q, c, c.clone(), i, i).shape == (0, T, 128)
