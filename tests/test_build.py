@@ -107,3 +107,47 @@ def test_direct_kernel_waits_match_its_loads(tmp_path):
         assert counts == [4 * words + 2 * copies + part, step - 2 - part, step, step, step], name
         assert n == 2 + part, name
     assert forms == 2 * 16  # tile forms and groups
+
+
+@pytest.mark.skipif(not os.path.exists(OBJDUMP), reason="llvm-objdump not installed")
+def test_mx_tile_kernel_waits_match_its_loads(tmp_path):
+    """The tiled product of 4-bit floats lets the copies of RING - 2 steps stay
+    in flight at its loop's wait, which is right only if a step is as many loads
+    as counted and no other memory operation (a register spilt to scratch, say)
+    is in the loop.  Seen in the built code, for every form and output type."""
+    lib = shutil.copy(build.LIB, tmp_path)
+    subprocess.run([OBJDUMP, "--offloading", lib], cwd=tmp_path, capture_output=True, check=True)
+    objects = [p for p in sorted(tmp_path.iterdir())
+               if "gfx950" in p.name and b"mx_tile_kernel" in p.read_bytes()]
+    assert len(objects) == 1
+    text = subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", str(objects[0])], capture_output=True,
+                          text=True, check=True).stdout
+    parts = re.split(r"\n[0-9a-f]+ <([^>]+)>:\n", text)
+    forms = set()
+    for name, body in zip(parts[1::2], parts[2::2]):
+        form = re.search(r"mx_tile_kernelINS_6MxTileILi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)E"
+                         r".*ELi(\d+)ELi\d+EEEvNS", name)
+        if form is None:
+            continue
+        xt, wt, wm, wn, ring, _ = map(int, form.groups())
+        forms.add(form.groups())
+        waves, rows = wm * wn, 16 * (xt * wm + wt * wn)
+        # a step: 128 bytes of codes a row, 1 KiB a copy; two words of scales, 64 a copy
+        step = rows // 8 // waves + -(-rows // 32 // waves)
+        seen = []  # loads, waits for them, barriers and the loop's branch, in order
+        for line in body.splitlines():
+            op = line.split("//")[0].strip()
+            if re.match(r"(buffer|global|flat|scratch)_", op):
+                seen.append("load" if op.startswith("buffer_load") and op.endswith("lds") else op)
+            elif op.startswith("s_waitcnt") and "vmcnt" in op:
+                seen.append(int(re.search(r"vmcnt\((\d+)\)", op)[1]))
+            elif op.startswith("s_barrier"):
+                seen.append("barrier")
+                if seen.count("barrier") == 3:
+                    break
+            elif op.startswith("s_cbranch_scc0"):
+                seen.append("loop")
+        assert seen == (["load"] * (ring * step) + [(ring - 1) * step, "barrier"]
+                        + [(ring - 2) * step, "barrier"] + ["load"] * step + ["loop"]
+                        + [0, "barrier"]), name
+    assert len(forms) == 6 * 3  # forms and output types
