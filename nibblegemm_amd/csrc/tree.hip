@@ -196,8 +196,8 @@ struct TreeShares {
 // keys.  A tile's rows of k and v are copied straight into one of two LDS
 // buffers while the tile before it is computed; two workgroups share a CU.
 //
-// What bounds it: 64 tokens over 65000 take 85 us of this kernel (16 sequences of
-// 27 over up to 8100 86, 4.2 TB/s; 2048 over 2048 112, 0.92 PFLOP/s).  A tile of
+// What bounds it: 64 tokens over 65000 take 86 us of this kernel (16 sequences of
+// 27 over up to 8100 85, 4.2 TB/s; 2048 over 2048 112, 0.92 PFLOP/s).  A tile of
 // a wave is 68 products of 16 cycles and 32 exponentials of 16 beside some 130
 // plain vector operations of 4; for the two waves of a SIMD that adds up to 4300
 // cycles, and a tile takes 4375: the two hardly overlap.  Neither a priority for
@@ -207,9 +207,11 @@ struct TreeShares {
 // instructions, 2048 over 2048 take 102 us in place of 121, 64 over 65000 83 in
 // place of 100 (with the join).
 // Three workgroups a CU (smaller tiles) took 283 us for the last of those, 64
-// queries a wave, which would halve the reads of LDS, 519 (registers spilt).
+// queries a wave, which would halve the reads of LDS, 519 (registers spilt).  The
+// form for 128 rows of head_dim 128 takes all 256 registers and spills 26; its loops
+// reach those only in the pass for infinities and NaN.
 //
-// One call of 16 tokens over 1000 is latency: 8.4 us, of which finding its share
+// One call of 16 tokens over 1000 is latency: 8.6 us, of which finding its share
 // and loading the queries take 2.3, the copies 0.9, each of two tiles 1.2, the
 // meeting of the waves and the stores 2.9 (4.5 with a barrier for each 16 rows).
 template <class E, int D, int QT, int WK>
@@ -354,9 +356,11 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   };
   // What this lane's queries see of a tail's keys, a bit for each of its scores;
   // whether any lane's sees anything.  Four neighbouring keys are four bytes of the
-  // mask, loaded at once, from a place in the row, and shifted to theirs.  A wave
-  // leaves a tile out that it sees nothing of.  (15 trees of 444 tokens 99 us, 134
-  // with single bytes, loaded behind the products, and no tile left out.)
+  // mask in one load, from a place in the row, and shifted to theirs.  The choice of
+  // loads by T stands in every turn of the loops, so the KS QT loads of a tile wait
+  // for one another, ahead of the tile's barrier.  A wave leaves a tile out that it
+  // sees nothing of.  (15 trees of 444 tokens 95 to 99 us, 134 with single bytes,
+  // loaded behind the products, and no tile left out.)
   uint32_t seen[QT];
   auto look = [&](int i) {
     typedef uint32_t word_t __attribute__((aligned(1)));
@@ -642,7 +646,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
 // together; the sums are then loaded eight shares at a time, those of shares
 // that saw nothing not at all (a share of no weight counts: an infinity or a NaN in
 // its sums must not be lost).  Memory and latency bound it: 64 rows of 8 shares
-// and 8 kv heads 2.8 us, 256 rows of 32 shares 8 us, 34 MB (loads begun before
+// and 8 kv heads 3 us, 256 rows of 32 shares 8 us, 34 MB (loads begun before
 // the statistics are there gained 0.6 us on the first, lost 2 on ragged trees).
 template <class E, int D>
 __global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(TreeArgs a) {

@@ -75,7 +75,8 @@ def attention_decode(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
 
     qkv fp16 [1, (n_heads + 2 n_kv) * 128]: the token's q | k | v (the q|k|v
     projection's output).  k_cache, v_cache fp16 [n_kv, max_seq, 128]; the
-    call writes the token's k (rotated) and v at row ``pos``.  Returns fp16
+    call writes the token's k (rotated) and v at row ``pos`` (and raises the
+    caches' version counters, as a tensor operation would).  Returns fp16
     [1, n_heads * 128] = ``softmax(q k^T / sqrt(128)) v`` per query head,
     head i reading kv head ``i // (n_heads // n_kv)``.  ``rope`` is the
     (cos, sin) pair of :func:`rope_tables` or None."""
@@ -204,7 +205,7 @@ def qk_norm_rope(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     weight`` (weights [D] of qkv's dtype; None: no norm of those heads), then
     rotated by the (cos, sin) of :func:`rope_tables` (None: no rotation), in
     fp32 with one rounding.  k and v go to row ``slots`` of their sequence's
-    caches; q is returned as [B, T, n_heads * D].
+    caches, whose version counters rise; q is returned as [B, T, n_heads * D].
 
     A token whose slot is no row of the cache (-1, say) or whose position is
     no row of the tables is padding: it writes no cache row and its q is zero.
@@ -331,7 +332,9 @@ def tree_mask(parents: torch.Tensor) -> torch.Tensor:
     """The mask of :func:`attention_tree` for trees given by ``parents``, int
     [T] or [B, T]: the index of a token's parent, which comes before it, or -1
     for a token that follows the cached ones.  bool [T, T] or [B, T, T]: a
-    token sees itself and its ancestors."""
+    token sees itself and its ancestors.  Tensor operations on the parents' device,
+    a few for each level of the deepest tree, which wait for their results: masks
+    are made outside a captured step, and on the CPU where the parents are there."""
     if parents.dim() not in (1, 2) or parents.is_floating_point():
         raise ValueError(f"parents must be an integer [T] or [B, T] tensor, got {parents.dtype} "
                          f"{tuple(parents.shape)}")
