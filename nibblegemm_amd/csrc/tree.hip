@@ -50,7 +50,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // and thousands of 2^-25, which a sink leaves to the rest, are not lost.  (A slack
 // of 4 and a lift of 11: 4 x 8 tokens over 3000, 32 heads of 64 on 4, 16.2 us in
 // place of 15.7; 16 x 27 over 8100 105.8 in place of 103.)  bf16 has the range of
-// fp32.
+// fp32.  The slack is measured by a difference, which is exact: a sum would round to
+// the steps of a large maximum.  (Below 2^28, in powers of two, that is; beyond it a
+// score's own rounding in fp32 passes what fp16 has left.)
 constexpr float kTreeSlack = 8.0f;
 template <class E>
 constexpr float kTreeLift = std::is_same_v<E, Half> ? 7.0f : 0.0f;
@@ -421,7 +423,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   auto move = [&]() {
     bool moves = false;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) moves |= m[t] > top[t] + (kTreeSlack + kTreeLift<E>);
+    for (int t = 0; t < QT; ++t) moves |= m[t] - top[t] > kTreeSlack + kTreeLift<E>;
     if (!__any(moves)) return;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {

@@ -278,7 +278,8 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     ``softmax(scale q k^T) v`` over what the token sees, head i reading kv head
     ``i // (n_heads // n_kv)``, scale ``1 / sqrt(D)`` by default, in fp32 with
     the probabilities rounded to q's dtype (in fp16 those below 2^-21 of the
-    largest in steps of 2^-31 of it).
+    largest in steps of 2^-31 of it).  Scores are below 2^28 log(2) in magnitude,
+    2^31 log(2) in bf16: their rounding in fp32 would overflow beyond.
 
     Tokens behind a sequence's last, and tokens that see nothing, give zeros.
     Rows that a token does not see have no part in its output, whatever they

@@ -806,3 +806,28 @@ def test_a_batch_of_none():
         assert glue.attention_tree(q, c, c.clone(), n).shape == (0, T, 256)
         assert glue.attention_tree(q, c, c.clone(), n, mask, n).shape == (0, T, 256)
         assert glue.qk_norm_rope(q, c, c.clone(), i, i).shape == (0, T, 128)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("up", [2, 4, 16, 36])
+@pytest.mark.parametrize("power", [10, 11, 12, 12.5, 13])
+@pytest.mark.parametrize("T,n_heads", [(1, 4), (7, 4), (15, 4), (40, 4)])
+def test_scores_whose_steps_are_whole_powers_of_two(T, n_heads, power, up, dtype):
+    """Scores of up to 2^26 in powers of two, where fp32 has steps of 8, and a
+    maximum that rises by 4 up in a later tile: no probability overflows."""
+    D, n = 128, 128
+    base = 2.0 ** power if power != 12.5 else 6144.0
+    q = torch.zeros((1, T, n_heads, D), dtype=dtype)
+    k = torch.zeros((1, 1, n + T, D), dtype=dtype)
+    q[..., 0], q[..., 1] = base, 4.0
+    k[0, 0, 0, 0], k[0, 0, 0, 1] = base, 2.0
+    k[0, 0, 64, 0], k[0, 0, 64, 1] = base, 2.0 + up
+    v = torch.randn((1, 1, n + T, D), generator=torch.Generator().manual_seed(3)).to(dtype)
+    got = run_tree(q, k, v, torch.tensor([n], dtype=torch.int32), scale=math.log(2.0)).cpu().double()
+    # The scores differ by 4 up, each off by a few steps of 2^-24 of itself at most.
+    far = 4.0 * up - 4 * base * base * 2.0 ** -23
+    lo, hi = (v[0, 0, i].double() for i in (0, 64))
+    info = torch.finfo(dtype)
+    off = (lo - hi).abs() * min(1.0, 2.0 ** -far) + hi.abs() * info.eps + 2.0 ** -20
+    assert ((got - hi).abs() <= off).all()
