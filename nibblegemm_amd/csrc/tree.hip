@@ -25,15 +25,13 @@
 
 #include "nibble_common.h"
 #include "nibble_copy.h"
-#include "nibble_reduce.h"
+#include "nibble_split.h"
 
 namespace nibble {
 namespace {
 
 constexpr int kTreeThreads = 256;
 constexpr int kTreeKeys = 64;        // keys of a tile
-constexpr int kTreeMaxSplits = 64;   // of one sequence
-constexpr int kTreeWorkgroups = 512;  // two a CU
 // What a share more costs, in the time of a tile: the join's turn, and a query
 // row's sums written and read again.  us with these / with as many shares as there
 // is room for: 1 x 100 tokens (32 heads on 8) over 1000 21.8 / 27.7, 1 x 64 over 4000
@@ -41,7 +39,6 @@ constexpr int kTreeWorkgroups = 512;  // two a CU
 // 10.6 / 13.9 (13.8 with half the first); half the second -7 to +19%, twice it 2 to
 // 14% slower.
 constexpr float kTreeShareCost = 0.08f, kTreeRowCost = 4.8e-4f;
-constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are relative to a query's reference, 2^lift below a maximum.  It
 // moves only when a score passes that maximum by more than the slack (in powers of
 // two): until then they are at most 2^(slack + lift), and the sums need no
@@ -75,6 +72,7 @@ struct TreeArgs {
   bool fold;              // row tiles from both ends to the middle
   float scale;  // its magnitude times log2(e); 1 for a scale of zero
   float sign;   // its sign
+  __device__ int tiles(int b) const;  // of a sequence's rows
 };
 
 // Unit (16 bytes) u of LDS row r lies at unit u ^ tree_swizzle(r): eight rows of
@@ -84,23 +82,6 @@ __device__ __forceinline__ int tree_swizzle(int r) {
   return ((r & 3) << 1 | (r >> 2 & 1) | (r & 8)) & (UNITS - 1);
 }
 
-// A lane's value and the one of the lane 32 (16) away, in either order.
-struct Pair {
-  float a, b;
-};
-template <int DIST>
-__device__ __forceinline__ Pair swap_pair(float v) {
-  const uint32_t i = __builtin_bit_cast(uint32_t, v);
-  const auto r = DIST == 32 ? __builtin_amdgcn_permlane32_swap(i, i, false, false)
-                            : __builtin_amdgcn_permlane16_swap(i, i, false, false);
-  const uint32_t x = r[0], y = r[1];  // (a bit cast of r[1] itself takes r[0])
-  return {__builtin_bit_cast(float, x), __builtin_bit_cast(float, y)};
-}
-__device__ __forceinline__ float swap_max(float v) {
-  const Pair a = swap_pair<32>(v);
-  const Pair b = swap_pair<16>(fmaxf(a.a, a.b));
-  return fmaxf(b.a, b.b);
-}
 // What of sequence b there is: cached tokens and tree tokens within the cache.
 struct TreeSpan {
   int len, live, total;
@@ -110,88 +91,9 @@ struct TreeSpan {
     total = min(len + live, a.seq);
   }
 };
-
-// How the cached rows are split when there are fewer (sequence, kv head, row
-// tile)s than room for workgroups.  The lengths are on the GPU, so every wave
-// works it out alike: a share is at most `per` tiles of one sequence, and per is
-// (to a 16th) the least for which all sequences' shares together are at most
-// a.shares.  Shares are numbered in the order of the sequences, of which there
-// are fewer than a.shares; one without rows keeps a share, which writes that it
-// saw nothing.
-struct TreeShares {
-  static constexpr int kChunks = kTreeWorkgroups / 64;  // of sequences, one a lane
-  int per = 0, found = -1, first = 0, count = 0;
-  // Finds the sequence that share `want` is of, and that sequence's shares.
-  __device__ __forceinline__ TreeShares(const TreeArgs& a, int want) {
-    if (a.B == 1) {
-      const int all = tiles(a, 0);
-      per = max((all + a.shares - 1) / a.shares,
-                max((all + kTreeMaxSplits - 1) / kTreeMaxSplits, worth(a, static_cast<float>(all))));
-      count = shares_of(all);
-      found = want < count ? 0 : -1;
-      return;
-    }
-    const int lane = threadIdx.x & 63;
-    int t[kChunks];  // tiles; 0 where there is no sequence
-    float most_f = 0.0f, total = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      t[i] = 0;
-      if (64 * i < a.B) {
-        t[i] = 64 * i + lane < a.B ? tiles(a, 64 * i + lane) : 0;
-        most_f = fmaxf(most_f, static_cast<float>(t[i]));  // (below 2^24: exact)
-        total += static_cast<float>(t[i]);
-      }
-    }
-    const int most = static_cast<int>(wave_max(most_f));
-    total = wave_sum(total);
-    per = static_cast<int>(ceilf(total / static_cast<float>(a.shares)));
-    per = max(max(per, (most + kTreeMaxSplits - 1) / kTreeMaxSplits), worth(a, total));
-    per = __builtin_amdgcn_readfirstlane(per);
-    int high = max(per, most);  // enough: one share each
-    for (int low = per; low < high;) {
-      const bool close = high - low <= low / 16;
-      const int mid = close ? low : low + (high - low) / 2;
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < kChunks; ++i)
-        if (64 * i < a.B) n += 64 * i + lane < a.B ? max(1, (t[i] + mid - 1) / mid) : 0;
-      if (wave_sum(static_cast<float>(n)) <= static_cast<float>(a.shares)) high = mid;
-      else low = close ? high : mid + 1;
-    }
-    per = high;
-    int before = 0;
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i)
-      if (64 * i < a.B && found < 0) {
-        const int n = 64 * i + lane < a.B ? shares_of(t[i]) : 0;
-        int upto = n;
-#pragma unroll
-        for (int x = 1; x < 64; x *= 2) {
-          const int y = __shfl_up(upto, x);
-          if (lane >= x) upto += y;
-        }
-        const int start = before + upto - n;
-        const uint64_t hit = __ballot(want >= start && want < start + n);
-        if (hit != 0) {
-          const int at = __builtin_ctzll(hit);
-          found = 64 * i + at;
-          first = __builtin_amdgcn_readlane(start, at);
-          count = __builtin_amdgcn_readlane(n, at);
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
-      }
-  }
-  // per tiles in turn, and total / per shares whose sums are written and joined:
-  // the least of per + join_cost total / per.
-  static __device__ __forceinline__ int worth(const TreeArgs& a, float total) {
-    return max(static_cast<int>(__builtin_amdgcn_sqrtf(a.join_cost * total)), 1);
-  }
-  static __device__ __forceinline__ int tiles(const TreeArgs& a, int b) {
-    return (TreeSpan(a, b).total + kTreeKeys - 1) / kTreeKeys;
-  }
-  __device__ __forceinline__ int shares_of(int t) const { return max(1, (t + per - 1) / per); }
-};
+__device__ __forceinline__ int TreeArgs::tiles(int b) const {
+  return (TreeSpan(*this, b).total + kTreeKeys - 1) / kTreeKeys;
+}
 
 // One workgroup: 16 QT WQ query rows of one kv head (WQ = 4 / WK waves along
 // the rows, WK along the keys), one share of the cached rows, in tiles of 64
@@ -252,7 +154,7 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   int b = w, share = 0, per = 0x3fffffff;  // the whole sequence
   if (a.shares > 0) {
     if (w >= a.shares) return;
-    const TreeShares shares(a, w);
+    const Shares<TreeArgs> shares(a, w);
     if (shares.found < 0) return;
     b = shares.found, share = w - shares.first, per = shares.per;
     // (for the kernel that joins them)
@@ -643,77 +545,6 @@ __global__ __launch_bounds__(kTreeThreads, 2) void tree_kernel(TreeArgs a) {
   }
 }
 
-// Joins the shares of a row: D / 4 lanes a row, four outputs each, the rows of
-// one (sequence, kv head) in a workgroup.  The lanes read the shares' statistics
-// together; the sums are then loaded eight shares at a time, those of shares
-// that saw nothing not at all (a share of no weight counts: an infinity or a NaN in
-// its sums must not be lost).  Memory and latency bound it: 64 rows of 8 shares
-// and 8 kv heads 3 us, 256 rows of 32 shares 8 us, 34 MB (loads begun before
-// the statistics are there gained 0.6 us on the first, lost 2 on ragged trees).
-template <class E, int D>
-__global__ __launch_bounds__(kTreeThreads) void tree_join_kernel(TreeArgs a) {
-  using T = typename E::type;
-  constexpr int LANES = D / 4, PER = kTreeMaxSplits / LANES;  // splits a lane looks at
-  const int rows_all = a.T * a.qpk;
-  const int parts = (rows_all + kTreeThreads / LANES - 1) / (kTreeThreads / LANES);
-  const int unit = blockIdx.x / parts;
-  const int b = unit / a.n_kv, h = unit - b * a.n_kv;
-  const int at = (blockIdx.x - unit * parts) * (kTreeThreads / LANES) + threadIdx.x / LANES;
-  const bool in = at < rows_all;
-  const int r = in ? at : 0;  // (lanes without a row shuffle along)
-  const int lane = threadIdx.x % LANES, d = lane * 4;
-  const int first = a.runs[2 * b], count = a.runs[2 * b + 1];
-  const float* const st = a.partial + static_cast<int64_t>(a.n_kv) * a.shares * rows_all * D;
-  const int64_t rec0 = (static_cast<int64_t>(h) * a.shares + first) * rows_all + r;
-  float tops[PER], w[PER], m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int u = 0; u < PER; ++u) {
-    const int s = u * LANES + lane;
-    const float* p = st + (rec0 + static_cast<int64_t>(s) * rows_all) * 2;
-    tops[u] = s < count ? p[0] : -INFINITY;
-    w[u] = s < count ? p[1] : 0.0f;
-    m = fmaxf(m, tops[u]);
-  }
-#pragma unroll
-  for (int x = LANES / 2; x > 0; x /= 2) m = fmaxf(m, __shfl_xor(m, x, LANES));
-#pragma unroll
-  for (int u = 0; u < PER; ++u) {
-    const float keep = tops[u] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(tops[u] - m);
-    l += w[u] * keep;
-    w[u] = tops[u] == -INFINITY ? -1.0f : keep;  // (negative: no sums)
-  }
-#pragma unroll
-  for (int x = LANES / 2; x > 0; x /= 2) l += __shfl_xor(l, x, LANES);
-  f4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int u = 0; u < PER; ++u)
-    for (int s0 = 0; s0 < LANES && u * LANES + s0 < count; s0 += 8) {
-      f4_t v[8];
-      float k[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        k[e] = __shfl(w[u], s0 + e, LANES);
-        v[e] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        if (!(k[e] < 0.0f))
-          v[e] = *reinterpret_cast<const f4_t*>(
-              a.partial + (rec0 + static_cast<int64_t>(u * LANES + s0 + e) * rows_all) * D + d);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] += v[e][i] * k[e];
-    }
-  if (!in) return;
-  const int i = r / a.qpk;
-  typedef T vec4 __attribute__((ext_vector_type(4)));
-  vec4 y;
-#pragma unroll
-  for (int x = 0; x < 4; ++x) y[x] = static_cast<T>(l == 0.0f ? 0.0f : o[x] / l);
-  *reinterpret_cast<vec4*>(static_cast<T*>(a.out) +
-                           ((static_cast<int64_t>(b) * a.T + i) * a.n_heads + h * a.qpk +
-                            (r - i * a.qpk)) * D + d) = y;
-}
-
 struct TreePlan {
   int form = 0, rows = 16, row_tiles = 1, shares = 0;
   size_t workspace_bytes = 0;
@@ -743,8 +574,8 @@ int plan_tree(int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv, int6
                (long long)n_kv);
   // Room for more workgroups than there are (sequence, kv head, row tile)s: the
   // cached rows are split, unless there are but a few tiles of them.
-  const int64_t room = kTreeWorkgroups / (n_kv * p->row_tiles);
-  if (room > batch && batch < 64 * TreeShares::kChunks && max_seq > 4 * kTreeKeys) {
+  const int64_t room = kSplitWorkgroups / (n_kv * p->row_tiles);
+  if (room > batch && batch < kSplitWorkgroups && max_seq > 4 * kTreeKeys) {
     p->shares = static_cast<int>(room);
     p->workspace_bytes =
         static_cast<size_t>(n_kv * room * rows) * (head_dim + 2) * 4 + static_cast<size_t>(batch) * 8;
@@ -763,7 +594,7 @@ hipError_t launch_tree(const TreeArgs& a, const TreePlan& p, hipStream_t stream)
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.shares == 0) return e;
   const int64_t parts = ceil_div(static_cast<int64_t>(a.T) * a.qpk, kTreeThreads / (D / 4));
-  tree_join_kernel<E, D><<<dim3(static_cast<unsigned>(a.B * a.n_kv * parts)), kTreeThreads, 0,
+  join_kernel<E, D><<<dim3(static_cast<unsigned>(a.B * a.n_kv * parts)), kTreeThreads, 0,
                            stream>>>(a);
   return hipGetLastError();
 }
@@ -847,7 +678,7 @@ extern "C" int nibble_attention_tree(const void* Q, int64_t dtype, int64_t batch
   a.shares = p.shares;
   a.row_tiles = p.row_tiles;
   a.join_cost = kTreeShareCost + kTreeRowCost * static_cast<float>(tokens * n_heads);
-  a.fold = mask == nullptr && batch * n_kv_heads * p.row_tiles <= kTreeWorkgroups;
+  a.fold = mask == nullptr && batch * n_kv_heads * p.row_tiles <= kSplitWorkgroups;
   a.scale = scale == 0.0f ? 1.0f : std::fabs(scale) * kLog2e;
   a.sign = scale > 0.0f ? 1.0f : scale < 0.0f ? -1.0f : 0.0f;
   const hipError_t e = dtype == 0 ? (head_dim == 64 ? launch_tree<Half, 64>(a, p, stream)
