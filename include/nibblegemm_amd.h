@@ -50,7 +50,7 @@
 extern "C" {
 #endif
 
-#define NIBBLE_ABI_VERSION 16
+#define NIBBLE_ABI_VERSION 17
 
 #if defined(__GNUC__) || defined(__clang__)
 #define NIBBLE_API __attribute__((visibility("default")))
@@ -475,6 +475,74 @@ NIBBLE_API int nibble_attention_tree(const void* Q, int64_t dtype, int64_t batch
 NIBBLE_API size_t nibble_attention_tree_workspace_bytes(int64_t batch, int64_t tokens,
                                                         int64_t n_heads, int64_t n_kv_heads,
                                                         int64_t head_dim, int64_t max_seq);
+
+/*
+ * Paged caches.  No counterpart in the reference's extension.  Keys and values lie
+ * in n_pages pages of page_rows (16, 32, 64, 128 or 256) rows, element (page, h, r, d)
+ * at page page_stride + h head_stride + r row_stride + d elements, the strides
+ * multiples of 16 bytes, a row's at most 2^22 elements.  Rows m page_rows .. of
+ * sequence b are page table[b][m] (int32 [batch, table_pages]); an entry outside [0,
+ * n_pages) is no page.  The elements are 16 bits wide (dtype: 0 fp16, 1 bf16, as of the
+ * call's other tensors), or, with scales, 8: the value is code 2^(scale - 127), code an
+ * 8-bit float (e4m3 without infinities), scale uint8 [n_pages, n_kv_heads], one a page
+ * and head.  head_dim 64 or 128.  K, V 16-byte aligned, the table 4.
+ */
+typedef struct {
+  void* K;
+  void* V;
+  void* k_scales; /* both NULL: 16-bit pages */
+  void* v_scales;
+  const void* table;
+  int64_t n_pages, n_kv_heads, page_rows, head_dim, table_pages;
+  int64_t k_page_stride, k_head_stride, k_row_stride;
+  int64_t v_page_stride, v_head_stride, v_row_stride;
+} nibble_paged_cache;
+
+/* Norms of the query and key heads (weights [head_dim], NULL: none), rotary embedding
+ * of a head's first rope_dim elements (a multiple of 16; tables [rope_rows, rope_dim /
+ * 2], both NULL: none) in halves (i, i + rope_dim / 2) or, interleaved, pairs (2 i, 2 i
+ * + 1), and the append: QKV [batch, tokens, (n_heads + 2 n_kv_heads) head_dim], q to
+ * Q_out [batch, tokens, n_heads head_dim], k and v of token t < sizes[b] (NULL: tokens)
+ * to row lengths[b] + t of sequence b.  positions int32 [batch, tokens] (NULL: a token's
+ * row).  A token without a page or without a position in the tables writes no row, and
+ * zeros to Q_out.  8-bit pages: a page whose first row is new takes the least scale
+ * under which its new rows fit (of those whose products with all codes are values of
+ * dtype); one with earlier rows the larger of its own and that, its earlier rows
+ * rescaled; rows behind are left.  Magnitudes beyond dtype's largest value count as
+ * that value; infinities and NaN become NaN.  Pages that a call writes belong to one
+ * sequence each.  batch at most 65535, tokens 2^20; a launch ends at 2^24 - 1
+ * workgroups. */
+NIBBLE_API int nibble_paged_append(const void* QKV, int64_t dtype, int64_t batch, int64_t tokens,
+                                   int64_t n_heads, const nibble_paged_cache* cache,
+                                   const void* lengths, const void* sizes, const void* positions,
+                                   const void* q_weight, const void* k_weight, float eps,
+                                   const void* rope_cos, const void* rope_sin, int64_t rope_rows,
+                                   int64_t rope_dim, int64_t interleaved, void* Q_out,
+                                   void* stream);
+
+/* Attention of the newest tokens of several sequences over their pages: Q [batch,
+ * tokens, n_heads head_dim]; token i < sizes[b] (NULL: tokens) of sequence b is row r =
+ * lengths[b] + i and sees the rows j <= r that have a page, of these, with window > 0,
+ * those with r - j < window or j < sinks.  Out [batch, tokens, n_heads head_dim] =
+ * softmax(scale q k^T) v, zeros for tokens that see nothing and behind a sequence's
+ * last.  scale is finite, also times log2(e).  window (0: none) and sinks are at most
+ * 2^30.  The workspace (nibble_attention_paged_workspace_bytes, 256-byte aligned; NULL
+ * when that is 0) needs no initial contents. */
+NIBBLE_API int nibble_attention_paged(const void* Q, int64_t dtype, int64_t batch, int64_t tokens,
+                                      int64_t n_heads, const nibble_paged_cache* cache,
+                                      const void* lengths, const void* sizes, int64_t window,
+                                      int64_t sinks, float scale, void* Out, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+NIBBLE_API size_t nibble_attention_paged_workspace_bytes(int64_t batch, int64_t tokens,
+                                                         int64_t n_heads, int64_t n_kv_heads,
+                                                         int64_t head_dim, int64_t max_rows);
+
+/* The values of a cache: rows 0 .. rows - 1 of each sequence to K_out and V_out
+ * [batch, n_kv_heads, rows, head_dim] of dtype (that of 16-bit pages), 16-byte aligned;
+ * zeros from lengths[b] on and where there is no page. */
+NIBBLE_API int nibble_paged_values(const nibble_paged_cache* cache, int64_t dtype, int64_t batch,
+                                   const void* lengths, int64_t rows, void* K_out, void* V_out,
+                                   void* stream);
 
 /*
  * Microscaled 4-bit floats (OCP MXFP4).  No counterpart in the reference.  A

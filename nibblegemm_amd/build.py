@@ -31,7 +31,7 @@ LIB = os.path.join(LIBDIR, "libnibblegemm_amd.so")
 
 HIP_SOURCES = ["abi.hip", "dequant.hip", "gemv.hip", "gemm.hip", "glue.hip", "chain.hip", "probe.hip",
                "quantize.hip", "mx.hip",
-               "qk_norm.hip", "tree.hip"]
+               "qk_norm.hip", "tree.hip", "paged.hip", "paged_attention.hip"]
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [

@@ -310,6 +310,95 @@ static PyObject* py_attention_tree_ws(PyObject* self, PyObject* const* a, Py_ssi
   return PyLong_FromSize_t(nibble_attention_tree_workspace_bytes(B, T, nh, nkv, hd, ms));
 }
 
+/* A cache in 16 arguments: K, V, k_scales, v_scales, table, n_pages, n_kv, page_rows, head_dim,
+ * table_pages, kp, kh, kr, vp, vh, vr */
+#define PAGED_ARGS 16
+static int take_paged(PyObject* const* a, nibble_paged_cache* c) {
+  void* table;
+  long long n[11];
+  if (!take_ptr(a[0], &c->K) || !take_ptr(a[1], &c->V) || !take_ptr(a[2], &c->k_scales) ||
+      !take_ptr(a[3], &c->v_scales) || !take_ptr(a[4], &table))
+    return 0;
+  for (int i = 0; i < 11; ++i)
+    if (!take_i64(a[5 + i], &n[i])) return 0;
+  c->table = table;
+  c->n_pages = n[0], c->n_kv_heads = n[1], c->page_rows = n[2], c->head_dim = n[3];
+  c->table_pages = n[4];
+  c->k_page_stride = n[5], c->k_head_stride = n[6], c->k_row_stride = n[7];
+  c->v_page_stride = n[8], c->v_head_stride = n[9], c->v_row_stride = n[10];
+  return 1;
+}
+
+/* paged_append(QKV, dtype, batch, tokens, n_heads, <cache>, lengths, sizes, positions, q_weight,
+ * k_weight, eps, cos, sin, rope_rows, rope_dim, interleaved, Q_out, stream) */
+static PyObject* py_paged_append(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (!nargs_is(n, 18 + PAGED_ARGS, "paged_append")) return NULL;
+  nibble_paged_cache c;
+  void *qkv, *len, *sizes, *pos, *qw, *kw, *rc, *rs, *out, *stream;
+  long long dt, B, T, nh, rows, dim, inter;
+  PyObject* const* z = a + 5 + PAGED_ARGS;
+  double eps = PyFloat_AsDouble(z[5]);
+  if (eps == -1.0 && PyErr_Occurred()) return NULL;
+  if (!take_ptr(a[0], &qkv) || !take_i64(a[1], &dt) || !take_i64(a[2], &B) || !take_i64(a[3], &T) ||
+      !take_i64(a[4], &nh) || !take_paged(a + 5, &c) || !take_ptr(z[0], &len) ||
+      !take_ptr(z[1], &sizes) || !take_ptr(z[2], &pos) || !take_ptr(z[3], &qw) ||
+      !take_ptr(z[4], &kw) || !take_ptr(z[6], &rc) || !take_ptr(z[7], &rs) ||
+      !take_i64(z[8], &rows) || !take_i64(z[9], &dim) || !take_i64(z[10], &inter) ||
+      !take_ptr(z[11], &out) || !take_ptr(z[12], &stream))
+    return NULL;
+  return PyLong_FromLong(nibble_paged_append(qkv, dt, B, T, nh, &c, len, sizes, pos, qw, kw,
+                                             (float)eps, rc, rs, rows, dim, inter, out, stream));
+}
+
+/* attention_paged(Q, dtype, batch, tokens, n_heads, <cache>, lengths, sizes, window, sinks, scale,
+ * Out, ws, ws_bytes, stream) */
+static PyObject* py_attention_paged(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (!nargs_is(n, 14 + PAGED_ARGS, "attention_paged")) return NULL;
+  nibble_paged_cache c;
+  void *q, *len, *sizes, *out, *ws, *stream;
+  long long dt, B, T, nh, window, sinks, wsb;
+  PyObject* const* z = a + 5 + PAGED_ARGS;
+  double scale = PyFloat_AsDouble(z[4]);
+  if (scale == -1.0 && PyErr_Occurred()) return NULL;
+  if (!take_ptr(a[0], &q) || !take_i64(a[1], &dt) || !take_i64(a[2], &B) || !take_i64(a[3], &T) ||
+      !take_i64(a[4], &nh) || !take_paged(a + 5, &c) || !take_ptr(z[0], &len) ||
+      !take_ptr(z[1], &sizes) || !take_i64(z[2], &window) || !take_i64(z[3], &sinks) ||
+      !take_ptr(z[5], &out) || !take_ptr(z[6], &ws) || !take_i64(z[7], &wsb) ||
+      !take_ptr(z[8], &stream))
+    return NULL;
+  return PyLong_FromLong(nibble_attention_paged(q, dt, B, T, nh, &c, len, sizes, window, sinks,
+                                                (float)scale, out, ws,
+                                                (size_t)(wsb < 0 ? 0 : wsb), stream));
+}
+
+/* attention_paged_workspace_bytes(batch, tokens, n_heads, n_kv, head_dim, max_rows) */
+static PyObject* py_attention_paged_ws(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (!nargs_is(n, 6, "attention_paged_workspace_bytes")) return NULL;
+  long long B, T, nh, nkv, hd, ms;
+  if (!take_i64(a[0], &B) || !take_i64(a[1], &T) || !take_i64(a[2], &nh) ||
+      !take_i64(a[3], &nkv) || !take_i64(a[4], &hd) || !take_i64(a[5], &ms))
+    return NULL;
+  return PyLong_FromSize_t(nibble_attention_paged_workspace_bytes(B, T, nh, nkv, hd, ms));
+}
+
+/* paged_values(<cache>, dtype, batch, lengths, rows, K_out, V_out, stream) */
+static PyObject* py_paged_values(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+  (void)self;
+  if (!nargs_is(n, 7 + PAGED_ARGS, "paged_values")) return NULL;
+  nibble_paged_cache c;
+  void *len, *ko, *vo, *stream;
+  long long dt, B, rows;
+  PyObject* const* z = a + PAGED_ARGS;
+  if (!take_paged(a, &c) || !take_i64(z[0], &dt) || !take_i64(z[1], &B) || !take_ptr(z[2], &len) ||
+      !take_i64(z[3], &rows) || !take_ptr(z[4], &ko) || !take_ptr(z[5], &vo) ||
+      !take_ptr(z[6], &stream))
+    return NULL;
+  return PyLong_FromLong(nibble_paged_values(&c, dt, B, len, rows, ko, vo, stream));
+}
+
 /* dequant(Wq, wr, wc, S, sr, sc, g, fast, W, stream) */
 static PyObject* py_dequant(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   (void)self;
@@ -595,6 +684,14 @@ static PyMethodDef kMethods[] = {
      "nibble_attention_tree"},
     {"attention_tree_workspace_bytes", (PyCFunction)(void (*)(void))py_attention_tree_ws,
      METH_FASTCALL, "nibble_attention_tree_workspace_bytes"},
+    {"paged_append", (PyCFunction)(void (*)(void))py_paged_append, METH_FASTCALL,
+     "nibble_paged_append"},
+    {"attention_paged", (PyCFunction)(void (*)(void))py_attention_paged, METH_FASTCALL,
+     "nibble_attention_paged"},
+    {"attention_paged_workspace_bytes", (PyCFunction)(void (*)(void))py_attention_paged_ws,
+     METH_FASTCALL, "nibble_attention_paged_workspace_bytes"},
+    {"paged_values", (PyCFunction)(void (*)(void))py_paged_values, METH_FASTCALL,
+     "nibble_paged_values"},
     {"chain_create", (PyCFunction)(void (*)(void))py_chain_create, METH_FASTCALL,
      "nibble_chain_create"},
     {"chain_run", (PyCFunction)(void (*)(void))py_chain_run, METH_FASTCALL, "nibble_chain_run"},
