@@ -78,17 +78,13 @@ def _check_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
     ks, vs = k_pages.stride(), v_pages.stride()
     if ks[3] != 1 or vs[3] != 1:
         raise RuntimeError("the elements of a cache row must be adjacent")
-    if table.dim() != 2:
-        raise ValueError(f"table must be [B, width], got {list(table.shape)}")
-    _check_index("table", table, table.shape, k_pages)
     k_scales = v_scales = None
     if scales is not None:
         for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
             if t.dtype is not _FLOAT8:
                 raise RuntimeError(f"{name} must be float8_e4m3fn beside scales, got {t.dtype}")
             if t.get_device() != index:
-                _check_gpu(name, t, scales[0])
-                raise RuntimeError(f"{name} must live on GPU {index}")
+                raise RuntimeError(f"{name} must live on GPU {index}, got {t.device}")
         for name, t in zip(("k_scales", "v_scales"), scales):
             if t.get_device() != index:
                 _check_gpu(name, t, k_pages)
@@ -99,6 +95,9 @@ def _check_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
         k_scales, v_scales = scales[0].data_ptr(), scales[1].data_ptr()
     elif k_pages.dtype is _FLOAT8:
         raise RuntimeError("8-bit pages need scales")
+    if table.dim() != 2:
+        raise ValueError(f"table must be [B, width], got {list(table.shape)}")
+    _check_index("table", table, table.shape, k_pages)
     if written:
         for n, k, v in zip(shape, ks, vs):
             if n > 1 and (k == 0 or v == 0):
