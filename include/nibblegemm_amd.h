@@ -527,7 +527,8 @@ NIBBLE_API int nibble_paged_append(const void* QKV, int64_t dtype, int64_t batch
  * softmax(scale q k^T) v, zeros for tokens that see nothing and behind a sequence's
  * last.  scale is finite, also times log2(e).  window (0: none) and sinks are at most
  * 2^30.  The workspace (nibble_attention_paged_workspace_bytes, 256-byte aligned; NULL
- * when that is 0) needs no initial contents. */
+ * when that is 0) begins with nibble_attention_paged_counter_bytes that are zero before
+ * the first call and restored to zero by each; max_rows is table_pages page_rows. */
 NIBBLE_API int nibble_attention_paged(const void* Q, int64_t dtype, int64_t batch, int64_t tokens,
                                       int64_t n_heads, const nibble_paged_cache* cache,
                                       const void* lengths, const void* sizes, int64_t window,
@@ -536,6 +537,9 @@ NIBBLE_API int nibble_attention_paged(const void* Q, int64_t dtype, int64_t batc
 NIBBLE_API size_t nibble_attention_paged_workspace_bytes(int64_t batch, int64_t tokens,
                                                          int64_t n_heads, int64_t n_kv_heads,
                                                          int64_t head_dim, int64_t max_rows);
+NIBBLE_API size_t nibble_attention_paged_counter_bytes(int64_t batch, int64_t tokens,
+                                                       int64_t n_heads, int64_t n_kv_heads,
+                                                       int64_t head_dim, int64_t max_rows);
 
 /* The values of a cache: rows 0 .. rows - 1 of each sequence to K_out and V_out
  * [batch, n_kv_heads, rows, head_dim] of dtype (that of 16-bit pages), 16-byte aligned;

@@ -373,7 +373,8 @@ static PyObject* py_attention_paged(PyObject* self, PyObject* const* a, Py_ssize
                                                 (size_t)(wsb < 0 ? 0 : wsb), stream));
 }
 
-/* attention_paged_workspace_bytes(batch, tokens, n_heads, n_kv, head_dim, max_rows) */
+/* attention_paged_workspace_bytes(batch, tokens, n_heads, n_kv, head_dim, max_rows):
+ * (workspace bytes, counter bytes) */
 static PyObject* py_attention_paged_ws(PyObject* self, PyObject* const* a, Py_ssize_t n) {
   (void)self;
   if (!nargs_is(n, 6, "attention_paged_workspace_bytes")) return NULL;
@@ -381,7 +382,9 @@ static PyObject* py_attention_paged_ws(PyObject* self, PyObject* const* a, Py_ss
   if (!take_i64(a[0], &B) || !take_i64(a[1], &T) || !take_i64(a[2], &nh) ||
       !take_i64(a[3], &nkv) || !take_i64(a[4], &hd) || !take_i64(a[5], &ms))
     return NULL;
-  return PyLong_FromSize_t(nibble_attention_paged_workspace_bytes(B, T, nh, nkv, hd, ms));
+  size_t ws = nibble_attention_paged_workspace_bytes(B, T, nh, nkv, hd, ms);
+  size_t cb = nibble_attention_paged_counter_bytes(B, T, nh, nkv, hd, ms);
+  return Py_BuildValue("(nn)", (Py_ssize_t)ws, (Py_ssize_t)cb);
 }
 
 /* paged_values(<cache>, dtype, batch, lengths, rows, K_out, V_out, stream) */

@@ -22,6 +22,18 @@ __device__ __forceinline__ void lds_copy16(const void* base, uint32_t bytes, uin
                : "s"(dst), "v"(voff), "s"(rsrc), "s"(soff)
                : "memory", "m0");
 }
+// The same for bytes that are read once (nt): a streaming read of 272 MB 6.9 TB/s, 6.0
+// without.
+__device__ __forceinline__ void lds_stream16(const void* base, uint32_t bytes, uint32_t dst,
+                                             uint32_t voff) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  const u4_t rsrc = {static_cast<uint32_t>(b), static_cast<uint32_t>(b >> 32) & 0xffffu, bytes,
+                     0x00020000u};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+               :
+               : "s"(dst), "v"(voff), "s"(rsrc)
+               : "memory", "m0");
+}
 // The same with 4 bytes a lane, landing at dst + 4 l.
 __device__ __forceinline__ void lds_copy4(const void* base, uint32_t bytes, uint32_t dst,
                                           uint32_t voff, uint32_t soff = 0) {

@@ -24,95 +24,13 @@
 #include <cmath>
 #include <type_traits>
 
-#include "nibble_common.h"
-#include "nibble_float8.h"
-#include "nibble_split.h"
+#include "paged_rows.h"
 
 namespace nibble {
 
 int check_paged(const nibble_paged_cache* c, int64_t dtype, int64_t batch);
 
 namespace {
-
-constexpr int kPagedThreads = 256;
-constexpr int kPagedKeys = 64;  // keys of a tile
-constexpr float kPagedShareCost = 0.08f, kPagedRowCost = 4.8e-4f;
-// Probabilities are relative to a query's reference, 2^lift below a maximum, which
-// moves only when a score passes that maximum by more than the slack (in powers of two).
-// fp16 ends at 2^16 and has steps of 2^-24 at least, so its reference lies as low as it
-// can; bf16 has the range of fp32.
-constexpr float kPagedSlack = 8.0f;
-template <class E>
-constexpr float kPagedLift = std::is_same_v<E, Half> ? 7.0f : 0.0f;
-
-struct PagedSpan;
-
-struct AttendArgs {
-  const void* q;  // [B, T, n_heads, D]
-  const char* k;  // element (page, h, r, d) at page kp + h kh + r kr bytes + d elements
-  const char* v;
-  const uint8_t* k_scales;  // [n_pages, n_kv], 8-bit pages
-  const uint8_t* v_scales;
-  const int32_t* table;    // [B, width]
-  const int32_t* lengths;  // [B]
-  const int32_t* sizes;    // [B] or null: T each
-  void* out;               // [B, T, n_heads, D]
-  float* partial;          // [n_kv][shares][rows][D], then [..][2] (top, sum), when shares > 0
-  int* runs;               // [B][2]: a sequence's first share and their number
-  int64_t kp, kh, kr, vp, vh, vr;
-  int B, T, n_heads, n_kv, qpk, width, n_pages, shift;
-  int window, sinks;      // window: 2^30 where there is none
-  int shares, row_tiles;  // shares: 0 where no sequence's rows are split
-  float join_cost;        // of one share, in tiles
-  bool fold;              // row tiles from both ends to the middle
-  float scale;            // its magnitude times log2(e); 1 for a scale of zero
-  float sign;             // its sign
-  __device__ int tiles(int b) const;  // that some token of sequence b sees
-};
-
-__device__ __forceinline__ int tiles_of(int rows) { return (rows + kPagedKeys - 1) / kPagedKeys; }
-
-// The tiles that a run of tokens sees: [0, first) and [from, upto).
-struct Seen {
-  int first, from, upto;
-  // low, end: the first row in the window of the run's first token, and the row
-  // behind the last token's own.
-  __device__ __forceinline__ Seen(int low, int sinks, int end) {
-    first = low > 0 ? tiles_of(min(sinks, end)) : 0;
-    from = low / kPagedKeys;
-    if (from <= first) first = from = 0;
-    upto = tiles_of(end);
-  }
-};
-
-// What of sequence b there is: earlier rows, tokens, and all rows.
-struct PagedSpan {
-  int len, live, total;
-  __device__ __forceinline__ PagedSpan(const AttendArgs& a, int b) {
-    const int room = a.width << a.shift;
-    len = min(max(a.lengths[b], 0), room);
-    live = a.sizes != nullptr ? min(max(a.sizes[b], 0), a.T) : a.T;
-    total = live > 0 ? min(len + live, room) : 0;
-  }
-  __device__ __forceinline__ Seen seen(const AttendArgs& a) const {
-    return Seen(total > 0 ? max(len - a.window + 1, 0) : 0, a.sinks, total);
-  }
-};
-__device__ __forceinline__ int AttendArgs::tiles(int b) const {
-  const Seen s = PagedSpan(*this, b).seen(*this);
-  return s.first + s.upto - s.from;
-}
-
-// Unit (16 bytes) u of LDS row r lies at unit u ^ paged_swizzle(r): the reads below
-// cover 32 banks once.  16-bit rows: eight rows of a K read, four rows' 32-byte pieces
-// of a V read.  8-bit rows: eight rows of a K read, the units of rows 4g .. 4g + 3 of two
-// 16-row tiles of a V read.
-template <int UNITS, bool Q8>
-__device__ __forceinline__ int paged_swizzle(int r) {
-  if (!Q8) return ((r & 3) << 1 | (r >> 2 & 1) | (r & 8)) & (UNITS - 1);
-  const int high = (r >> 2 ^ r >> 4) & 1;
-  return UNITS == 8 ? (r & 3) | high << 2 : (r >> 1 & 1) | high << 1;
-}
 
 // One workgroup: 16 QT WQ query rows of one kv head (WQ = 4 / WK waves along the
 // rows, WK along the keys), one share of the rows, in tiles of 64 keys.  A tile's rows
@@ -168,7 +86,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_kernel(AttendArgs a) {
   } else if (w >= a.B) {
     return;
   }
-  const PagedSpan span(a, b);
+  const PagedSpan span = PagedSpan(a, b).uniform();
   const int rows_all = a.T * a.qpk, rows = span.live * a.qpk;
   const int r0 = row_tile * ROWS;
   const int rw = r0 + wq * 16 * QT;  // this wave's first row
@@ -608,8 +526,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_kernel(AttendArgs a) {
 }
 
 struct PagedPlan {
-  int form = 0, rows = 16, row_tiles = 1, shares = 0;
-  size_t workspace_bytes = 0;
+  int form = 0, rows = 16, row_tiles = 1, shares = 0, slots = 0;
+  size_t counter_bytes = 0, workspace_bytes = 0;
 };
 
 int plan_paged(int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv, int64_t head_dim,
@@ -639,8 +557,12 @@ int plan_paged(int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv, int
   const int64_t room = kSplitWorkgroups / (n_kv * p->row_tiles);
   if (room > batch && batch < kSplitWorkgroups && max_rows > 4 * kPagedKeys) {
     p->shares = static_cast<int>(room);
-    p->workspace_bytes =
-        static_cast<size_t>(n_kv * room * rows) * (head_dim + 2) * 4 + static_cast<size_t>(batch) * 8;
+    p->slots = static_cast<int>(p->form <= 1 ? room + batch : room);
+    // (a counter a sequence and kv head, of which there are fewer than workgroups)
+    p->counter_bytes = p->form <= 1 ? kSplitWorkgroups * sizeof(int) : 0;
+    p->workspace_bytes = p->counter_bytes +
+                         static_cast<size_t>(n_kv * p->slots * rows) * (head_dim + 2) * 4 +
+                         static_cast<size_t>(p->form <= 1 ? 0 : batch) * 8;
   }
   return NIBBLE_OK;
 }
@@ -649,9 +571,13 @@ template <class E, int D, bool Q8>
 hipError_t launch_paged(const AttendArgs& a, const PagedPlan& p, hipStream_t stream) {
   const int64_t pairs = static_cast<int64_t>(p.shares > 0 ? p.shares : a.B) * a.n_kv;
   const dim3 grid(static_cast<unsigned>(ceil_div(pairs, 8) * 8 * p.row_tiles));
-  if (p.form == 0) paged_kernel<E, D, 1, 4, Q8><<<grid, kPagedThreads, 0, stream>>>(a);
-  else if (p.form == 1) paged_kernel<E, D, 2, 4, Q8><<<grid, kPagedThreads, 0, stream>>>(a);
-  else if (p.form == 2) paged_kernel<E, D, 2, 2, Q8><<<grid, kPagedThreads, 0, stream>>>(a);
+  if (p.form <= 1) {
+    const dim3 lines(static_cast<unsigned>(pairs));
+    if (p.form == 0) rows_kernel<E, D, 1, Q8><<<lines, kPagedThreads, 0, stream>>>(a);
+    else rows_kernel<E, D, 2, Q8><<<lines, kPagedThreads, 0, stream>>>(a);
+    return hipGetLastError();
+  }
+  if (p.form == 2) paged_kernel<E, D, 2, 2, Q8><<<grid, kPagedThreads, 0, stream>>>(a);
   else paged_kernel<E, D, 2, 1, Q8><<<grid, kPagedThreads, 0, stream>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.shares == 0) return e;
@@ -679,6 +605,14 @@ extern "C" size_t nibble_attention_paged_workspace_bytes(int64_t batch, int64_t 
   PagedPlan p;
   if (plan_paged(batch, tokens, n_heads, n_kv_heads, head_dim, max_rows, &p) != NIBBLE_OK) return 0;
   return p.workspace_bytes;
+}
+
+extern "C" size_t nibble_attention_paged_counter_bytes(int64_t batch, int64_t tokens,
+                                                       int64_t n_heads, int64_t n_kv_heads,
+                                                       int64_t head_dim, int64_t max_rows) {
+  PagedPlan p;
+  if (plan_paged(batch, tokens, n_heads, n_kv_heads, head_dim, max_rows, &p) != NIBBLE_OK) return 0;
+  return p.counter_bytes;
 }
 
 extern "C" int nibble_attention_paged(const void* Q, int64_t dtype, int64_t batch, int64_t tokens,
@@ -724,8 +658,9 @@ extern "C" int nibble_attention_paged(const void* Q, int64_t dtype, int64_t batc
   a.sizes = static_cast<const int32_t*>(sizes);
   a.out = Out;
   a.qpk = static_cast<int>(n_heads / c.n_kv_heads);
-  a.partial = static_cast<float*>(workspace);
-  a.runs = reinterpret_cast<int*>(a.partial + static_cast<size_t>(c.n_kv_heads) * p.shares * tokens *
+  a.counters = static_cast<int*>(workspace);
+  a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.counter_bytes);
+  a.runs = reinterpret_cast<int*>(a.partial + static_cast<size_t>(c.n_kv_heads) * p.slots * tokens *
                                               a.qpk * (c.head_dim + 2));
   a.kp = c.k_page_stride * bytes, a.kh = c.k_head_stride * bytes, a.kr = c.k_row_stride * bytes;
   a.vp = c.v_page_stride * bytes, a.vh = c.v_head_stride * bytes, a.vr = c.v_row_stride * bytes;
@@ -739,6 +674,7 @@ extern "C" int nibble_attention_paged(const void* Q, int64_t dtype, int64_t batc
   a.window = window > 0 ? static_cast<int>(window) : 1 << 30;
   a.sinks = static_cast<int>(sinks);
   a.shares = p.shares;
+  a.slots = p.slots;
   a.row_tiles = p.row_tiles;
   a.join_cost = kPagedShareCost + kPagedRowCost * static_cast<float>(tokens * n_heads);
   a.fold = batch * c.n_kv_heads * p.row_tiles <= kSplitWorkgroups;

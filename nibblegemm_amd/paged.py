@@ -242,7 +242,8 @@ def attention_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     key = ("paged", B, T, n_heads, n_kv, D, cache[7] * cache[9])
     plan = _ws_plan.get(key)
     if plan is None:
-        plan = (ext.attention_paged_workspace_bytes(*key[1:]), -1)
+        need, counters = ext.attention_paged_workspace_bytes(*key[1:])
+        plan = (need, counters if counters else -1)
         _ws_plan[key] = plan
     ws, ws_bytes = _workspace(plan, dev, _stream(dev))
     out = torch.empty_like(q)

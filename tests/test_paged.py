@@ -421,10 +421,10 @@ def test_values_rejections(kwargs, needle):
 
 def test_attention_workspace():
     ext = ng.extension()
-    assert ext.attention_paged_workspace_bytes(1, 1, 32, 8, 128, 128) == 0
-    need = ext.attention_paged_workspace_bytes(1, 1, 32, 8, 128, 65536)
-    assert need > 0
-    assert ext.attention_paged_workspace_bytes(1, 1, 32, 8, 96, 65536) == 0  # a refused plan
+    assert ext.attention_paged_workspace_bytes(1, 1, 32, 8, 128, 128) == (0, 0)
+    need, counters = ext.attention_paged_workspace_bytes(1, 1, 32, 8, 128, 65536)
+    assert need > counters > 0 and counters % 256 == 0
+    assert ext.attention_paged_workspace_bytes(1, 1, 32, 8, 96, 65536) == (0, 0)  # a refused plan
     big = dict(T=1, nh=32, nkv=8, width=4096)
     assert attend(ext, **big) == WORKSPACE and "workspace" in ext.last_error()
     assert attend(ext, **big, ws=P, wsb=need - 1) == WORKSPACE
