@@ -549,20 +549,22 @@ int plan_paged(int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv, int
   p->form = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
   p->rows = 16 << p->form;
   p->row_tiles = static_cast<int>(ceil_div(rows, p->rows));
-  NIBBLE_CHECK(ceil_div(batch * n_kv, 8) * 8 * p->row_tiles * kPagedThreads < (int64_t(1) << 32),
+  NIBBLE_CHECK(ceil_div(batch, 8) * 8 * n_kv * p->row_tiles * kPagedThreads < (int64_t(1) << 32),
                "%lld sequences of %lld kv heads: a launch ends at 2^32 threads", (long long)batch,
                (long long)n_kv);
   // Room for more workgroups than there are (sequence, kv head, row tile)s: the
   // cached rows are split, unless there are but a few tiles of them.
   const int64_t room = kSplitWorkgroups / (n_kv * p->row_tiles);
-  if (room > batch && batch < kSplitWorkgroups && max_rows > 4 * kPagedKeys) {
+  const bool line = p->form <= 1;
+  if (line ? room > 0 && batch <= kSplitWorkgroups && batch * n_kv < 4 * kSplitWorkgroups
+           : room > batch && batch < kSplitWorkgroups) {
+    if (max_rows <= 4 * kPagedKeys) return NIBBLE_OK;
     p->shares = static_cast<int>(room);
-    p->slots = static_cast<int>(p->form <= 1 ? room + batch : room);
-    // (a counter a sequence and kv head, of which there are fewer than workgroups)
-    p->counter_bytes = p->form <= 1 ? kSplitWorkgroups * sizeof(int) : 0;
+    p->slots = static_cast<int>(line ? 2 * room : room);
+    p->counter_bytes = line ? 4 * kSplitWorkgroups * sizeof(int) : 0;  // a sequence and kv head
     p->workspace_bytes = p->counter_bytes +
                          static_cast<size_t>(n_kv * p->slots * rows) * (head_dim + 2) * 4 +
-                         static_cast<size_t>(p->form <= 1 ? 0 : batch) * 8;
+                         static_cast<size_t>(line ? 0 : batch) * 8;
   }
   return NIBBLE_OK;
 }
@@ -572,7 +574,8 @@ hipError_t launch_paged(const AttendArgs& a, const PagedPlan& p, hipStream_t str
   const int64_t pairs = static_cast<int64_t>(p.shares > 0 ? p.shares : a.B) * a.n_kv;
   const dim3 grid(static_cast<unsigned>(ceil_div(pairs, 8) * 8 * p.row_tiles));
   if (p.form <= 1) {
-    const dim3 lines(static_cast<unsigned>(pairs));
+    const dim3 lines(static_cast<unsigned>(
+        ceil_div(p.shares > 0 ? p.shares : a.B, 8) * 8 * a.n_kv));
     if (p.form == 0) rows_kernel<E, D, 1, Q8><<<lines, kPagedThreads, 0, stream>>>(a);
     else rows_kernel<E, D, 2, Q8><<<lines, kPagedThreads, 0, stream>>>(a);
     return hipGetLastError();

@@ -30,31 +30,70 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// The sequences' tiles one behind the other, cut into a.shares shares of `per` tiles
-// (the last one less, or nothing), whatever sequences they are of.  The lengths are on
-// the GPU: every wave works it out alike, 64 sequences at a time, one a lane.  A share's
-// piece of sequence b has slot share + b, which rises from piece to piece.
+// Sum of the values of a wave's lanes.
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+
+// What a sequence more costs a share, in tiles of one byte a value (its queries, pages
+// and first rows come one behind the other, and its waves meet), and what pieces that
+// are joined cost.
+constexpr int kSequenceCost = 4, kJoinCost = 5;
+
+// Which tiles of which sequences a share has.  Where it costs no more than a sequence's
+// start, every sequence is cut by itself, into equal pieces (one, if that is as good):
+// `per` tiles at most, the least of a few for which there are enough shares.  Else the
+// sequences' tiles are laid one behind the other, a sequence's behind a gap of what it
+// costs, and all that is cut into equal shares.  The lengths are on the GPU: every wave
+// works it out alike, 64 sequences at a time, one a lane.
 struct Line {
-  int upto = 0;              // tiles to the end of this lane's sequence, of the 64 from `from`
-  int from = 0, before = 0;  // and the tiles before those
-  int per = 0, total = 0;
-  bool empties = false;      // there are sequences without a tile
-  __device__ __forceinline__ void cut(const AttendArgs& a) {
+  int n = 0, upto = 0;       // of this lane's sequence, of the 64 from `from`: tiles and gap
+  int from = 0, before = 0;  // (or pieces), those to its end, and those before the 64
+  int per = 0, total = 0, gap = 0;
+  bool alone = false;    // a share has a piece of one sequence
+  bool empties = false;  // there are sequences without a tile
+  __device__ __forceinline__ void cut(const AttendArgs& a, int sequence_cost) {
+    gap = sequence_cost;
 #pragma unroll 1
     for (int i = 0; i < a.B; i += 64) take(a, i, total), total = last();
-    // per tiles in turn, and total / per shares whose sums are written and joined
-    const int worth = static_cast<int>(
-        __builtin_amdgcn_sqrtf(a.join_cost * static_cast<float>(total)));
-    per = __builtin_amdgcn_readfirstlane(max(max((total + a.shares - 1) / a.shares, worth), 1));
+    per = __builtin_amdgcn_readfirstlane(max((total + a.shares - 1) / a.shares, 1));
+    if (a.B > 64) return;
+    if (a.B == 1) {  // (the same without a look at other lanes)
+      const int tiles = total > 0 ? total - gap : 0;
+      const int worth = static_cast<int>(
+          __builtin_amdgcn_sqrtf(a.join_cost * static_cast<float>(tiles)));
+      const int least = max(max((tiles + a.shares - 1) / a.shares, worth), 1);
+      const int size = tiles <= least + kJoinCost ? max(tiles, 1) : least;
+      alone = true, gap = 0;
+      upto = total = __builtin_amdgcn_readfirstlane((tiles + size - 1) / size);
+      return;
+    }
+    const int tiles = n > 0 ? n - gap : 0;
+    // (below 2^24: exact in fp32)
+    const int most = __builtin_amdgcn_readfirstlane(static_cast<int>(wave_max(static_cast<float>(tiles))));
+    const int all = wave_total(tiles);
+    // `least` tiles in turn, and all / least pieces whose sums are written and joined
+    const int worth = static_cast<int>(__builtin_amdgcn_sqrtf(a.join_cost * static_cast<float>(all)));
+    const int least = __builtin_amdgcn_readfirstlane(
+        max(max((all + a.shares - 1) / a.shares, worth), 1));
+    // one piece each, or as many of `least` and a few more tiles as there is room for
+#pragma unroll 1
+    for (int k = -1; k <= 4; ++k) {
+      const int size = k < 0 ? most : least + (sequence_cost * k + 3) / 4;
+      if (k < 0 && most > least + kJoinCost) continue;
+      const int pieces = tiles > 0 ? (tiles + size - 1) / size : 0;
+      if (size > 0 && wave_total(pieces) <= a.shares) {
+        alone = true, gap = 0, n = pieces, upto = wave_scan(pieces), total = last();
+        return;
+      }
+    }
   }
   __device__ __forceinline__ void take(const AttendArgs& a, int i, int tiles) {
-    const int b = i + static_cast<int>(threadIdx.x & 63), n = b < a.B ? a.tiles(b) : 0;
-    empties |= __any(b < a.B && n == 0) != 0;
+    const int b = i + static_cast<int>(threadIdx.x & 63), t = b < a.B ? a.tiles(b) : 0;
+    empties |= __any(b < a.B && t == 0) != 0;
+    n = t > 0 ? t + gap : 0;
     from = i, before = tiles, upto = before + wave_scan(n);
   }
   __device__ __forceinline__ int last() const { return __builtin_amdgcn_readlane(upto, 63); }
-  // The sequence of tile x < total, and the tiles [start, end) of the line that it has.
-  // (x does not fall from call to call.)
+  // The sequence at place x < total of the line, and the places [start, end) that it has.
   __device__ __forceinline__ int find(const AttendArgs& a, int x, int* start, int* end) {
     if (a.B > 64 && (x < before || x >= last())) {
       int tiles = 0;
@@ -88,7 +127,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void rows_kernel(AttendArgs a) {
   constexpr int BYTES = Q8 ? D : 2 * D, UNITS = BYTES / 16;  // of a row; its 16-byte units
   constexpr int CROWS = 64 / UNITS, COPIES = 16 / CROWS;     // rows of a copy; of k or v, a unit
   constexpr int kUnit = 16 * BYTES;
-  constexpr int NB = 16384 / (2 * kUnit);
+  constexpr int NB = 8192 / (2 * kUnit);
   constexpr int kPending = (2 * NB - 1) * COPIES;  // copies behind those that are waited for
   constexpr int QUADS = D / 4, ALL = QT * 16;
   constexpr int ROWS = kPagedThreads / QUADS;  // rows of outputs at once
@@ -98,15 +137,18 @@ __global__ __launch_bounds__(kPagedThreads, 2) void rows_kernel(AttendArgs a) {
   typedef T vec4 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) s4_t lds4_t;
   typedef __attribute__((address_space(3))) i2_t lds2_t;
-  static_assert(4 * 4 * ALL * D <= 4 * NB * 2 * kUnit, "the sums fit");
-  __shared__ __attribute__((aligned(16))) char ring[4 * NB * 2 * kUnit];
+  constexpr int kRing = 4 * NB * 2 * kUnit, kSums = 4 * 4 * ALL * D;
+  __shared__ __attribute__((aligned(16))) char ring[kRing > kSums ? kRing : kSums];
   __shared__ float stat[2][4][ALL > ROWS ? ALL : ROWS];
   __shared__ int arrived;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int g = lane >> 4, c = lane & 15;
-  const int w = blockIdx.x / a.n_kv, h = blockIdx.x - w * a.n_kv;
+  // The heads of a share on one XCD (id % 8): they read the same pages.
+  const int eight = blockIdx.x / (8 * a.n_kv), in_eight = blockIdx.x - eight * 8 * a.n_kv;
+  const int w = 8 * eight + (in_eight & 7), h = in_eight >> 3;
+  if (w >= (a.shares > 0 ? a.shares : a.B)) return;
   const int rows_all = a.T * a.qpk;
   const int u = threadIdx.x % QUADS, mine = threadIdx.x / QUADS;  // of an output: its quad, row
   f4_t* const red = reinterpret_cast<f4_t*>(ring);
@@ -127,11 +169,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void rows_kernel(AttendArgs a) {
     return top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - most);
   };
 
-  int at = 0, upto = 1;  // of the line: tiles (or, where nothing is split, this sequence)
+  int at = 0, upto = 1;  // this share's places (or, where nothing is split, a sequence)
   Line line;
   if (a.shares > 0) {
-    line.cut(a);
-    at = w * line.per, upto = min(at + line.per, line.total);
+    line.cut(a, Q8 ? kSequenceCost : kSequenceCost / 2);
+    at = line.alone ? w : w * line.per, upto = min(line.alone ? w + 1 : at + line.per, line.total);
     if (line.empties)  // zeros for sequences of which nothing is seen
 #pragma unroll 1
       for (int b = w; b < a.B; b += a.shares)
@@ -141,17 +183,28 @@ __global__ __launch_bounds__(kPagedThreads, 2) void rows_kernel(AttendArgs a) {
   }
 #pragma unroll 1
   while (at < upto) {
-    // The next sequence's tiles [x0, x0 + count), those that it sees counted.
-    int b = w, start = 0, stop = 0, x0 = 0, count;
-    if (a.shares > 0) {
-      b = line.find(a, at, &start, &stop);
-      x0 = at - start, count = min(upto, stop) - at;
-    } else {
-      count = __builtin_amdgcn_readfirstlane(a.tiles(b));
-    }
-    const bool whole = a.shares == 0 || (x0 == 0 && start + count == stop);
+    // The next sequence's tiles [x0, x0 + count), those that it sees counted: piece
+    // `piece` of `pieces`, the first of which is of share `first`.
+    int b = w, start = 0, stop = 0;
+    if (a.shares > 0) b = line.find(a, at, &start, &stop);
     const PagedSpan span = PagedSpan(a, b).uniform();
     const Seen all = span.seen(a);
+    int x0 = 0, count = all.first + all.upto - all.from, first = w, pieces = 1;
+    if (line.alone) {
+      first = start, pieces = stop - start;
+      const int size = (count + pieces - 1) / pieces;
+      x0 = (w - start) * size, count = min(size, count - x0);
+      at = upto;
+    } else if (a.shares > 0) {
+      start += line.gap;
+      const int begin = max(at, start);
+      at = min(upto, stop);
+      if (begin >= at) continue;
+      first = start / line.per, pieces = (stop - 1) / line.per - first + 1;
+      x0 = begin - start, count = at - begin;
+    } else {
+      at = upto;
+    }
     const int rows = span.live * a.qpk, late = span.live - 1, end = span.total;
     const int low = max(span.len - a.window + 1, 0);
     auto key_of = [&](int i) {  // of this wave's unit of the i-th tile
@@ -463,8 +516,13 @@ __global__ __launch_bounds__(kPagedThreads, 2) void rows_kernel(AttendArgs a) {
         red[(wave * ALL + row) * QUADS + ((4 * d + g) ^ (c & 7))] = acc[t][d];
     }
     lds_barrier();
-    // A piece's sums [rows][D], and its rows' (top, sum), seen by every XCD.
-    const int slot = w + b;
+    // A piece's sums [rows][D], and its rows' (top, sum), seen by every XCD.  A share has
+    // two places: the second for a sequence that begins within it, and goes on.
+    auto slot_of = [&](int s) {
+      return 2 * s + (!line.alone && s == first && s * line.per < start ? 1 : 0);
+    };
+    const int slot = slot_of(w);
+    const bool whole = pieces == 1;
     auto sums_of = [&](int s) {
       const int64_t n = static_cast<int64_t>(rows_all) * D;
       return coherent(a.partial + (static_cast<int64_t>(h) * a.slots + s) * n);
@@ -499,7 +557,6 @@ __global__ __launch_bounds__(kPagedThreads, 2) void rows_kernel(AttendArgs a) {
     }
     if (!whole) {
       // The piece is written; the last of its sequence (and head) to be so joins them.
-      const int first = start / line.per, pieces = (stop - 1) / line.per - first + 1;
       wait_vm_stores();
       lds_barrier();
       int* const counter = a.counters + b * a.n_kv + h;
@@ -523,10 +580,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void rows_kernel(AttendArgs a) {
           for (int s0 = 0; s0 < pieces; s0 += N * G) {
             float tops[N], ls[N], most = mr;
             f4_t v[N];
-            const auto sums = sums_of(first + b + s0), stats = stats_of(first + b + s0);
+            const auto sums = sums_of(2 * (first + s0)), stats = stats_of(2 * (first + s0));
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-              const int s = min(e * G + grp, pieces - 1 - s0), at_row = s * rows_all + row;
+              const int s = min(e * G + grp, pieces - 1 - s0);
+              const int at_row = (slot_of(first + s0 + s) - 2 * (first + s0)) * rows_all + row;
               const u2_t st = __builtin_bit_cast(
                   u2_t, __builtin_amdgcn_raw_buffer_load_b64(stats, at_row * 8, 0, kCoherent));
               tops[e] = __builtin_bit_cast(float, static_cast<uint32_t>(st[0]));
@@ -573,7 +631,6 @@ __global__ __launch_bounds__(kPagedThreads, 2) void rows_kernel(AttendArgs a) {
         }
       }
     }
-    at = a.shares > 0 ? at + count : upto;
     if (at < upto) lds_barrier();  // the sums have been read
   }
 }
