@@ -24,6 +24,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "paged_prompt.h"
 #include "paged_rows.h"
 
 namespace nibble {
@@ -581,7 +582,7 @@ hipError_t launch_paged(const AttendArgs& a, const PagedPlan& p, hipStream_t str
     return hipGetLastError();
   }
   if (p.form == 2) paged_kernel<E, D, 2, 2, Q8><<<grid, kPagedThreads, 0, stream>>>(a);
-  else paged_kernel<E, D, 2, 1, Q8><<<grid, kPagedThreads, 0, stream>>>(a);
+  else prompt_kernel<E, D, 1, Q8><<<grid, kPagedThreads, 0, stream>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.shares == 0) return e;
   const int64_t parts = ceil_div(static_cast<int64_t>(a.T) * a.qpk, kSplitThreads / (D / 4));

@@ -1,0 +1,520 @@
+// Attention over a paged cache for many query rows a kv head: prompts, and parts of them.
+#pragma once
+
+#include "paged_attention.h"
+
+namespace nibble {
+namespace {
+
+typedef float f16_t __attribute__((ext_vector_type(16)));
+
+template <class E>
+__device__ __forceinline__ f16_t mfma32(typename E::vec8 a, typename E::vec8 b, f16_t c) {
+  if constexpr (std::is_same_v<E, Half>) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+// c + x[0] + x[1]
+template <class E, class V>
+__device__ __forceinline__ float add_pair(V x, float c) {
+  const typename E::type one = static_cast<typename E::type>(1.0f);
+  if constexpr (std::is_same_v<E, Half>) return __builtin_amdgcn_fdot2(x, V{one, one}, c, false);
+  else return __builtin_amdgcn_fdot2_f32_bf16(x, V{one, one}, c, false);
+}
+
+// Unit (16 bytes) u of LDS row r lies at unit u ^ prompt_swizzle(r), so that eight rows of
+// a K read, and the rows of a V read (four and 32 bytes of each, or, of 8 bits, 4h .. 4h +
+// 3 and 8 + 4h .. and 16 bytes), cover 32 banks once.
+template <int UNITS, bool Q8>
+__device__ __forceinline__ int prompt_swizzle(int r) {
+  if (!Q8) return paged_swizzle<UNITS, false>(r);
+  const int high = (r >> 2 ^ r >> 3) & 1;
+  return UNITS == 8 ? (r & 3) | high << 2 : (r >> 1 & 1) | high << 1;
+}
+
+// One workgroup: 128 QN query rows of one kv head, 32 QN a wave, and one share of the rows, in
+// tiles of 64 keys, which are copied straight into LDS, v into one of two buffers while the
+// tile before is computed, k, a tile ahead of it, into one of three.
+//
+// A 32x32x16 product takes keys as rows and queries as columns, so lane (f = l / 32, c = l
+// % 32) gets the scores of query c for keys 8 a + 4 f .. + 3 (a = 0 .. 3) of a 32-key tile,
+// and its probabilities are where the second product (V^T P^T) wants them, if its k runs
+// over a lane's keys in turn.
+template <class E, int D, int QN, bool Q8>
+__global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(AttendArgs a) {
+  using T = typename E::type;
+  using vec8 = typename E::vec8;
+  constexpr int KT = kPagedKeys, ROWS = 128 * QN;
+  constexpr int BYTES = Q8 ? D : 2 * D, UNITS = BYTES / 16;  // of a row; its 16-byte units
+  constexpr int CROWS = 64 / UNITS, COPIES = 16 / CROWS;     // rows of a copy; of k or v, a wave
+  constexpr uint32_t kTile = KT * BYTES;                     // bytes of a tile of k or v
+  typedef short s4_t __attribute__((ext_vector_type(4)));
+  typedef int i2_t __attribute__((ext_vector_type(2)));
+  typedef T pair_t __attribute__((ext_vector_type(2)));
+  typedef unsigned short us4_t __attribute__((ext_vector_type(4)));
+  typedef unsigned short us8_t __attribute__((ext_vector_type(8)));
+  typedef __attribute__((address_space(3))) s4_t lds4_t;
+  typedef __attribute__((address_space(3))) i2_t lds2_t;
+  __shared__ __attribute__((aligned(16))) char kv[5 * kTile];  // v, v, k, k, k
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int f = lane >> 5, c = lane & 31;
+  // Workgroup -> (share, kv head), row tile: the row tiles that read the same cache rows
+  // run on one XCD (id % 8) and share its L2.  The later row tiles are longer: longest
+  // first, or, where all are on the CUs at once, two a CU, each with its counterpart.
+  const int slot = blockIdx.x >> 3;
+  const int pair = slot / a.row_tiles * 8 + (blockIdx.x & 7);
+  const int rt = slot % a.row_tiles;
+  const int row_tile = a.fold && rt >= (a.row_tiles + 1) / 2 ? rt - (a.row_tiles + 1) / 2
+                                                             : a.row_tiles - 1 - rt;
+  const int w = pair / a.n_kv, h = pair - w * a.n_kv;
+  int b = w, share = 0, per = 0x3fffffff;  // the whole sequence
+  if (a.shares > 0) {
+    if (w >= a.shares) return;
+    const Shares<AttendArgs> shares(a, w);
+    if (shares.found < 0) return;
+    b = shares.found, share = w - shares.first, per = shares.per;
+    // (for the kernel that joins them)
+    if (share == 0 && h == 0 && rt == 0 && threadIdx.x == 0)
+      a.runs[2 * b] = shares.first, a.runs[2 * b + 1] = shares.count;
+  } else if (w >= a.B) {
+    return;
+  }
+  const PagedSpan span = PagedSpan(a, b).uniform();
+  const int rows_all = a.T * a.qpk, rows = span.live * a.qpk;
+  const int r0 = row_tile * ROWS;
+
+  // Rows of the cache [low, end) and those before a.sinks matter to this workgroup's
+  // tokens, early to late; of their tiles it takes those of its share: [a0, a0 + na) and
+  // those from b0 on.
+  const int early = r0 / a.qpk, late = (min(r0 + ROWS, rows) - 1) / a.qpk;
+  const int end = r0 < rows ? min(span.total, span.len + late + 1) : 0;
+  const int low = end > 0 ? max(span.len + early - a.window + 1, 0) : 0;
+  int a0, na, b0, count;
+  {
+    const Seen all = span.seen(a), own(low, a.sinks, end);
+    const int x0 = min(share * per, 0x3fffffff), x1 = x0 + min(per, 0x3fffffff);  // of all's tiles
+    const int shift = all.from - all.first;  // from place to tile, behind the first
+    a0 = x0;
+    na = max(0, min(all.first > 0 ? min(x1, all.first) : x1, own.first) - a0);
+    b0 = max(max(x0, all.first) + shift, own.from);
+    count = na + max(0, min(x1 + shift, own.upto) - b0);
+  }
+  auto key_of = [&](int i) { return (i < na ? a0 + i : b0 + i - na) * KT; };
+
+  // Queries: lane (f, c) holds of row c of 32 the elements that it multiplies with those of
+  // a key: of 16 8 f .., or with 8-bit keys, of 32 16 f ...
+  vec8 q[QN][D / 16];
+  int pos[QN];  // the row of its token
+#pragma unroll
+  for (int t = 0; t < QN; ++t) {
+    const int r = r0 + (wave * QN + t) * 32 + c;
+    const bool in = r < rows;
+    const int node = in ? r / a.qpk : 0;
+    pos[t] = span.len + node;
+    const T* const from = static_cast<const T*>(a.q) +
+                          ((static_cast<int64_t>(b) * a.T + node) * a.n_heads + h * a.qpk +
+                           (in ? r - node * a.qpk : 0)) * D;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      const int e = Q8 ? 32 * (s / 2) + 16 * f + 8 * (s % 2) : 16 * s + 8 * f;
+      q[t][s] = in ? *reinterpret_cast<const vec8*>(from + e) : vec8{};
+    }
+    if (a.sign != 1.0f) {  // a scale that is not positive: its sign goes into q, exactly
+#pragma unroll
+      for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          q[t][s][i] = static_cast<T>(static_cast<float>(q[t][s][i]) * a.sign);
+    }
+  }
+
+  // The pages of a tile's four 16-row groups: lane l has that of group l % 4.
+  const int32_t* const table = a.table + static_cast<int64_t>(b) * a.width;
+  auto entry = [&](int i) {
+    return table[min((key_of(min(i, count - 1)) + 16 * (lane & 3)) >> a.shift, a.width - 1)];
+  };
+  auto is_page = [&](int page) { return page >= 0 && page < a.n_pages; };
+  const uint32_t lds0 = lds_address(kv) + wave * COPIES * 1024u;
+  // This wave's copies of tile i's k (v), whose pages are `pages`; rows that none of the
+  // workgroup's tokens sees read as zeros.
+  auto copy = [&](int i, int pages, const char* base, int64_t page_stride, int64_t row_stride,
+                  uint32_t dst) {
+    const int page = __builtin_amdgcn_readlane(pages, wave);
+    const int key0 = key_of(i) + 16 * wave;
+    const int here = is_page(page) ? end : 0;
+    const char* const from = base + (is_page(page) ? page : 0) * page_stride +
+                             (key0 & ((1 << a.shift) - 1)) * row_stride;
+#pragma unroll
+    for (int u = 0; u < COPIES; ++u) {
+      const int r = u * CROWS + lane / UNITS, key = key0 + r;
+      const bool in = key < here && (key >= low || key < a.sinks);
+      const uint32_t unit16 = ((lane % UNITS) ^ prompt_swizzle<UNITS, Q8>(16 * wave + r)) * 16u;
+      lds_copy16(from, 0x7fffffffu, dst + u * 1024u,
+                 in ? r * static_cast<uint32_t>(row_stride) + unit16 : kOutOfRange);
+    }
+  };
+  auto copy_k = [&](int i, int pages, uint32_t buf) {
+    copy(i, pages, a.k + h * a.kh, a.kp, a.kr, lds0 + buf);
+  };
+  auto copy_v = [&](int i, int pages) {
+    copy(i, pages, a.v + h * a.vh, a.vp, a.vr, lds0 + (i & 1) * kTile);
+  };
+
+  f16_t acc[QN][D / 32];
+  float top[QN], sum[QN][2];  // the reference of query c, in powers of two; of the probabilities
+#pragma unroll
+  for (int t = 0; t < QN; ++t) {
+    top[t] = -INFINITY, sum[t][0] = sum[t][1] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) acc[t][d] = f16_t{};
+  }
+
+  // Byte offsets within a tile: of row c, k elements 8 f .. of each 16 (8 bits: 16 f .. of
+  // each 32); v elements 4 (l % 4) .. of 16 of row 4 f + l / 4 % 4 (8 bits: 8 (l % 2) .. of
+  // row 4 f + l / 2 % 4, + 8 for l / 8 % 2), the second 16 of 32 for l / 16 % 2.
+  const int half = lane >> 4 & 1;
+  const int krow = c * BYTES + ((f ^ prompt_swizzle<UNITS, Q8>(c)) * 16);
+  int vrow;
+  if constexpr (Q8) {
+    const int x = lane >> 1 & 7, r = 8 * (x >> 2) + 4 * f + (x & 3);
+    vrow = r * BYTES + ((half ^ prompt_swizzle<UNITS, true>(r)) * 16) + 8 * (lane & 1);
+  } else {
+    const int r = 4 * f + (lane >> 2 & 3);
+    vrow = r * BYTES + (((2 * half + (lane >> 1 & 1)) ^ prompt_swizzle<UNITS, false>(r)) * 16) +
+           8 * (lane & 1);
+  }
+  float kscale[4], vscale[4];  // 8 bits: of a tile's 16-row groups
+  struct Scores {
+    f16_t s[QN];  // of 32 keys
+  };
+  // K's operands of 32 keys: the e-th product takes lane elements from LDS four products
+  // ahead.
+  constexpr int N = D / 16, AHEAD = 4;
+  constexpr int kFree = Q8 ? AHEAD - 1 : AHEAD;  // product e leaves room for that of e + kFree
+  struct Ahead {
+    vec8 at[AHEAD];
+  };
+  // (j: which 32 keys of the tile at `buf`.  8 bits: two products' elements side by side)
+  auto read_k = [&](Ahead& x, int e, uint32_t buf, int j) {
+    if constexpr (Q8) {
+      if (e % 2 == 1 || e >= N) return;
+      const float s = c < 16 ? kscale[2 * j] : kscale[2 * j + 1];
+      const u4_t w4 =
+          *reinterpret_cast<const u4_t*>(kv + buf + j * 32 * BYTES + (krow ^ (32 * (e / 2))));
+      x.at[e % AHEAD] = from_float8<E>(w4[0], w4[1], s, s);
+      x.at[e % AHEAD + 1] = from_float8<E>(w4[2], w4[3], s, s);
+    } else if (e < N) {
+      x.at[e % AHEAD] =
+          *reinterpret_cast<const vec8*>(kv + buf + j * 32 * BYTES + (krow ^ (32 * e)));
+    }
+  };
+  // V^T of the n-th 16 keys for 32 elements.
+  auto values = [&](int buf, int d, int n) {
+    const uint32_t vt = lds_address(kv) + buf * kTile + n * 16 * BYTES;
+    if constexpr (Q8) {
+      const i2_t v2 = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+          (lds2_t*)(uintptr_t)(vt + (vrow ^ (32 * d))));
+      return from_float8<E>(v2[0], v2[1], vscale[n], vscale[n]);
+    } else {
+      s4_t v2[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        v2[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds4_t*)(uintptr_t)(vt + e * 8 * BYTES + (vrow ^ (64 * d) ^ (UNITS > 8 ? 128 * e : 0))));
+      return __builtin_bit_cast(
+          vec8, us8_t(__builtin_shufflevector(__builtin_bit_cast(us4_t, v2[0]),
+                                              __builtin_bit_cast(us4_t, v2[1]), 0, 1, 2, 3, 4, 5, 6, 7)));
+    }
+  };
+  // Hides what this lane's queries do not see of 32 keys; `has`: which of their two 16-row
+  // groups has a page.
+  auto hide = [&](Scores& x, int key0, uint32_t has) {
+    auto below = [](int n) { return (1u << min(max(n, 0), 4)) - 1u; };
+#pragma unroll
+    for (int t = 0; t < QN; ++t)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int key = key0 + 8 * u + 4 * f;
+        const uint32_t near = ~below(pos[t] - a.window + 1 - key) | below(a.sinks - key);
+        uint32_t seen = near & below(min(pos[t] + 1, end) - key);
+        seen = (has >> (u / 2) & 1u) != 0 ? seen : 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((seen >> e & 1u) == 0) x.s[t][4 * u + e] = -INFINITY;
+      }
+  };
+  auto move = [&](const Scores& x) {
+    float m[QN];
+    bool moves = false;
+#pragma unroll
+    for (int t = 0; t < QN; ++t) {
+      m[t] = x.s[t][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) m[t] = fmaxf(m[t], x.s[t][e]);
+      m[t] *= a.scale;
+      moves |= m[t] - top[t] > kPagedSlack + kPagedLift<E>;
+    }
+    if (!__any(moves)) return;
+#pragma unroll
+    for (int t = 0; t < QN; ++t) {
+      const Pair both = swap_pair<32>(m[t]);
+      const float up = fmaxf(fmaxf(both.a, both.b) - kPagedLift<E>, top[t]);
+      const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - up);
+      top[t] = up;
+      sum[t][0] *= keep, sum[t][1] *= keep;
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[t][d][e] *= keep;
+    }
+  };
+  // Probabilities and sums of 32 keys (the j-th of tile i), beside the scores of the next
+  // 32 (the next_j-th of the tile at `buf`): a product of the scores, two exponentials, and
+  // so on, then the sums' products.
+  auto turn = [&](const Scores& x, Scores& next, int i, int j, uint32_t buf, int next_j) {
+    Ahead k, v;
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) read_k(k, e, buf, next_j);
+    move(x);
+    vec8 p[QN][2];
+    float base[QN];
+#pragma unroll
+    for (int t = 0; t < QN; ++t) base[t] = top[t] == -INFINITY ? 0.0f : top[t];
+    auto read_v = [&](int e) { v.at[e % AHEAD] = values(i & 1, e % (D / 32), 2 * j + e / (D / 32)); };
+    constexpr int PER = 16 / N;  // scores beside a product
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+#pragma unroll
+      for (int t = 0; t < QN; ++t) {
+        next.s[t] = mfma32<E>(k.at[e % AHEAD], q[t][e], e == 0 ? f16_t{} : next.s[t]);
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+          const int at = e * PER + u;
+          p[t][at / 8][at % 8] = static_cast<T>(
+              __builtin_amdgcn_exp2f(__builtin_fmaf(x.s[t][at], a.scale, -base[t])));
+          // (The probabilities are rounded to 16 bits because the matrix cores take them so:
+          // each is off by half a step at most, in fp16 of 2^-24 at least, and the sum, in
+          // fp32, is of the rounded.)
+          if (u % 2 == 1)
+            sum[t][u / 2 & 1] = add_pair<E>(
+                pair_t{p[t][at / 8][at % 8 - 1], p[t][at / 8][at % 8]}, sum[t][u / 2 & 1]);
+        }
+      }
+      read_k(k, e + kFree, buf, next_j);
+      if (e + AHEAD >= N) read_v(e + AHEAD - N);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    constexpr int M = D / 16;
+#pragma unroll
+    for (int e = 0; e < M; ++e) {
+#pragma unroll
+      for (int t = 0; t < QN; ++t)
+        acc[t][e % (D / 32)] = mfma32<E>(v.at[e % AHEAD], p[t][e / (D / 32)], acc[t][e % (D / 32)]);
+      if (e + AHEAD < M) read_v(e + AHEAD);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Takes what is not finite out of this wave's 16 rows of a tile's v, for a hidden row's
+  // infinity or NaN must not meet its zero probability.  What tokens that see them are to
+  // have is left for the end.
+  bool cleaned = false;
+  auto clean = [&](int buf) {
+    u4_t* const vt = reinterpret_cast<u4_t*>(kv + buf * kTile + 16 * wave * BYTES);
+    const float s = wave < 2 ? (wave == 0 ? vscale[0] : vscale[1])
+                             : (wave == 2 ? vscale[2] : vscale[3]);
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < 16 * UNITS / 64; ++e) {
+      u4_t x = vt[e * 64 + lane];
+      if constexpr (Q8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const us8_t y = __builtin_bit_cast(us8_t, from_float8<E>(x[i], 0, s, s));
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const bool is = (y[n] & E::kExponent) == E::kExponent;
+            any |= is;
+            x[i] &= is ? ~(0xffu << (8 * n)) : ~0u;
+          }
+        }
+      } else {
+        const us8_t y = __builtin_bit_cast(us8_t, x);
+        const us8_t fine = (y & E::kExponent) == E::kExponent ? us8_t{} : y;
+        x = __builtin_bit_cast(u4_t, fine);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) any |= fine[n] != y[n];
+      }
+      if (__any(any)) vt[e * 64 + lane] = x;
+    }
+    cleaned |= __any(any) != 0;
+  };
+
+  // Pages (and scales) of tiles i (0), i + 1 and i + 2, and which of tile i's groups, and of
+  // the next one's, have a page.
+  int pages1 = 0, pages2 = 0, k1 = 0, v0 = 0, v1 = 0;
+  uint32_t has0 = 0, has1 = 0;
+  auto scales_of = [&](int pages, int* k, int* v) {
+    if constexpr (Q8) {
+      const int64_t at = static_cast<int64_t>(is_page(pages) ? pages : 0) * a.n_kv + h;
+      *k = a.k_scales[at], *v = a.v_scales[at];
+    }
+  };
+  auto spread = [&](int bytes, float (&to)[4]) {
+    if constexpr (Q8) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) to[n] = power(__builtin_amdgcn_readlane(bytes, n));
+    }
+  };
+  // Every query sees all of a tile's keys.
+  auto plain = [&](int i, uint32_t has) {
+    const int key0 = key_of(i);
+    return has == 15u && key0 + KT <= min(span.len + early + 1, end) &&
+           (key0 > span.len + late - a.window || key0 + KT <= a.sinks);
+  };
+  Scores x, y;
+  uint32_t buf0 = 2 * kTile, buf1 = 3 * kTile, buf2 = 4 * kTile;  // of k of tiles i, i + 1, i + 2
+  if (count > 0) {
+    pages1 = entry(0);
+    pages2 = entry(1);
+    int k0 = 0;
+    scales_of(pages1, &k0, &v0);
+    scales_of(pages2, &k1, &v1);
+    has0 = __ballot(is_page(pages1)) & 15u;
+    has1 = __ballot(is_page(pages2)) & 15u;
+    copy_k(0, pages1, buf0);
+    copy_v(0, pages1);
+    if (count > 1) copy_k(1, pages2, buf1);
+    pages1 = pages2;
+    pages2 = entry(2);
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+    lds_barrier();
+    spread(k0, kscale);
+    Ahead k;
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) read_k(k, e, buf0, 0);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+#pragma unroll
+      for (int t = 0; t < QN; ++t)
+        x.s[t] = mfma32<E>(k.at[e % AHEAD], q[t][e], e == 0 ? f16_t{} : x.s[t]);
+      read_k(k, e + kFree, buf0, 0);
+    }
+  }
+#pragma unroll 1
+  for (int i = 0; i < count; ++i) {
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // v of tile i and k of tile i + 1 are there
+    lds_barrier();
+    const uint32_t has = has0;
+    const int key0 = key_of(i);
+    const bool all = plain(i, has);
+    spread(v0, vscale);
+    if (!all) {
+      clean(i & 1);
+      lds_barrier();
+    }
+    const int next_k = k1;
+    v0 = v1, has0 = has1;
+    if (i + 1 < count) copy_v(i + 1, pages1);
+    if (i + 2 < count) {
+      copy_k(i + 2, pages2, buf2);
+      scales_of(pages2, &k1, &v1);
+      has1 = __ballot(is_page(pages2)) & 15u;
+      pages1 = pages2;
+      pages2 = entry(i + 3);
+    }
+    if (!all) hide(x, key0, has);
+    turn(x, y, i, 0, buf0, 1);
+    spread(next_k, kscale);
+    if (!all) hide(y, key0 + 32, has >> 2);
+    turn(y, x, i, 1, buf1, 0);
+    const uint32_t free = buf0;
+    buf0 = buf1, buf1 = buf2, buf2 = free;
+  }
+
+  // What was taken out comes back to the tokens that see it: an infinity as it is, a NaN as
+  // both (which make a NaN).
+  lds_barrier();
+  if (lane == 0) reinterpret_cast<int*>(kv)[wave] = cleaned ? 1 : 0;
+  lds_barrier();
+  const int4 flags = *reinterpret_cast<const int4*>(kv);
+  if (__builtin_amdgcn_readfirstlane(flags.x | flags.y | flags.z | flags.w) != 0) {
+#pragma unroll 1
+    for (int i = 0; i < count; ++i)
+#pragma unroll 1
+      for (int key = key_of(i); key < min(key_of(i) + KT, end); ++key) {
+        const int page = __builtin_amdgcn_readfirstlane(table[min(key >> a.shift, a.width - 1)]);
+        const uint32_t has = __ballot(is_page(entry(i))) & 15u;
+        if (!is_page(page) || plain(i, has)) continue;
+        const char* const row = a.v + h * a.vh + page * a.vp + (key & ((1 << a.shift) - 1)) * a.vr;
+        const float s = Q8 ? power(a.v_scales[static_cast<int64_t>(page) * a.n_kv + h]) : 1.0f;
+        bool sees[QN];
+#pragma unroll
+        for (int t = 0; t < QN; ++t)
+          sees[t] = key <= pos[t] && (key > pos[t] - a.window || key < a.sinks);
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          us4_t v;
+          if constexpr (Q8) {
+            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(row + 8 * n + 4 * f);
+            const us8_t z = __builtin_bit_cast(us8_t, from_float8<E>(w1, 0, s, s));
+            v = __builtin_shufflevector(z, z, 0, 1, 2, 3);
+          } else {
+            v = *reinterpret_cast<const us4_t*>(row + 16 * n + 8 * f);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float z = (v[e] & E::kExponent) != E::kExponent ? 0.0f
+                            : (v[e] & 0x7fff) != E::kExponent     ? __builtin_nanf("")
+                            : (v[e] >> 15) != 0                   ? -INFINITY : INFINITY;
+#pragma unroll
+            for (int t = 0; t < QN; ++t) acc[t][n / 4][4 * (n % 4) + e] += sees[t] ? z : 0.0f;
+          }
+        }
+      }
+  }
+
+  // A query's sums, and those of its probabilities over both halves of its lanes.
+  const int64_t rec0 = (static_cast<int64_t>(h) * a.shares + w) * rows_all;
+  float* const sums = a.partial + rec0 * D;
+  float* const stats = a.partial + static_cast<int64_t>(a.n_kv) * a.shares * rows_all * D + rec0 * 2;
+#pragma unroll
+  for (int t = 0; t < QN; ++t) {
+    const int r = r0 + (wave * QN + t) * 32 + c;
+    const Pair both = swap_pair<32>(sum[t][0] + sum[t][1]);
+    const bool behind = r >= rows;  // the last token
+    const float l = behind ? 0.0f : both.a + both.b;
+    if (behind) top[t] = -INFINITY;
+    else if (top[t] == -INFINITY && l != 0.0f) top[t] = 0.0f;  // NaN scores alone
+    if (r >= rows_all) continue;
+    if (a.shares == 0) {
+      const int node = r / a.qpk;
+      T* const out = static_cast<T*>(a.out) +
+                     ((static_cast<int64_t>(b) * a.T + node) * a.n_heads + h * a.qpk +
+                      (r - node * a.qpk)) * D + 4 * f;
+      typedef T vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int e = 0; e < D / 8; ++e) {
+        vec4 y;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          y[x] = static_cast<T>(l == 0.0f ? 0.0f : acc[t][e / 4][4 * (e % 4) + x] / l);
+        *reinterpret_cast<vec4*>(out + 8 * e) = y;
+      }
+    } else {
+      if (top[t] != -INFINITY) {
+#pragma unroll
+        for (int e = 0; e < D / 8; ++e) {
+          f4_t y;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) y[x] = acc[t][e / 4][4 * (e % 4) + x];
+          *reinterpret_cast<f4_t*>(sums + static_cast<int64_t>(r) * D + 8 * e + 4 * f) = y;
+        }
+      }
+      if (f == 0) stats[2 * r] = top[t], stats[2 * r + 1] = l;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace nibble
