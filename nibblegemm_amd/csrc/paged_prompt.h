@@ -13,14 +13,6 @@ __device__ __forceinline__ f16_t mfma32(typename E::vec8 a, typename E::vec8 b, 
   if constexpr (std::is_same_v<E, Half>) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
-// c + x[0] + x[1]
-template <class E, class V>
-__device__ __forceinline__ float add_pair(V x, float c) {
-  const typename E::type one = static_cast<typename E::type>(1.0f);
-  if constexpr (std::is_same_v<E, Half>) return __builtin_amdgcn_fdot2(x, V{one, one}, c, false);
-  else return __builtin_amdgcn_fdot2_f32_bf16(x, V{one, one}, c, false);
-}
-
 // Unit (16 bytes) u of LDS row r lies at unit u ^ prompt_swizzle(r), so that eight rows of
 // a K read, and the rows of a V read (four and 32 bytes of each, or, of 8 bits, 4h .. 4h +
 // 3 and 8 + 4h .. and 16 bytes), cover 32 banks once.
@@ -49,7 +41,6 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
   constexpr uint32_t kTile = KT * BYTES;                     // bytes of a tile of k or v
   typedef short s4_t __attribute__((ext_vector_type(4)));
   typedef int i2_t __attribute__((ext_vector_type(2)));
-  typedef T pair_t __attribute__((ext_vector_type(2)));
   typedef unsigned short us4_t __attribute__((ext_vector_type(4)));
   typedef unsigned short us8_t __attribute__((ext_vector_type(8)));
   typedef __attribute__((address_space(3))) s4_t lds4_t;
@@ -129,43 +120,92 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
     }
   }
 
-  // The pages of a tile's four 16-row groups: lane l has that of group l % 4.
+  // Where the tiles' rows are, of 64 tiles, one a lane: the addresses of the 16 rows that
+  // this wave copies, whether all of those are seen by some token, which of a tile's 16-row
+  // groups have a page, and the scales of the groups, a byte each.
   const int32_t* const table = a.table + static_cast<int64_t>(b) * a.width;
-  auto entry = [&](int i) {
-    return table[min((key_of(min(i, count - 1)) + 16 * (lane & 3)) >> a.shift, a.width - 1)];
-  };
   auto is_page = [&](int page) { return page >= 0 && page < a.n_pages; };
-  const uint32_t lds0 = lds_address(kv) + wave * COPIES * 1024u;
-  // This wave's copies of tile i's k (v), whose pages are `pages`; rows that none of the
-  // workgroup's tokens sees read as zeros.
-  auto copy = [&](int i, int pages, const char* base, int64_t page_stride, int64_t row_stride,
-                  uint32_t dst) {
-    const int page = __builtin_amdgcn_readlane(pages, wave);
-    const int key0 = key_of(i) + 16 * wave;
-    const int here = is_page(page) ? end : 0;
-    const char* const from = base + (is_page(page) ? page : 0) * page_stride +
-                             (key0 & ((1 << a.shift) - 1)) * row_stride;
+  auto page_at = [&](int key) { return table[min(key >> a.shift, a.width - 1)]; };
+  struct Places {
+    uint64_t k, v;
+    uint32_t has, k_scales, v_scales;
+  };
+  Places places = {};
+  uint64_t whole = 0;
+  auto look_up = [&](int i) {
+    const int key0 = key_of(min(i + lane, count - 1)), mine = key0 + 16 * wave;
+    const int page = page_at(mine);
+    const uint64_t at = is_page(page) ? page : 0, in_page = mine & ((1 << a.shift) - 1);
+    places.k = reinterpret_cast<uint64_t>(a.k) + h * a.kh + at * a.kp + in_page * a.kr;
+    places.v = reinterpret_cast<uint64_t>(a.v) + h * a.vh + at * a.vp + in_page * a.vr;
+    places.has = places.k_scales = places.v_scales = 0;
 #pragma unroll
-    for (int u = 0; u < COPIES; ++u) {
-      const int r = u * CROWS + lane / UNITS, key = key0 + r;
-      const bool in = key < here && (key >= low || key < a.sinks);
-      const uint32_t unit16 = ((lane % UNITS) ^ prompt_swizzle<UNITS, Q8>(16 * wave + r)) * 16u;
-      lds_copy16(from, 0x7fffffffu, dst + u * 1024u,
-                 in ? r * static_cast<uint32_t>(row_stride) + unit16 : kOutOfRange);
+    for (int n = 0; n < 4; ++n) {
+      const int of = page_at(key0 + 16 * n);
+      places.has |= is_page(of) ? 1u << n : 0u;
+      if constexpr (Q8) {
+        const int64_t s = static_cast<int64_t>(is_page(of) ? of : 0) * a.n_kv + h;
+        places.k_scales |= static_cast<uint32_t>(a.k_scales[s]) << (8 * n);
+        places.v_scales |= static_cast<uint32_t>(a.v_scales[s]) << (8 * n);
+      }
+    }
+    whole = __ballot(is_page(page) && mine + 16 <= end && (mine >= low || mine + 16 <= a.sinks));
+  };
+  // Of one tile, in scalar registers.
+  struct Tile {
+    uint64_t k, v;
+    uint32_t has, k_scales, v_scales;
+    bool whole;
+  };
+  auto tile_of = [&](int i) {
+    auto lane64 = [&](uint64_t x) {
+      const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(x), i & 63);
+      const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(x >> 32), i & 63);
+      return static_cast<uint64_t>(hi) << 32 | lo;
+    };
+    Tile t = {lane64(places.k), lane64(places.v), 0, 0, 0, (whole >> (i & 63) & 1u) != 0};
+    t.has = __builtin_amdgcn_readlane(static_cast<int>(places.has), i & 63);
+    if constexpr (Q8) {
+      t.k_scales = __builtin_amdgcn_readlane(static_cast<int>(places.k_scales), i & 63);
+      t.v_scales = __builtin_amdgcn_readlane(static_cast<int>(places.v_scales), i & 63);
+    }
+    return t;
+  };
+  const uint32_t lds0 = lds_address(kv) + wave * COPIES * 1024u;
+  uint32_t from_k[COPIES], from_v[COPIES];  // a lane's byte in 16 rows of k and v
+#pragma unroll
+  for (int u = 0; u < COPIES; ++u) {
+    const int r = u * CROWS + lane / UNITS;
+    const uint32_t unit16 = ((lane % UNITS) ^ prompt_swizzle<UNITS, Q8>(16 * wave + r)) * 16u;
+    from_k[u] = r * static_cast<uint32_t>(a.kr) + unit16;
+    from_v[u] = r * static_cast<uint32_t>(a.vr) + unit16;
+  }
+  // This wave's copies of tile i's k (v), from `at`; rows that none of the workgroup's
+  // tokens sees read as zeros.
+  auto copy = [&](int i, const Tile& t, uint64_t at, const uint32_t (&from)[COPIES], uint32_t dst) {
+    const void* const base = reinterpret_cast<const void*>(at);
+    if (t.whole) {
+#pragma unroll
+      for (int u = 0; u < COPIES; ++u) lds_copy16(base, 0x7fffffffu, dst + u * 1024u, from[u]);
+    } else {
+      const int key0 = key_of(i) + 16 * wave, here = (t.has >> wave & 1u) != 0 ? end : 0;
+#pragma unroll
+      for (int u = 0; u < COPIES; ++u) {
+        const int key = key0 + u * CROWS + lane / UNITS;
+        const bool in = key < here && (key >= low || key < a.sinks);
+        lds_copy16(base, 0x7fffffffu, dst + u * 1024u, in ? from[u] : kOutOfRange);
+      }
     }
   };
-  auto copy_k = [&](int i, int pages, uint32_t buf) {
-    copy(i, pages, a.k + h * a.kh, a.kp, a.kr, lds0 + buf);
-  };
-  auto copy_v = [&](int i, int pages) {
-    copy(i, pages, a.v + h * a.vh, a.vp, a.vr, lds0 + (i & 1) * kTile);
-  };
+  auto copy_k = [&](int i, const Tile& t, uint32_t buf) { copy(i, t, t.k, from_k, lds0 + buf); };
+  auto copy_v = [&](int i, const Tile& t) { copy(i, t, t.v, from_v, lds0 + (i & 1) * kTile); };
 
   f16_t acc[QN][D / 32];
-  float top[QN], sum[QN][2];  // the reference of query c, in powers of two; of the probabilities
+  float top[QN];   // the reference of query c, in powers of two
+  f16_t sum[QN];   // of the probabilities: sixteen copies
 #pragma unroll
   for (int t = 0; t < QN; ++t) {
-    top[t] = -INFINITY, sum[t][0] = sum[t][1] = 0.0f;
+    top[t] = -INFINITY, sum[t] = f16_t{};
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) acc[t][d] = f16_t{};
   }
@@ -185,6 +225,9 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
            8 * (lane & 1);
   }
   float kscale[4], vscale[4];  // 8 bits: of a tile's 16-row groups
+  vec8 ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = static_cast<T>(1.0f);
   struct Scores {
     f16_t s[QN];  // of 32 keys
   };
@@ -195,33 +238,45 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
   struct Ahead {
     vec8 at[AHEAD];
   };
-  // (j: which 32 keys of the tile at `buf`.  8 bits: two products' elements side by side)
-  auto read_k = [&](Ahead& x, int e, uint32_t buf, int j) {
+  // Places in LDS of its reads, of the tile that is read: the rest of an address is a
+  // constant.
+  constexpr int KA = Q8 ? D / 32 : D / 16, VA = Q8 ? D / 32 : D / 16;
+  uint32_t ka[KA], va[VA];
+#pragma unroll
+  for (int e = 0; e < KA; ++e) ka[e] = lds_address(kv) + 2 * kTile + (krow ^ (32 * e));
+#pragma unroll
+  for (int e = 0; e < VA; ++e)
+    va[e] = lds_address(kv) +
+            (Q8 ? vrow ^ (32 * e) : vrow ^ (64 * (e / 2)) ^ (UNITS > 8 ? 128 * (e % 2) : 0));
+  auto shift_by = [](auto& at, uint32_t by) {
+#pragma unroll
+    for (uint32_t& x : at) x += by;
+  };
+  typedef __attribute__((address_space(3))) const u4_t lds_u4_t;
+  // (j: which 32 keys of the tile.  8 bits: two products' elements side by side)
+  auto read_k = [&](Ahead& x, int e, int j) {
     if constexpr (Q8) {
       if (e % 2 == 1 || e >= N) return;
       const float s = c < 16 ? kscale[2 * j] : kscale[2 * j + 1];
-      const u4_t w4 =
-          *reinterpret_cast<const u4_t*>(kv + buf + j * 32 * BYTES + (krow ^ (32 * (e / 2))));
+      const u4_t w4 = *(lds_u4_t*)(uintptr_t)(ka[e / 2] + j * 32 * BYTES);
       x.at[e % AHEAD] = from_float8<E>(w4[0], w4[1], s, s);
       x.at[e % AHEAD + 1] = from_float8<E>(w4[2], w4[3], s, s);
     } else if (e < N) {
-      x.at[e % AHEAD] =
-          *reinterpret_cast<const vec8*>(kv + buf + j * 32 * BYTES + (krow ^ (32 * e)));
+      x.at[e % AHEAD] = __builtin_bit_cast(vec8, *(lds_u4_t*)(uintptr_t)(ka[e] + j * 32 * BYTES));
     }
   };
   // V^T of the n-th 16 keys for 32 elements.
-  auto values = [&](int buf, int d, int n) {
-    const uint32_t vt = lds_address(kv) + buf * kTile + n * 16 * BYTES;
+  auto values = [&](int d, int n) {
     if constexpr (Q8) {
-      const i2_t v2 = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-          (lds2_t*)(uintptr_t)(vt + (vrow ^ (32 * d))));
+      const i2_t v2 =
+          __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2_t*)(uintptr_t)(va[d] + n * 16 * BYTES));
       return from_float8<E>(v2[0], v2[1], vscale[n], vscale[n]);
     } else {
       s4_t v2[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         v2[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds4_t*)(uintptr_t)(vt + e * 8 * BYTES + (vrow ^ (64 * d) ^ (UNITS > 8 ? 128 * e : 0))));
+            (lds4_t*)(uintptr_t)(va[2 * d + e] + n * 16 * BYTES + e * 8 * BYTES));
       return __builtin_bit_cast(
           vec8, us8_t(__builtin_shufflevector(__builtin_bit_cast(us4_t, v2[0]),
                                               __builtin_bit_cast(us4_t, v2[1]), 0, 1, 2, 3, 4, 5, 6, 7)));
@@ -262,26 +317,27 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
       const float up = fmaxf(fmaxf(both.a, both.b) - kPagedLift<E>, top[t]);
       const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - up);
       top[t] = up;
-      sum[t][0] *= keep, sum[t][1] *= keep;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sum[t][e] *= keep;
 #pragma unroll
       for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[t][d][e] *= keep;
     }
   };
-  // Probabilities and sums of 32 keys (the j-th of tile i), beside the scores of the next
-  // 32 (the next_j-th of the tile at `buf`): a product of the scores, two exponentials, and
+  // Probabilities and sums of the j-th 32 keys of a tile, beside the scores of the next 32
+  // (the next_j-th of theirs): a product of the scores, two exponentials, and
   // so on, then the sums' products.
-  auto turn = [&](const Scores& x, Scores& next, int i, int j, uint32_t buf, int next_j) {
+  auto turn = [&](const Scores& x, Scores& next, int j, int next_j) {
     Ahead k, v;
 #pragma unroll
-    for (int e = 0; e < AHEAD; ++e) read_k(k, e, buf, next_j);
+    for (int e = 0; e < AHEAD; ++e) read_k(k, e, next_j);
     move(x);
     vec8 p[QN][2];
     float base[QN];
 #pragma unroll
     for (int t = 0; t < QN; ++t) base[t] = top[t] == -INFINITY ? 0.0f : top[t];
-    auto read_v = [&](int e) { v.at[e % AHEAD] = values(i & 1, e % (D / 32), 2 * j + e / (D / 32)); };
+    auto read_v = [&](int e) { v.at[e % AHEAD] = values(e % (D / 32), 2 * j + e / (D / 32)); };
     constexpr int PER = 16 / N;  // scores beside a product
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -293,24 +349,24 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
           const int at = e * PER + u;
           p[t][at / 8][at % 8] = static_cast<T>(
               __builtin_amdgcn_exp2f(__builtin_fmaf(x.s[t][at], a.scale, -base[t])));
-          // (The probabilities are rounded to 16 bits because the matrix cores take them so:
-          // each is off by half a step at most, in fp16 of 2^-24 at least, and the sum, in
-          // fp32, is of the rounded.)
-          if (u % 2 == 1)
-            sum[t][u / 2 & 1] = add_pair<E>(
-                pair_t{p[t][at / 8][at % 8 - 1], p[t][at / 8][at % 8]}, sum[t][u / 2 & 1]);
         }
       }
-      read_k(k, e + kFree, buf, next_j);
+      read_k(k, e + kFree, next_j);
       if (e + AHEAD >= N) read_v(e + AHEAD - N);
       __builtin_amdgcn_sched_barrier(0);
     }
+    // (The probabilities are rounded to 16 bits because the matrix cores take them so: each
+    // is off by half a step at most, in fp16 of 2^-24 at least, and the sum, ones times P^T
+    // in fp32, is of the rounded.  v_dot2, which would add pairs, takes the matrix cores'
+    // turns: four beside each product and the two take 1.6 times as long.)
     constexpr int M = D / 16;
 #pragma unroll
     for (int e = 0; e < M; ++e) {
 #pragma unroll
-      for (int t = 0; t < QN; ++t)
+      for (int t = 0; t < QN; ++t) {
+        if (e % (D / 32) == 0) sum[t] = mfma32<E>(ones, p[t][e / (D / 32)], sum[t]);
         acc[t][e % (D / 32)] = mfma32<E>(v.at[e % AHEAD], p[t][e / (D / 32)], acc[t][e % (D / 32)]);
+      }
       if (e + AHEAD < M) read_v(e + AHEAD);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -350,20 +406,10 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
     cleaned |= __any(any) != 0;
   };
 
-  // Pages (and scales) of tiles i (0), i + 1 and i + 2, and which of tile i's groups, and of
-  // the next one's, have a page.
-  int pages1 = 0, pages2 = 0, k1 = 0, v0 = 0, v1 = 0;
-  uint32_t has0 = 0, has1 = 0;
-  auto scales_of = [&](int pages, int* k, int* v) {
-    if constexpr (Q8) {
-      const int64_t at = static_cast<int64_t>(is_page(pages) ? pages : 0) * a.n_kv + h;
-      *k = a.k_scales[at], *v = a.v_scales[at];
-    }
-  };
-  auto spread = [&](int bytes, float (&to)[4]) {
+  auto spread = [&](uint32_t bytes, float (&to)[4]) {
     if constexpr (Q8) {
 #pragma unroll
-      for (int n = 0; n < 4; ++n) to[n] = power(__builtin_amdgcn_readlane(bytes, n));
+      for (int n = 0; n < 4; ++n) to[n] = power(bytes >> (8 * n) & 255);
     }
   };
   // Every query sees all of a tile's keys.
@@ -374,60 +420,53 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
   };
   Scores x, y;
   uint32_t buf0 = 2 * kTile, buf1 = 3 * kTile, buf2 = 4 * kTile;  // of k of tiles i, i + 1, i + 2
+  Tile now = {}, next = {};  // tiles i and i + 1
   if (count > 0) {
-    pages1 = entry(0);
-    pages2 = entry(1);
-    int k0 = 0;
-    scales_of(pages1, &k0, &v0);
-    scales_of(pages2, &k1, &v1);
-    has0 = __ballot(is_page(pages1)) & 15u;
-    has1 = __ballot(is_page(pages2)) & 15u;
-    copy_k(0, pages1, buf0);
-    copy_v(0, pages1);
-    if (count > 1) copy_k(1, pages2, buf1);
-    pages1 = pages2;
-    pages2 = entry(2);
+    look_up(0);
+    now = tile_of(0), next = tile_of(1);
+    copy_k(0, now, buf0);
+    copy_v(0, now);
+    if (count > 1) copy_k(1, next, buf1);
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
     lds_barrier();
-    spread(k0, kscale);
+    spread(now.k_scales, kscale);
     Ahead k;
 #pragma unroll
-    for (int e = 0; e < AHEAD; ++e) read_k(k, e, buf0, 0);
+    for (int e = 0; e < AHEAD; ++e) read_k(k, e, 0);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
 #pragma unroll
       for (int t = 0; t < QN; ++t)
         x.s[t] = mfma32<E>(k.at[e % AHEAD], q[t][e], e == 0 ? f16_t{} : x.s[t]);
-      read_k(k, e + kFree, buf0, 0);
+      read_k(k, e + kFree, 0);
     }
   }
 #pragma unroll 1
   for (int i = 0; i < count; ++i) {
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // v of tile i and k of tile i + 1 are there
     lds_barrier();
-    const uint32_t has = has0;
+    const uint32_t has = now.has;
     const int key0 = key_of(i);
     const bool all = plain(i, has);
-    spread(v0, vscale);
+    spread(now.v_scales, vscale);
     if (!all) {
       clean(i & 1);
       lds_barrier();
     }
-    const int next_k = k1;
-    v0 = v1, has0 = has1;
-    if (i + 1 < count) copy_v(i + 1, pages1);
+    if (i + 1 < count) copy_v(i + 1, next);
+    now = next;
     if (i + 2 < count) {
-      copy_k(i + 2, pages2, buf2);
-      scales_of(pages2, &k1, &v1);
-      has1 = __ballot(is_page(pages2)) & 15u;
-      pages1 = pages2;
-      pages2 = entry(i + 3);
+      if (((i + 2) & 63) == 0) look_up(i + 2);
+      next = tile_of(i + 2);
+      copy_k(i + 2, next, buf2);
     }
     if (!all) hide(x, key0, has);
-    turn(x, y, i, 0, buf0, 1);
-    spread(next_k, kscale);
+    turn(x, y, 0, 1);
+    spread(now.k_scales, kscale);
+    shift_by(ka, buf1 - buf0);
     if (!all) hide(y, key0 + 32, has >> 2);
-    turn(y, x, i, 1, buf1, 0);
+    turn(y, x, 1, 0);
+    shift_by(va, i % 2 == 0 ? kTile : 0u - kTile);
     const uint32_t free = buf0;
     buf0 = buf1, buf1 = buf2, buf2 = free;
   }
@@ -443,8 +482,8 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
     for (int i = 0; i < count; ++i)
 #pragma unroll 1
       for (int key = key_of(i); key < min(key_of(i) + KT, end); ++key) {
-        const int page = __builtin_amdgcn_readfirstlane(table[min(key >> a.shift, a.width - 1)]);
-        const uint32_t has = __ballot(is_page(entry(i))) & 15u;
+        const int page = __builtin_amdgcn_readfirstlane(page_at(key));
+        const uint32_t has = __ballot(is_page(page_at(key_of(i) + 16 * (lane & 3)))) & 15u;
         if (!is_page(page) || plain(i, has)) continue;
         const char* const row = a.v + h * a.vh + page * a.vp + (key & ((1 << a.shift) - 1)) * a.vr;
         const float s = Q8 ? power(a.v_scales[static_cast<int64_t>(page) * a.n_kv + h]) : 1.0f;
@@ -474,16 +513,14 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
       }
   }
 
-  // A query's sums, and those of its probabilities over both halves of its lanes.
   const int64_t rec0 = (static_cast<int64_t>(h) * a.shares + w) * rows_all;
   float* const sums = a.partial + rec0 * D;
   float* const stats = a.partial + static_cast<int64_t>(a.n_kv) * a.shares * rows_all * D + rec0 * 2;
 #pragma unroll
   for (int t = 0; t < QN; ++t) {
     const int r = r0 + (wave * QN + t) * 32 + c;
-    const Pair both = swap_pair<32>(sum[t][0] + sum[t][1]);
     const bool behind = r >= rows;  // the last token
-    const float l = behind ? 0.0f : both.a + both.b;
+    const float l = behind ? 0.0f : sum[t][0];
     if (behind) top[t] = -INFINITY;
     else if (top[t] == -INFINITY && l != 0.0f) top[t] = 0.0f;  // NaN scores alone
     if (r >= rows_all) continue;
