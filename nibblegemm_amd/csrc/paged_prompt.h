@@ -299,21 +299,23 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
           if ((seen >> e & 1u) == 0) x.s[t][4 * u + e] = -INFINITY;
       }
   };
-  auto move = [&](const Scores& x) {
-    float m[QN];
-    bool moves = false;
+  float m[QN];  // the largest of a lane's scores of the next 32 keys, not scaled
+  auto largest = [&](const Scores& x) {
 #pragma unroll
     for (int t = 0; t < QN; ++t) {
       m[t] = x.s[t][0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) m[t] = fmaxf(m[t], x.s[t][e]);
-      m[t] *= a.scale;
-      moves |= m[t] - top[t] > kPagedSlack + kPagedLift<E>;
     }
+  };
+  auto move = [&]() {
+    bool moves = false;
+#pragma unroll
+    for (int t = 0; t < QN; ++t) moves |= m[t] * a.scale - top[t] > kPagedSlack + kPagedLift<E>;
     if (!__any(moves)) return;
 #pragma unroll
     for (int t = 0; t < QN; ++t) {
-      const Pair both = swap_pair<32>(m[t]);
+      const Pair both = swap_pair<32>(m[t] * a.scale);
       const float up = fmaxf(fmaxf(both.a, both.b) - kPagedLift<E>, top[t]);
       const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - up);
       top[t] = up;
@@ -325,14 +327,15 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
         for (int e = 0; e < 16; ++e) acc[t][d][e] *= keep;
     }
   };
-  // Probabilities and sums of the j-th 32 keys of a tile, beside the scores of the next 32
-  // (the next_j-th of theirs): a product of the scores, two exponentials, and
-  // so on, then the sums' products.
-  auto turn = [&](const Scores& x, Scores& next, int j, int next_j) {
-    Ahead k, v;
-#pragma unroll
-    for (int e = 0; e < AHEAD; ++e) read_k(k, e, next_j);
-    move(x);
+  // Probabilities and sums of the j-th 32 keys of a tile, whose scores are x, beside the
+  // scores of the next 32 (the next_j-th of theirs): a product of the scores, two
+  // exponentials, and so on, then the sums' products, beside them the next scores' maximum
+  // and the first operands of the products after them (the after_j-th 32 keys where
+  // `between` has left ka).
+  Ahead k;
+  auto turn = [&](const Scores& x, Scores& next, int j, int next_j, int after_j, auto between) {
+    Ahead v;
+    move();
     vec8 p[QN][2];
     float base[QN];
 #pragma unroll
@@ -355,6 +358,7 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
       if (e + AHEAD >= N) read_v(e + AHEAD - N);
       __builtin_amdgcn_sched_barrier(0);
     }
+    between();
     // (The probabilities are rounded to 16 bits because the matrix cores take them so: each
     // is off by half a step at most, in fp16 of 2^-24 at least, and the sum, ones times P^T
     // in fp32, is of the rounded.  v_dot2, which would add pairs, takes the matrix cores'
@@ -368,7 +372,9 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
         acc[t][e % (D / 32)] = mfma32<E>(v.at[e % AHEAD], p[t][e / (D / 32)], acc[t][e % (D / 32)]);
       }
       if (e + AHEAD < M) read_v(e + AHEAD);
-      __builtin_amdgcn_sched_barrier(0);
+      if (e + AHEAD >= M) read_k(k, e + AHEAD - M, after_j);
+      if (e == M / 2) largest(next);
+      if (e < M / 2 || e == M - 1) __builtin_amdgcn_sched_barrier(0);
     }
   };
   // Takes what is not finite out of this wave's 16 rows of a tile's v, for a hidden row's
@@ -430,7 +436,6 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
     __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
     lds_barrier();
     spread(now.k_scales, kscale);
-    Ahead k;
 #pragma unroll
     for (int e = 0; e < AHEAD; ++e) read_k(k, e, 0);
 #pragma unroll
@@ -440,6 +445,9 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
         x.s[t] = mfma32<E>(k.at[e % AHEAD], q[t][e], e == 0 ? f16_t{} : x.s[t]);
       read_k(k, e + kFree, 0);
     }
+    largest(x);
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) read_k(k, e, 1);
   }
 #pragma unroll 1
   for (int i = 0; i < count; ++i) {
@@ -460,12 +468,13 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
       next = tile_of(i + 2);
       copy_k(i + 2, next, buf2);
     }
-    if (!all) hide(x, key0, has);
-    turn(x, y, 0, 1);
-    spread(now.k_scales, kscale);
-    shift_by(ka, buf1 - buf0);
-    if (!all) hide(y, key0 + 32, has >> 2);
-    turn(y, x, 1, 0);
+    if (!all) hide(x, key0, has), largest(x);
+    turn(x, y, 0, 1, 0, [&]() {
+      spread(now.k_scales, kscale);
+      shift_by(ka, buf1 - buf0);
+    });
+    if (!all) hide(y, key0 + 32, has >> 2), largest(y);
+    turn(y, x, 1, 0, 1, []() {});
     shift_by(va, i % 2 == 0 ? kTile : 0u - kTile);
     const uint32_t free = buf0;
     buf0 = buf1, buf1 = buf2, buf2 = free;
