@@ -43,9 +43,10 @@ struct PagedArgs {
   const float* sin;
   void* q_out;  // [B, T, n_heads, D]
   int64_t kp, kh, kr, vp, vh, vr;  // in bytes
-  int64_t heads;                   // those that a lane group has each: B T (n_heads [+ 2 n_kv])
-  int B, T, n_heads, n_kv, width, n_pages, shift, rope_rows, R;
-  int tasks, spans;  // 8-bit: (sequence, page, head, k or v)s, pages a sequence's tokens may reach
+  uint32_t heads;                  // those that a lane group has each: B T (n_heads [+ 2 n_kv])
+  uint32_t T;
+  int B, n_heads, n_kv, width, n_pages, shift, rope_rows, R;
+  uint32_t tasks, spans;  // 8-bit: (sequence, page, head, k or v)s, pages that a run of tokens may reach
   unsigned head_blocks;
   float eps;
   bool interleaved;
@@ -57,7 +58,8 @@ struct Rows {
   __device__ __forceinline__ Rows(const PagedArgs& a, int b) {
     const int room = a.width << a.shift;
     len = min(max(a.lengths[b], 0), room);
-    live = min(a.sizes != nullptr ? min(max(a.sizes[b], 0), a.T) : a.T, room - len);
+    const int T = static_cast<int>(a.T);
+    live = min(a.sizes != nullptr ? min(max(a.sizes[b], 0), T) : T, room - len);
   }
 };
 
@@ -141,17 +143,17 @@ __device__ __forceinline__ void append_heads(const PagedArgs& a) {
   using vec8 = typename E::vec8;
   constexpr int LANES = D / 16;
   const int j = threadIdx.x % LANES;
-  const int64_t x = static_cast<int64_t>(blockIdx.x) * (kPagedThreads / LANES) + threadIdx.x / LANES;
+  const uint32_t x = blockIdx.x * (kPagedThreads / LANES) + threadIdx.x / LANES;
   // (heads behind the last take part in the reductions, as copies of it)
-  const int64_t at = x < a.heads ? x : a.heads - 1;
-  const int all = a.n_heads + 2 * a.n_kv, some = Q8 ? a.n_heads : all;
-  const int64_t token = at / some;
+  const uint32_t at = min(x, a.heads - 1);
+  const uint32_t all = a.n_heads + 2 * a.n_kv, some = Q8 ? a.n_heads : all;
+  const uint32_t token = at / some, in_batch = token / a.T;
   const int head = static_cast<int>(at - token * some);
-  const int b = static_cast<int>(token / a.T), t = static_cast<int>(token - static_cast<int64_t>(b) * a.T);
+  const int b = static_cast<int>(in_batch), t = static_cast<int>(token - in_batch * a.T);
   const Runs runs(a, j);
-  const T* from = static_cast<const T*>(a.qkv) + (token * all + head) * D;
-  vec8 lo = *reinterpret_cast<const vec8*>(from + runs.lo);
-  vec8 hi = *reinterpret_cast<const vec8*>(from + runs.hi);
+  const T* from = static_cast<const T*>(a.qkv) + (static_cast<int64_t>(token) * all + head) * D;
+  vec8 lo = __builtin_nontemporal_load(reinterpret_cast<const vec8*>(from + runs.lo));
+  vec8 hi = __builtin_nontemporal_load(reinterpret_cast<const vec8*>(from + runs.hi));
   const Rows rows(a, b);
   const int row = rows.len + t, pos = position(a, b, t, row);
   const int page = t < rows.live ? page_of(a.table, b, a.width, a.n_pages, row >> a.shift) : -1;
@@ -171,7 +173,7 @@ __device__ __forceinline__ void append_heads(const PagedArgs& a) {
   if (x >= a.heads || !(query || live)) return;
   T* o;
   if (query) {
-    o = static_cast<T*>(a.q_out) + (token * a.n_heads + head) * D;
+    o = static_cast<T*>(a.q_out) + (static_cast<int64_t>(token) * a.n_heads + head) * D;
   } else {
     const int h = head - a.n_heads - (value ? a.n_kv : 0), r = row & ((1 << a.shift) - 1);
     o = reinterpret_cast<T*>(value ? a.v + page * a.vp + h * a.vh + r * a.vr
@@ -181,89 +183,88 @@ __device__ __forceinline__ void append_heads(const PagedArgs& a) {
   *reinterpret_cast<vec8*>(o + runs.hi) = hi;
 }
 
-// The new rows of one page, one head, keys or values, by one wave (pages of 64 rows
-// and fewer) or four.  Every lane group holds its rows' values from the first look, for
-// the largest magnitude, to their rounding.
+// The new rows of one page, one head, keys or values: a task of one wave, two or four, by
+// the page's size.  A lane holds its rows' values from the first look, for the largest
+// magnitude, to their rounding.  (4 x 2000 tokens of 32 + 2 x 8 heads of 128 on pages of 64
+// @@; a wave a page, its values worked out twice, 71 us.)
 template <class E, int D, int P>
 __device__ __forceinline__ void append_page(const PagedArgs& a) {
   using T = typename E::type;
   using vec8 = typename E::vec8;
   constexpr int LANES = D / 16;
-  constexpr int WAVES = P > 64 ? 4 : 1, STEP = WAVES * 64 / LANES;  // rows at once
+  constexpr int WAVES = P * LANES <= 128 ? 1 : P * LANES <= 256 ? 2 : 4;
+  constexpr int STEP = WAVES * 64 / LANES;  // rows at once
   constexpr int N = P > STEP ? P / STEP : 1;
-  const int me = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;  // within the task
-  const int64_t task = (static_cast<int64_t>(blockIdx.x) - a.head_blocks) * (4 / WAVES) +
-                       (WAVES == 1 ? threadIdx.x >> 6 : 0);
+  const int me = threadIdx.x % (WAVES * 64);  // within the task
+  const uint32_t task = (blockIdx.x - a.head_blocks) * (4 / WAVES) + threadIdx.x / (WAVES * 64);
   __shared__ float part[4];
-  if (task >= a.tasks) return;  // (a wave's, or a workgroup's)
-  const int which = static_cast<int>(task & 1);
-  const int h = static_cast<int>((task >> 1) % a.n_kv);
-  const int64_t rest = (task >> 1) / a.n_kv;
-  const int b = static_cast<int>(rest / a.spans), m = static_cast<int>(rest - static_cast<int64_t>(b) * a.spans);
-  const Rows rows(a, b);
-  const int index = (rows.len >> a.shift) + m, first = index * P;  // the page's first row
-  const int begin = max(rows.len, first), end = min(rows.len + rows.live, first + P);
-  if (begin >= end) return;
-  const int page = page_of(a.table, b, a.width, a.n_pages, index);
-  if (page < 0) return;
-
+  const uint32_t rest = (task >> 1) / a.n_kv, in_batch = rest / a.spans;
+  const int which = static_cast<int>(task & 1), h = static_cast<int>((task >> 1) - rest * a.n_kv);
+  const int b = static_cast<int>(in_batch), m = static_cast<int>(rest - in_batch * a.spans);
+  int len = 0, index = 0, first = 0, begin = 0, end = 0, page = -1;
+  if (task < a.tasks) {
+    const Rows rows(a, b);
+    len = rows.len, index = (len >> a.shift) + m, first = index * P;  // the page's first row
+    begin = max(len, first), end = min(len + rows.live, first + P);
+    if (begin < end) page = page_of(a.table, b, a.width, a.n_pages, index);
+  }
   const int j = me % LANES, r0 = me / LANES;
   Runs runs(a, j);
   if (which != 0) runs.turns = false, runs.lo = 16 * j, runs.hi = 16 * j + 8;
   const int all = a.n_heads + 2 * a.n_kv;
-  const T* const from = static_cast<const T*>(a.qkv) +
-                        (static_cast<int64_t>(b) * a.T * all + a.n_heads + which * a.n_kv + h) * D;
-  vec8 raw[N][2];
-  int pos[N];
+  float f[N][8], g[N][8], top = -1.0f;  // below zero: no row
+  bool live[N];  // a row with a place, whose position the tables have
+  uint8_t* scale = nullptr;
+  int was = 0;
+  if (page >= 0) {
+    const T* const from = static_cast<const T*>(a.qkv) +
+                          (static_cast<int64_t>(b) * a.T * all + a.n_heads + which * a.n_kv + h) * D;
+    scale = (which != 0 ? a.v_scales : a.k_scales) + static_cast<int64_t>(page) * a.n_kv + h;
+    was = *scale;
+    int pos[N];
+    vec8 raw[N][2];
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int row = first + r0 + n * STEP, t = row - rows.len;
-    const bool in = row >= begin && row < end;
-    pos[n] = in ? position(a, b, t, row) : -1;
-    const T* x = from + static_cast<int64_t>(in ? t : begin - rows.len) * all * D;
-    raw[n][0] = *reinterpret_cast<const vec8*>(x + runs.lo);
-    raw[n][1] = *reinterpret_cast<const vec8*>(x + runs.hi);
-    if (a.cos == nullptr && in) pos[n] = 0;
-  }
-  auto values = [&](int n, float (&f)[8], float (&g)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      f[i] = static_cast<float>(raw[n][0][i]), g[i] = static_cast<float>(raw[n][1][i]);
-    if (which == 0) turn<E, D>(a, a.k_weight, runs, j, pos[n], f, g);
-  };
-  // (a token's own position names it live: a row's place, and the tables have it)
-  float top = 0.0f;
-  bool any = false;
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    float f[8], g[8];
-    values(n, f, g);
-    if (pos[n] < 0) continue;
-    any = true;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      // (an infinity or a NaN has no part in the scale)
-      const float x = fabsf(f[i]), y = fabsf(g[i]);
-      top = fmaxf(top, x < INFINITY ? fminf(x, kLargest<E>) : 0.0f);
-      top = fmaxf(top, y < INFINITY ? fminf(y, kLargest<E>) : 0.0f);
+    for (int n = 0; n < N; ++n) {
+      const int row = first + r0 + n * STEP;
+      const bool in = row >= begin && row < end;
+      pos[n] = in ? position(a, b, row - len, row) : -1;
+      live[n] = in && (a.cos == nullptr || pos[n] >= 0);
+      const T* x = from + static_cast<int64_t>((in ? row : begin) - len) * all * D;
+      raw[n][0] = __builtin_nontemporal_load(reinterpret_cast<const vec8*>(x + runs.lo));
+      raw[n][1] = __builtin_nontemporal_load(reinterpret_cast<const vec8*>(x + runs.hi));
     }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        f[n][i] = static_cast<float>(raw[n][0][i]), g[n][i] = static_cast<float>(raw[n][1][i]);
+      if (which == 0) turn<E, D>(a, a.k_weight, runs, j, pos[n], f[n], g[n]);
+      if (!live[n]) continue;
+      top = fmaxf(top, 0.0f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        // (an infinity or a NaN has no part in the scale)
+        const float x = fabsf(f[n][i]), y = fabsf(g[n][i]);
+        top = fmaxf(top, x < INFINITY ? fminf(x, kLargest<E>) : 0.0f);
+        top = fmaxf(top, y < INFINITY ? fminf(y, kLargest<E>) : 0.0f);
+      }
+    }
+    top = wave_max(top);
   }
-  top = wave_max(any ? top : -1.0f);  // below zero: no row
-  if (WAVES > 1) {
+  if (WAVES > 1) {  // (every wave has read the scale, too)
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    const int wave0 = threadIdx.x / (WAVES * 64) * WAVES;
+#pragma unroll
+    for (int x = 0; x < WAVES; ++x) top = fmaxf(top, part[wave0 + x]);
   }
   if (top < 0.0f) return;
 
-  uint8_t* const scale = (which != 0 ? a.v_scales : a.k_scales) +
-                         static_cast<int64_t>(page) * a.n_kv + h;
   char* const base = which != 0 ? a.v + page * a.vp + h * a.vh : a.k + page * a.kp + h * a.kh;
   const int64_t stride = which != 0 ? a.vr : a.kr;
-  const int was = *scale, need = exponent_for<E>(top);
+  const int need = exponent_for<E>(top);
   const bool fresh = begin == first;
-  const int e = fresh ? need : max(need, was);
-  if (WAVES > 1) __syncthreads();  // every wave has read the scale
+  const int e = fresh ? need : min(max(need, was), 254);
   if (!fresh && e != was) {  // earlier rows, on the new power of two
     const float by = power(max(127 + was - e, 1));
 #pragma unroll 1
@@ -280,25 +281,25 @@ __device__ __forceinline__ void append_page(const PagedArgs& a) {
     }
   }
   if (me == 0 && e != was) *scale = static_cast<uint8_t>(e);
-  const float inverse = power(254 - e), most = e == kHighExponent<E> ? kFloat8LastMax : kFloat8Max;
+  const float inverse = power(254 - e), most = e >= kHighExponent<E> ? kFloat8LastMax : kFloat8Max;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    float f[8], g[8];
-    values(n, f, g);
-    if (pos[n] < 0) continue;
+    if (!live[n]) continue;
     auto code = [&](float x) {
       const float y = x * inverse;
-      // (a comparison with an infinity or a NaN keeps them: they become NaN)
+      // (an infinity or a NaN becomes NaN)
       return fabsf(x) < INFINITY ? fminf(fmaxf(y, -most), most) : __builtin_nanf("");
     };
     char* const o = base + (r0 + n * STEP) * stride;
-    const uint32_t lo[2] = {to_float8(code(f[0]), code(f[1]), code(f[2]), code(f[3])),
-                            to_float8(code(f[4]), code(f[5]), code(f[6]), code(f[7]))};
-    const uint32_t hi[2] = {to_float8(code(g[0]), code(g[1]), code(g[2]), code(g[3])),
-                            to_float8(code(g[4]), code(g[5]), code(g[6]), code(g[7]))};
     typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
-    *reinterpret_cast<u2_t*>(o + runs.lo) = u2_t{lo[0], lo[1]};
-    *reinterpret_cast<u2_t*>(o + runs.hi) = u2_t{hi[0], hi[1]};
+    const float(&x)[8] = f[n];
+    const float(&y)[8] = g[n];
+    *reinterpret_cast<u2_t*>(o + runs.lo) =
+        u2_t{to_float8(code(x[0]), code(x[1]), code(x[2]), code(x[3])),
+             to_float8(code(x[4]), code(x[5]), code(x[6]), code(x[7]))};
+    *reinterpret_cast<u2_t*>(o + runs.hi) =
+        u2_t{to_float8(code(y[0]), code(y[1]), code(y[2]), code(y[3])),
+             to_float8(code(y[4]), code(y[5]), code(y[6]), code(y[7]))};
   }
 }
 
@@ -333,8 +334,9 @@ struct ValuesArgs {
   void* k_out;  // [B, n_kv, rows, D]
   void* v_out;
   int64_t kp, kh, kr, vp, vh, vr;  // in bytes
-  int64_t units;                   // B n_kv rows D / 16, of keys (and as many of values)
-  int n_kv, rows, width, n_pages, shift;
+  uint32_t units;                  // B n_kv rows D / 16, of keys (and as many of values)
+  uint32_t n_kv, rows;
+  int width, n_pages, shift;
 };
 
 // Sixteen values a thread, keys and values side by side.
@@ -342,13 +344,11 @@ template <class E, int D, bool Q8>
 __global__ __launch_bounds__(kPagedThreads) void values_kernel(ValuesArgs a) {
   using vec8 = typename E::vec8;
   constexpr int UNITS = D / 16;
-  const int64_t unit = static_cast<int64_t>(blockIdx.x) * kPagedThreads + threadIdx.x;
+  const uint32_t unit = blockIdx.x * kPagedThreads + threadIdx.x;
   if (unit >= a.units) return;
-  const int64_t at = unit / UNITS;
-  const int u = static_cast<int>(unit - at * UNITS);
-  const int64_t pair = at / a.rows;
-  const int row = static_cast<int>(at - pair * a.rows);
-  const int b = static_cast<int>(pair / a.n_kv), h = static_cast<int>(pair - static_cast<int64_t>(b) * a.n_kv);
+  const uint32_t at = unit / UNITS, pair = at / a.rows, in_batch = pair / a.n_kv;
+  const int u = static_cast<int>(unit % UNITS), row = static_cast<int>(at - pair * a.rows);
+  const int b = static_cast<int>(in_batch), h = static_cast<int>(pair - in_batch * a.n_kv);
   const int m = row >> a.shift, r = row & ((1 << a.shift) - 1);
   const int page = row < a.lengths[b] && m < a.width ? page_of(a.table, b, a.width, a.n_pages, m) : -1;
   vec8 y[2][2] = {};
@@ -376,7 +376,7 @@ __global__ __launch_bounds__(kPagedThreads) void values_kernel(ValuesArgs a) {
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      static_cast<vec8*>(i == 0 ? a.k_out : a.v_out)[2 * unit + e] = y[i][e];
+      static_cast<vec8*>(i == 0 ? a.k_out : a.v_out)[2 * static_cast<int64_t>(unit) + e] = y[i][e];
 }
 
 template <class E>
@@ -469,13 +469,14 @@ extern "C" int nibble_paged_append(const void* QKV, int64_t dtype, int64_t batch
   const bool q8 = c.k_scales != nullptr;
   const int64_t bytes = q8 ? 1 : 2, P = c.page_rows;
   PagedArgs a;
-  a.heads = batch * tokens * (n_heads + (q8 ? 0 : 2 * c.n_kv_heads));
-  const int64_t head_blocks = ceil_div(a.heads, kPagedThreads / (c.head_dim / 16));
+  const int64_t heads = batch * tokens * (n_heads + (q8 ? 0 : 2 * c.n_kv_heads));
+  const int64_t head_blocks = ceil_div(heads, kPagedThreads / (c.head_dim / 16));
   // pages that a run of tokens reaches, wherever it begins
   const int64_t spans = (tokens + P - 2) / P + 1;
   const int64_t tasks = q8 ? batch * spans * c.n_kv_heads * 2 : 0;
-  const int64_t blocks = head_blocks + ceil_div(tasks, P > 64 ? 1 : 4);
-  // (a launch ends at 2^32 threads)
+  const int64_t lanes = P * (c.head_dim / 16);  // of a task: a wave, two or four
+  const int64_t blocks = head_blocks + ceil_div(tasks, lanes <= 128 ? 4 : lanes <= 256 ? 2 : 1);
+  // (a launch ends at 2^32 threads; heads and tasks are fewer)
   NIBBLE_CHECK(blocks < (int64_t(1) << 32) / kPagedThreads, "too many tokens: %lld x %lld",
                (long long)batch, (long long)tokens);
   hipStream_t stream = static_cast<hipStream_t>(stream_);
@@ -499,7 +500,8 @@ extern "C" int nibble_paged_append(const void* QKV, int64_t dtype, int64_t batch
   a.kp = c.k_page_stride * bytes, a.kh = c.k_head_stride * bytes, a.kr = c.k_row_stride * bytes;
   a.vp = c.v_page_stride * bytes, a.vh = c.v_head_stride * bytes, a.vr = c.v_row_stride * bytes;
   a.B = static_cast<int>(batch);
-  a.T = static_cast<int>(tokens);
+  a.heads = static_cast<uint32_t>(heads);
+  a.T = static_cast<uint32_t>(tokens);
   a.n_heads = static_cast<int>(n_heads);
   a.n_kv = static_cast<int>(c.n_kv_heads);
   a.width = static_cast<int>(c.table_pages);
@@ -507,8 +509,8 @@ extern "C" int nibble_paged_append(const void* QKV, int64_t dtype, int64_t batch
   a.shift = P == 16 ? 4 : P == 32 ? 5 : P == 64 ? 6 : P == 128 ? 7 : 8;
   a.rope_rows = rope_cos != nullptr ? static_cast<int>(rope_rows) : 0;
   a.R = rope_cos != nullptr ? static_cast<int>(rope_dim) : 0;
-  a.tasks = static_cast<int>(tasks);
-  a.spans = static_cast<int>(spans);
+  a.tasks = static_cast<uint32_t>(tasks);
+  a.spans = static_cast<uint32_t>(spans);
   a.head_blocks = static_cast<unsigned>(head_blocks);
   a.eps = eps;
   a.interleaved = interleaved != 0;
@@ -534,8 +536,8 @@ extern "C" int nibble_paged_values(const nibble_paged_cache* cache, int64_t dtyp
   NIBBLE_CHECK(aligned(K_out, 16) && aligned(V_out, 16), "outputs must be 16-byte aligned");
   NIBBLE_CHECK(aligned(lengths, 4), "lengths must be 4-byte aligned");
   ValuesArgs a;
-  a.units = batch * c.n_kv_heads * rows * (c.head_dim / 16);
-  NIBBLE_CHECK(a.units < (int64_t(1) << 32) - kPagedThreads, "too many rows: %lld x %lld x %lld",
+  const int64_t units = batch * c.n_kv_heads * rows * (c.head_dim / 16);
+  NIBBLE_CHECK(units < (int64_t(1) << 32) - kPagedThreads, "too many rows: %lld x %lld x %lld",
                (long long)batch, (long long)c.n_kv_heads, (long long)rows);
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   DeviceGuard guard;
@@ -552,8 +554,9 @@ extern "C" int nibble_paged_values(const nibble_paged_cache* cache, int64_t dtyp
   a.v_out = V_out;
   a.kp = c.k_page_stride * bytes, a.kh = c.k_head_stride * bytes, a.kr = c.k_row_stride * bytes;
   a.vp = c.v_page_stride * bytes, a.vh = c.v_head_stride * bytes, a.vr = c.v_row_stride * bytes;
-  a.n_kv = static_cast<int>(c.n_kv_heads);
-  a.rows = static_cast<int>(rows);
+  a.units = static_cast<uint32_t>(units);
+  a.n_kv = static_cast<uint32_t>(c.n_kv_heads);
+  a.rows = static_cast<uint32_t>(rows);
   a.width = static_cast<int>(c.table_pages);
   a.n_pages = static_cast<int>(c.n_pages);
   a.shift = P == 16 ? 4 : P == 32 ? 5 : P == 64 ? 6 : P == 128 ? 7 : 8;
