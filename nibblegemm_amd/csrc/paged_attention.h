@@ -14,6 +14,9 @@ namespace {
 
 constexpr int kPagedThreads = 256;
 constexpr int kPagedKeys = 64;  // keys of a tile
+// What the sums of a share cost that are written and joined, in tiles: of a call, and of
+// its query rows.  (2 x 12 tokens of 32 + 2 x 4 heads over 20000 rows of 8 bits: 37 us, 35
+// if it costs nothing, 54 if four times that; 4 x 60 of 8 + 2 x 8 over 2000: 20, 24, 25.)
 constexpr float kPagedShareCost = 0.08f, kPagedRowCost = 4.8e-4f;
 // Probabilities are relative to a query's reference, 2^lift below a maximum, which
 // moves only when a score passes that maximum by more than the slack (in powers of two).
@@ -91,15 +94,11 @@ __device__ __forceinline__ int AttendArgs::tiles(int b) const {
   return s.first + s.upto - s.from;
 }
 
-// Unit (16 bytes) u of LDS row r lies at unit u ^ paged_swizzle(r): the reads below
-// cover 32 banks once.  16-bit rows: eight rows of a K read, four rows' 32-byte pieces
-// of a V read.  8-bit rows: eight rows of a K read, the units of rows 4g .. 4g + 3 of two
-// 16-row tiles of a V read.
-template <int UNITS, bool Q8>
+// Unit (16 bytes) u of LDS row r, 16-bit values, lies at unit u ^ paged_swizzle(r): eight
+// rows of a K read, and four rows' 32-byte pieces of a V read, cover 32 banks once.
+template <int UNITS>
 __device__ __forceinline__ int paged_swizzle(int r) {
-  if (!Q8) return ((r & 3) << 1 | (r >> 2 & 1) | (r & 8)) & (UNITS - 1);
-  const int high = (r >> 2 ^ r >> 4) & 1;
-  return UNITS == 8 ? (r & 3) | high << 2 : (r >> 1 & 1) | high << 1;
+  return ((r & 3) << 1 | (r >> 2 & 1) | (r & 8)) & (UNITS - 1);
 }
 
 }  // namespace

@@ -18,12 +18,12 @@ __device__ __forceinline__ f16_t mfma32(typename E::vec8 a, typename E::vec8 b, 
 // 3 and 8 + 4h .. and 16 bytes), cover 32 banks once.
 template <int UNITS, bool Q8>
 __device__ __forceinline__ int prompt_swizzle(int r) {
-  if (!Q8) return paged_swizzle<UNITS, false>(r);
+  if (!Q8) return paged_swizzle<UNITS>(r);
   const int high = (r >> 2 ^ r >> 3) & 1;
   return UNITS == 8 ? (r & 3) | high << 2 : (r >> 1 & 1) | high << 1;
 }
 
-// One workgroup: 128 QN query rows of one kv head, 32 QN a wave, and one share of the rows, in
+// One workgroup: 128 query rows of one kv head, 32 a wave, and one share of the rows, in
 // tiles of 64 keys, which are copied straight into LDS, v into one of two buffers while the
 // tile before is computed, k, a tile ahead of it, into one of three.
 //
@@ -31,11 +31,19 @@ __device__ __forceinline__ int prompt_swizzle(int r) {
 // % 32) gets the scores of query c for keys 8 a + 4 f .. + 3 (a = 0 .. 3) of a 32-key tile,
 // and its probabilities are where the second product (V^T P^T) wants them, if its k runs
 // over a lane's keys in turn.
-template <class E, int D, int QN, bool Q8>
-__global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(AttendArgs a) {
+//
+// The matrix cores bound it, and their power: of 2048 tokens of 32 + 2 x 8 heads of 128
+// the products alone would take 86 us at the rate of a large library product, and it takes
+// 113 to 130, by the card's clock, which falls to 1.9 GHz meanwhile.  What fills the time
+// between products was taken out: exponentials run beside the next scores' products, the
+// maximum beside the sums' products, addresses of 64 tiles are worked out at once.  Waves
+// whose rows are behind the last copy alone (a call of 64 rows on 8-bit pages 58 us, 63
+// if they compute, too; workgroups of two waves 59).
+template <class E, int D, bool Q8>
+__global__ __launch_bounds__(kPagedThreads, 2) void prompt_kernel(AttendArgs a) {
   using T = typename E::type;
   using vec8 = typename E::vec8;
-  constexpr int KT = kPagedKeys, ROWS = 128 * QN;
+  constexpr int KT = kPagedKeys, ROWS = 128;
   constexpr int BYTES = Q8 ? D : 2 * D, UNITS = BYTES / 16;  // of a row; its 16-byte units
   constexpr int CROWS = 64 / UNITS, COPIES = 16 / CROWS;     // rows of a copy; of k or v, a wave
   constexpr uint32_t kTile = KT * BYTES;                     // bytes of a tile of k or v
@@ -74,6 +82,7 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
   const PagedSpan span = PagedSpan(a, b).uniform();
   const int rows_all = a.T * a.qpk, rows = span.live * a.qpk;
   const int r0 = row_tile * ROWS;
+  const bool idle = r0 + 32 * wave >= rows;  // a wave that copies alone
 
   // Rows of the cache [low, end) and those before a.sinks matter to this workgroup's
   // tokens, early to late; of their tiles it takes those of its share: [a0, a0 + na) and
@@ -95,28 +104,27 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
 
   // Queries: lane (f, c) holds of row c of 32 the elements that it multiplies with those of
   // a key: of 16 8 f .., or with 8-bit keys, of 32 16 f ...
-  vec8 q[QN][D / 16];
-  int pos[QN];  // the row of its token
-#pragma unroll
-  for (int t = 0; t < QN; ++t) {
-    const int r = r0 + (wave * QN + t) * 32 + c;
+  vec8 q[D / 16];
+  int pos;  // the row of its token
+  {
+    const int r = r0 + 32 * wave + c;
     const bool in = r < rows;
     const int node = in ? r / a.qpk : 0;
-    pos[t] = span.len + node;
+    pos = span.len + node;
     const T* const from = static_cast<const T*>(a.q) +
                           ((static_cast<int64_t>(b) * a.T + node) * a.n_heads + h * a.qpk +
                            (in ? r - node * a.qpk : 0)) * D;
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
       const int e = Q8 ? 32 * (s / 2) + 16 * f + 8 * (s % 2) : 16 * s + 8 * f;
-      q[t][s] = in ? *reinterpret_cast<const vec8*>(from + e) : vec8{};
+      q[s] = in ? *reinterpret_cast<const vec8*>(from + e) : vec8{};
     }
     if (a.sign != 1.0f) {  // a scale that is not positive: its sign goes into q, exactly
 #pragma unroll
       for (int s = 0; s < D / 16; ++s)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          q[t][s][i] = static_cast<T>(static_cast<float>(q[t][s][i]) * a.sign);
+          q[s][i] = static_cast<T>(static_cast<float>(q[s][i]) * a.sign);
     }
   }
 
@@ -200,15 +208,9 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
   auto copy_k = [&](int i, const Tile& t, uint32_t buf) { copy(i, t, t.k, from_k, lds0 + buf); };
   auto copy_v = [&](int i, const Tile& t) { copy(i, t, t.v, from_v, lds0 + (i & 1) * kTile); };
 
-  f16_t acc[QN][D / 32];
-  float top[QN];   // the reference of query c, in powers of two
-  f16_t sum[QN];   // of the probabilities: sixteen copies
-#pragma unroll
-  for (int t = 0; t < QN; ++t) {
-    top[t] = -INFINITY, sum[t] = f16_t{};
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d) acc[t][d] = f16_t{};
-  }
+  f16_t acc[D / 32] = {};
+  float top = -INFINITY;  // the reference of query c, in powers of two
+  f16_t sum = {};         // of the probabilities: sixteen copies
 
   // Byte offsets within a tile: of row c, k elements 8 f .. of each 16 (8 bits: 16 f .. of
   // each 32); v elements 4 (l % 4) .. of 16 of row 4 f + l / 4 % 4 (8 bits: 8 (l % 2) .. of
@@ -228,9 +230,6 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
   vec8 ones;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = static_cast<T>(1.0f);
-  struct Scores {
-    f16_t s[QN];  // of 32 keys
-  };
   // K's operands of 32 keys: the e-th product takes lane elements from LDS four products
   // ahead.
   constexpr int N = D / 16, AHEAD = 4;
@@ -284,48 +283,37 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
   };
   // Hides what this lane's queries do not see of 32 keys; `has`: which of their two 16-row
   // groups has a page.
-  auto hide = [&](Scores& x, int key0, uint32_t has) {
+  auto hide = [&](f16_t& x, int key0, uint32_t has) {
     auto below = [](int n) { return (1u << min(max(n, 0), 4)) - 1u; };
 #pragma unroll
-    for (int t = 0; t < QN; ++t)
+    for (int u = 0; u < 4; ++u) {
+      const int key = key0 + 8 * u + 4 * f;
+      const uint32_t near = ~below(pos - a.window + 1 - key) | below(a.sinks - key);
+      uint32_t seen = near & below(min(pos + 1, end) - key);
+      seen = (has >> (u / 2) & 1u) != 0 ? seen : 0u;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int key = key0 + 8 * u + 4 * f;
-        const uint32_t near = ~below(pos[t] - a.window + 1 - key) | below(a.sinks - key);
-        uint32_t seen = near & below(min(pos[t] + 1, end) - key);
-        seen = (has >> (u / 2) & 1u) != 0 ? seen : 0u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if ((seen >> e & 1u) == 0) x.s[t][4 * u + e] = -INFINITY;
-      }
-  };
-  float m[QN];  // the largest of a lane's scores of the next 32 keys, not scaled
-  auto largest = [&](const Scores& x) {
-#pragma unroll
-    for (int t = 0; t < QN; ++t) {
-      m[t] = x.s[t][0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) m[t] = fmaxf(m[t], x.s[t][e]);
+      for (int e = 0; e < 4; ++e)
+        if ((seen >> e & 1u) == 0) x[4 * u + e] = -INFINITY;
     }
+  };
+  float m;  // the largest of a lane's scores of the next 32 keys, not scaled
+  auto largest = [&](const f16_t& x) {
+    m = x[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) m = fmaxf(m, x[e]);
   };
   auto move = [&]() {
-    bool moves = false;
+    if (!__any(m * a.scale - top > kPagedSlack + kPagedLift<E>)) return;
+    const Pair both = swap_pair<32>(m * a.scale);
+    const float up = fmaxf(fmaxf(both.a, both.b) - kPagedLift<E>, top);
+    const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top - up);
+    top = up;
 #pragma unroll
-    for (int t = 0; t < QN; ++t) moves |= m[t] * a.scale - top[t] > kPagedSlack + kPagedLift<E>;
-    if (!__any(moves)) return;
+    for (int e = 0; e < 16; ++e) sum[e] *= keep;
 #pragma unroll
-    for (int t = 0; t < QN; ++t) {
-      const Pair both = swap_pair<32>(m[t] * a.scale);
-      const float up = fmaxf(fmaxf(both.a, both.b) - kPagedLift<E>, top[t]);
-      const float keep = up == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(top[t] - up);
-      top[t] = up;
+    for (int d = 0; d < D / 32; ++d)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sum[t][e] *= keep;
-#pragma unroll
-      for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[t][d][e] *= keep;
-    }
+      for (int e = 0; e < 16; ++e) acc[d][e] *= keep;
   };
   // Probabilities and sums of the j-th 32 keys of a tile, whose scores are x, beside the
   // scores of the next 32 (the next_j-th of theirs): a product of the scores, two
@@ -333,26 +321,21 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
   // and the first operands of the products after them (the after_j-th 32 keys where
   // `between` has left ka).
   Ahead k;
-  auto turn = [&](const Scores& x, Scores& next, int j, int next_j, int after_j, auto between) {
+  auto turn = [&](const f16_t& x, f16_t& next, int j, int next_j, int after_j, auto between) {
     Ahead v;
     move();
-    vec8 p[QN][2];
-    float base[QN];
-#pragma unroll
-    for (int t = 0; t < QN; ++t) base[t] = top[t] == -INFINITY ? 0.0f : top[t];
+    vec8 p[2];
+    const float base = top == -INFINITY ? 0.0f : top;
     auto read_v = [&](int e) { v.at[e % AHEAD] = values(e % (D / 32), 2 * j + e / (D / 32)); };
     constexpr int PER = 16 / N;  // scores beside a product
 #pragma unroll
     for (int e = 0; e < N; ++e) {
+      next = mfma32<E>(k.at[e % AHEAD], q[e], e == 0 ? f16_t{} : next);
 #pragma unroll
-      for (int t = 0; t < QN; ++t) {
-        next.s[t] = mfma32<E>(k.at[e % AHEAD], q[t][e], e == 0 ? f16_t{} : next.s[t]);
-#pragma unroll
-        for (int u = 0; u < PER; ++u) {
-          const int at = e * PER + u;
-          p[t][at / 8][at % 8] = static_cast<T>(
-              __builtin_amdgcn_exp2f(__builtin_fmaf(x.s[t][at], a.scale, -base[t])));
-        }
+      for (int u = 0; u < PER; ++u) {
+        const int at = e * PER + u;
+        p[at / 8][at % 8] =
+            static_cast<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[at], a.scale, -base)));
       }
       read_k(k, e + kFree, next_j);
       if (e + AHEAD >= N) read_v(e + AHEAD - N);
@@ -366,11 +349,8 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
     constexpr int M = D / 16;
 #pragma unroll
     for (int e = 0; e < M; ++e) {
-#pragma unroll
-      for (int t = 0; t < QN; ++t) {
-        if (e % (D / 32) == 0) sum[t] = mfma32<E>(ones, p[t][e / (D / 32)], sum[t]);
-        acc[t][e % (D / 32)] = mfma32<E>(v.at[e % AHEAD], p[t][e / (D / 32)], acc[t][e % (D / 32)]);
-      }
+      if (e % (D / 32) == 0) sum = mfma32<E>(ones, p[e / (D / 32)], sum);
+      acc[e % (D / 32)] = mfma32<E>(v.at[e % AHEAD], p[e / (D / 32)], acc[e % (D / 32)]);
       if (e + AHEAD < M) read_v(e + AHEAD);
       if (e + AHEAD >= M) read_k(k, e + AHEAD - M, after_j);
       if (e == M / 2) largest(next);
@@ -424,7 +404,7 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
     return has == 15u && key0 + KT <= min(span.len + early + 1, end) &&
            (key0 > span.len + late - a.window || key0 + KT <= a.sinks);
   };
-  Scores x, y;
+  f16_t x, y;  // scores of 32 keys
   uint32_t buf0 = 2 * kTile, buf1 = 3 * kTile, buf2 = 4 * kTile;  // of k of tiles i, i + 1, i + 2
   Tile now = {}, next = {};  // tiles i and i + 1
   if (count > 0) {
@@ -440,9 +420,7 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
     for (int e = 0; e < AHEAD; ++e) read_k(k, e, 0);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-#pragma unroll
-      for (int t = 0; t < QN; ++t)
-        x.s[t] = mfma32<E>(k.at[e % AHEAD], q[t][e], e == 0 ? f16_t{} : x.s[t]);
+      x = mfma32<E>(k.at[e % AHEAD], q[e], e == 0 ? f16_t{} : x);
       read_k(k, e + kFree, 0);
     }
     largest(x);
@@ -468,14 +446,16 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
       next = tile_of(i + 2);
       copy_k(i + 2, next, buf2);
     }
-    if (!all) hide(x, key0, has), largest(x);
-    turn(x, y, 0, 1, 0, [&]() {
-      spread(now.k_scales, kscale);
-      shift_by(ka, buf1 - buf0);
-    });
-    if (!all) hide(y, key0 + 32, has >> 2), largest(y);
-    turn(y, x, 1, 0, 1, []() {});
-    shift_by(va, i % 2 == 0 ? kTile : 0u - kTile);
+    if (!idle) {
+      if (!all) hide(x, key0, has), largest(x);
+      turn(x, y, 0, 1, 0, [&]() {
+        spread(now.k_scales, kscale);
+        shift_by(ka, buf1 - buf0);
+      });
+      if (!all) hide(y, key0 + 32, has >> 2), largest(y);
+      turn(y, x, 1, 0, 1, []() {});
+      shift_by(va, i % 2 == 0 ? kTile : 0u - kTile);
+    }
     const uint32_t free = buf0;
     buf0 = buf1, buf1 = buf2, buf2 = free;
   }
@@ -496,10 +476,7 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
         if (!is_page(page) || plain(i, has)) continue;
         const char* const row = a.v + h * a.vh + page * a.vp + (key & ((1 << a.shift) - 1)) * a.vr;
         const float s = Q8 ? power(a.v_scales[static_cast<int64_t>(page) * a.n_kv + h]) : 1.0f;
-        bool sees[QN];
-#pragma unroll
-        for (int t = 0; t < QN; ++t)
-          sees[t] = key <= pos[t] && (key > pos[t] - a.window || key < a.sinks);
+        const bool sees = key <= pos && (key > pos - a.window || key < a.sinks);
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) {
           us4_t v;
@@ -515,8 +492,7 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
             const float z = (v[e] & E::kExponent) != E::kExponent ? 0.0f
                             : (v[e] & 0x7fff) != E::kExponent     ? __builtin_nanf("")
                             : (v[e] >> 15) != 0                   ? -INFINITY : INFINITY;
-#pragma unroll
-            for (int t = 0; t < QN; ++t) acc[t][n / 4][4 * (n % 4) + e] += sees[t] ? z : 0.0f;
+            acc[n / 4][4 * (n % 4) + e] += sees ? z : 0.0f;
           }
         }
       }
@@ -525,40 +501,37 @@ __global__ __launch_bounds__(kPagedThreads, QN == 1 ? 2 : 1) void prompt_kernel(
   const int64_t rec0 = (static_cast<int64_t>(h) * a.shares + w) * rows_all;
   float* const sums = a.partial + rec0 * D;
   float* const stats = a.partial + static_cast<int64_t>(a.n_kv) * a.shares * rows_all * D + rec0 * 2;
+  const int r = r0 + 32 * wave + c;
+  const bool behind = r >= rows;  // the last token
+  const float l = behind ? 0.0f : sum[0];
+  if (behind) top = -INFINITY;
+  else if (top == -INFINITY && l != 0.0f) top = 0.0f;  // NaN scores alone
+  if (r >= rows_all) return;
+  if (a.shares == 0) {
+    const int node = r / a.qpk;
+    T* const out = static_cast<T*>(a.out) +
+                   ((static_cast<int64_t>(b) * a.T + node) * a.n_heads + h * a.qpk +
+                    (r - node * a.qpk)) * D + 4 * f;
+    typedef T vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-  for (int t = 0; t < QN; ++t) {
-    const int r = r0 + (wave * QN + t) * 32 + c;
-    const bool behind = r >= rows;  // the last token
-    const float l = behind ? 0.0f : sum[t][0];
-    if (behind) top[t] = -INFINITY;
-    else if (top[t] == -INFINITY && l != 0.0f) top[t] = 0.0f;  // NaN scores alone
-    if (r >= rows_all) continue;
-    if (a.shares == 0) {
-      const int node = r / a.qpk;
-      T* const out = static_cast<T*>(a.out) +
-                     ((static_cast<int64_t>(b) * a.T + node) * a.n_heads + h * a.qpk +
-                      (r - node * a.qpk)) * D + 4 * f;
-      typedef T vec4 __attribute__((ext_vector_type(4)));
+    for (int e = 0; e < D / 8; ++e) {
+      vec4 y;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        y[x] = static_cast<T>(l == 0.0f ? 0.0f : acc[e / 4][4 * (e % 4) + x] / l);
+      *reinterpret_cast<vec4*>(out + 8 * e) = y;
+    }
+  } else {
+    if (top != -INFINITY) {
 #pragma unroll
       for (int e = 0; e < D / 8; ++e) {
-        vec4 y;
+        f4_t y;
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          y[x] = static_cast<T>(l == 0.0f ? 0.0f : acc[t][e / 4][4 * (e % 4) + x] / l);
-        *reinterpret_cast<vec4*>(out + 8 * e) = y;
+        for (int x = 0; x < 4; ++x) y[x] = acc[e / 4][4 * (e % 4) + x];
+        *reinterpret_cast<f4_t*>(sums + static_cast<int64_t>(r) * D + 8 * e + 4 * f) = y;
       }
-    } else {
-      if (top[t] != -INFINITY) {
-#pragma unroll
-        for (int e = 0; e < D / 8; ++e) {
-          f4_t y;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) y[x] = acc[t][e / 4][4 * (e % 4) + x];
-          *reinterpret_cast<f4_t*>(sums + static_cast<int64_t>(r) * D + 8 * e + 4 * f) = y;
-        }
-      }
-      if (f == 0) stats[2 * r] = top[t], stats[2 * r + 1] = l;
     }
+    if (f == 0) stats[2 * r] = top, stats[2 * r + 1] = l;
   }
 }
 
