@@ -25,6 +25,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "nibble_common.h"
 #include "paged_prompt.h"
 #include "paged_rows.h"
 

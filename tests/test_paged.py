@@ -9,13 +9,18 @@ errors, and, of 8-bit codes, the nearest one of a value known that well.
 from __future__ import annotations
 
 import math
+import os
+import re
+import shutil
+import subprocess
 
 import pytest
 import torch
 
 import nibblegemm_amd as ng
-from nibblegemm_amd import glue, paged
+from nibblegemm_amd import build, glue, paged
 
+OBJDUMP = os.path.join(os.path.dirname(os.path.dirname(build._hipcc())), "llvm", "bin", "llvm-objdump")
 INVALID, WORKSPACE = 1, 3
 P = 1 << 20  # aligned, never dereferenced
 dev = "cuda"
@@ -1091,3 +1096,58 @@ def test_refusals():
         paged.paged_values(k, v, t, n, rows=-1)
     # pages that are read may be expanded views
     assert paged.attention_paged(x, k[:1].expand(4, 2, 16, 128), v, t, n).shape == x.shape
+
+
+# ---------------------------------------------------------------------------
+# the built code
+# ---------------------------------------------------------------------------
+
+@pytest.mark.skipif(not os.path.exists(OBJDUMP), reason="llvm-objdump not installed")
+def test_rows_kernel_waits_match_its_copies(tmp_path):
+    """The kernel of a decode step reads a ring in LDS that is its wave's alone, and lets
+    all copies but the next ones stay in flight, by count: each of its four waits (k and
+    v, with and without a mask) has as many copies behind it as the ring has room for, less
+    those that it waits for.  Right only if k and v are as many copies each as counted, and
+    if whatever else the loop loads (pages, scales) is waited for in full.  Seen in the built
+    code, for every form and type."""
+    lib = shutil.copy(build.LIB, tmp_path)
+    subprocess.run([OBJDUMP, "--offloading", lib], cwd=tmp_path, capture_output=True, check=True)
+    objects = [p for p in sorted(tmp_path.iterdir())
+               if "gfx950" in p.name and b"rows_kernel" in p.read_bytes()]
+    forms = set()
+    for at in objects:
+        text = subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", str(at)], capture_output=True,
+                              text=True, check=True).stdout
+        parts = re.split(r"\n[0-9a-f]+ <([^>]+)>:\n", text)
+        for name, body in zip(parts[1::2], parts[2::2]):
+            form = re.search(r"rows_kernelINS_(4Half|6Bfloat)ELi(\d+)ELi(\d+)ELb(\d)EEE", name)
+            if form is None:
+                continue
+            forms.add(form.groups())
+            unit = 16 * int(form[2]) * (1 if form[4] == "1" else 2)  # bytes of 16 rows of k
+            copies, ring = unit // 1024, 8192 // (2 * unit)
+            seen = []  # copies, other memory operations, waits and barriers, in order
+            for line in body.splitlines():
+                op = line.split("//")[0].strip()
+                if re.match(r"(buffer|global|flat|scratch)_", op):
+                    seen.append("copy" if op.endswith("lds") else op.split()[0])
+                elif op.startswith("s_waitcnt") and "vmcnt" in op:
+                    seen.append(int(re.search(r"vmcnt\((\d+)\)", op)[1]))
+                elif op.startswith("s_barrier"):
+                    seen.append("barrier")
+            last = len(seen) - seen[::-1].index("copy")
+            seen = seen[seen.index("copy"):seen.index("barrier", last) + 1]
+            # pages' and scales' loads, each with its wait
+            rest, i = [], 0
+            while i < len(seen):
+                loads = 0
+                while seen[i + loads] in ("global_load_dword", "global_load_ubyte"):
+                    loads += 1
+                if loads == 0:
+                    rest.append(seen[i])
+                else:
+                    assert seen[i + loads] == 0, name
+                i += loads + 1
+            turn = [(2 * ring - 1) * copies] + ["copy"] * copies
+            assert rest == ["copy"] * (2 * copies) + turn * 4 + [0, "barrier"], name
+    assert len(forms) == 2 * 2 * 2 * 2  # types, heads, tiles of 16 query rows, bits
