@@ -178,7 +178,8 @@ extern "C" int nibble_attention_paged(const void* Q, int64_t dtype, int64_t batc
   a.T = static_cast<int>(tokens);
   a.n_heads = static_cast<int>(n_heads);
   a.n_kv = static_cast<int>(c.n_kv_heads);
-  a.width = static_cast<int>(c.table_pages);
+  // (where there are no pages, there are no scales to read either)
+  a.width = c.n_pages > 0 ? static_cast<int>(c.table_pages) : 0;
   a.n_pages = static_cast<int>(c.n_pages);
   a.shift = P == 16 ? 4 : P == 32 ? 5 : P == 64 ? 6 : P == 128 ? 7 : 8;
   a.window = window > 0 ? static_cast<int>(window) : 1 << 30;

@@ -539,6 +539,20 @@ def test_append_to_no_pages_at_all():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("T", [1, 40, 200])
+def test_attention_over_no_pages_at_all(T, bits):
+    k, v, scales = paged.paged_cache(0, 1, 16, 64, F16 if bits == 16 else F8)
+    table = torch.zeros((2, 40), dtype=torch.int32, device=dev)
+    n = to_dev(ints([0, 400]))
+    q = torch.full((2, T, 64), 3.0, dtype=F16, device=dev)
+    out = paged.attention_paged(q, k, v, table, n, scales=scales)
+    assert torch.equal(out, torch.zeros_like(q))
+    dense = paged.paged_values(k, v, table, n, scales, rows=500)
+    assert not dense[0].any() and not dense[1].any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D,page", [(64, 16), (128, 32), (128, 64), (64, 128), (128, 256)])
 def test_append_raises_the_scale(D, page, dtype):
