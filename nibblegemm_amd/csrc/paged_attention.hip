@@ -65,7 +65,9 @@ int plan_paged(int64_t batch, int64_t tokens, int64_t n_heads, int64_t n_kv, int
   // cached rows are split, unless there are but a few tiles of them.
   const int64_t room = kSplitWorkgroups / (n_kv * p->row_tiles);
   const bool line = p->rows <= 32;  // rows_kernel's
-  if (line ? room > 0 && batch <= kSplitWorkgroups && batch * n_kv < 4 * kSplitWorkgroups
+  // (the line's length, in tiles and gaps, has to stay far below 2^31)
+  if (line ? room > 0 && batch <= kSplitWorkgroups && batch * n_kv < 4 * kSplitWorkgroups &&
+                 batch * (max_rows / kPagedKeys + 8) < (int64_t(1) << 30)
            : room > batch && batch < kSplitWorkgroups) {
     if (max_rows <= 4 * kPagedKeys) return NIBBLE_OK;
     p->shares = static_cast<int>(room);

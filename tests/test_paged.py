@@ -430,6 +430,9 @@ def test_attention_workspace():
     need, counters = ext.attention_paged_workspace_bytes(1, 1, 32, 8, 128, 65536)
     assert need > counters > 0 and counters % 256 == 0
     assert ext.attention_paged_workspace_bytes(1, 1, 32, 8, 96, 65536) == (0, 0)  # a refused plan
+    # the tiles of all sequences are counted in 32 bits: not where they may pass them
+    assert ext.attention_paged_workspace_bytes(63, 1, 8, 2, 64, (1 << 30) - 16)[0] > 0
+    assert ext.attention_paged_workspace_bytes(400, 1, 8, 2, 64, (1 << 30) - 16) == (0, 0)
     big = dict(T=1, nh=32, nkv=8, width=4096)
     assert attend(ext, **big) == WORKSPACE and "workspace" in ext.last_error()
     assert attend(ext, **big, ws=P, wsb=need - 1) == WORKSPACE
