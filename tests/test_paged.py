@@ -760,6 +760,37 @@ def test_many_sequences_of_uneven_lengths(n_kv, n_heads, B, bits):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("T,n_heads,n_kv,B", [(40, 1, 1, 100), (34, 2, 2, 255), (130, 1, 1, 9), (1, 8, 8, 300),
+                                              (2, 64, 64, 9), (9, 16, 2, 70)])
+def test_many_sequences_of_many_rows_or_heads(T, n_heads, n_kv, B, bits):
+    """More sequences than a wave has lanes, of calls that are split or not, with and
+    without tokens, by either kernel; more kv heads than room for shares."""
+    g = torch.Generator().manual_seed(B)
+    lengths = (torch.rand(B, generator=g) ** 8 * 1500).int().tolist()
+    sizes = torch.randint(0, T + 1, (B,), generator=g).int().tolist()
+    case = attention_case(T, n_heads, n_kv, 64, 16, lengths, BF16, bits, sizes=sizes)
+    check_attention(*case)
+    check_attention(*case, 70, 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 5, 60])
+def test_expanded_pages_are_read(T):
+    """One page for all places of the pool, one row for all of a page: strides of zero."""
+    g = torch.Generator().manual_seed(T)
+    page = torch.randn((1, 2, 16, 64), generator=g).half()
+    row = torch.randn((5, 1, 1, 64), generator=g).half()
+    k, v = to_dev(page).expand(5, 2, 16, 64), to_dev(row).expand(5, 2, 16, 64)
+    table, n = to_dev(ints([[4, 0, 2, 1, 3] * 5])), to_dev(ints([300]))
+    q = to_dev(torch.randn((1, T, 4 * 64), generator=g).half())
+    want = paged.attention_paged(q, k.contiguous(), v.contiguous(), table, n)
+    assert torch.equal(paged.attention_paged(q, k, v, table, n), want)
+    with pytest.raises(RuntimeError, match="expanded"):
+        paged.paged_append(to_dev(torch.zeros((1, T, 8 * 64)).half()), k, v, table, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 8])
 def test_a_page_that_passes_32_bits(bits):
     """Pages 4 GiB and more into a pool, read and written."""
     n_kv, page, D, dtype = 8, 256, 128, BF16
