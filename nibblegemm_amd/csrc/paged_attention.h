@@ -16,7 +16,7 @@ constexpr int kPagedThreads = 256;
 constexpr int kPagedKeys = 64;  // keys of a tile
 // What the sums of a share cost that are written and joined, in tiles: of a call, and of
 // its query rows.  (2 x 12 tokens of 32 + 2 x 4 heads over 20000 rows of 8 bits: 37 us, 35
-// if it costs nothing, 54 if four times that; 4 x 60 of 8 + 2 x 8 over 2000: 20, 24, 25.)
+// if it costs nothing, 54 if four times that; 4 x 60 of 8 + 2 x 8 over 2000: 20, 25, 27.)
 constexpr float kPagedShareCost = 0.08f, kPagedRowCost = 4.8e-4f;
 // Probabilities are relative to a query's reference, 2^lift below a maximum, which
 // moves only when a score passes that maximum by more than the slack (in powers of two).

@@ -37,8 +37,9 @@ __device__ __forceinline__ int prompt_swizzle(int r) {
 // 113 to 130, by the card's clock, which falls to 1.9 GHz meanwhile.  What fills the time
 // between products was taken out: exponentials run beside the next scores' products, the
 // maximum beside the sums' products, addresses of 64 tiles are worked out at once.  Waves
-// whose rows are behind the last copy alone (a call of 64 rows on 8-bit pages 58 us, 63
-// if they compute, too; workgroups of two waves 59).
+// whose rows are behind the last copy alone (64 rows over 32 x 4096 of 8 bits: 5 us of 58
+// less than if they compute, too; as much as by workgroups of two waves, which take 4 more
+// than these on 16 bits).
 template <class E, int D, bool Q8>
 __global__ __launch_bounds__(kPagedThreads, 2) void prompt_kernel(AttendArgs a) {
   using T = typename E::type;
@@ -67,12 +68,12 @@ __global__ __launch_bounds__(kPagedThreads, 2) void prompt_kernel(AttendArgs a) 
   const int row_tile = a.fold && rt >= (a.row_tiles + 1) / 2 ? rt - (a.row_tiles + 1) / 2
                                                              : a.row_tiles - 1 - rt;
   const int w = pair / a.n_kv, h = pair - w * a.n_kv;
-  int b = w, share = 0, per = 0x3fffffff;  // the whole sequence
+  int b = w, share = 0, pieces = 1;
   if (a.shares > 0) {
     if (w >= a.shares) return;
     const Shares<AttendArgs> shares(a, w);
     if (shares.found < 0) return;
-    b = shares.found, share = w - shares.first, per = shares.per;
+    b = shares.found, share = w - shares.first, pieces = shares.count;
     // (for the kernel that joins them)
     if (share == 0 && h == 0 && rt == 0 && threadIdx.x == 0)
       a.runs[2 * b] = shares.first, a.runs[2 * b + 1] = shares.count;
@@ -92,8 +93,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void prompt_kernel(AttendArgs a) 
   const int low = end > 0 ? max(span.len + early - a.window + 1, 0) : 0;
   int a0, na, b0, count;
   {
+    // (a sequence's shares are equal: with as many tiles as Shares allows and a rest, 64 rows
+    // over 32 x 4096 take 66 us in place of 60, of 8 bits 58 in place of 52)
     const Seen all = span.seen(a), own(low, a.sinks, end);
-    const int x0 = min(share * per, 0x3fffffff), x1 = x0 + min(per, 0x3fffffff);  // of all's tiles
+    const int per = (all.first + all.upto - all.from + pieces - 1) / pieces;
+    const int x0 = share * per, x1 = x0 + per;  // of all's tiles
     const int shift = all.from - all.first;  // from place to tile, behind the first
     a0 = x0;
     na = max(0, min(all.first > 0 ? min(x1, all.first) : x1, own.first) - a0);
