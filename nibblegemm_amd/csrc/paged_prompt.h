@@ -156,9 +156,14 @@ __global__ __launch_bounds__(kPagedThreads, 2) void prompt_kernel(AttendArgs a) 
       const int of = page_at(key0 + 16 * n);
       places.has |= is_page(of) ? 1u << n : 0u;
       if constexpr (Q8) {
-        const int64_t s = static_cast<int64_t>(is_page(of) ? of : 0) * a.n_kv + h;
-        places.k_scales |= static_cast<uint32_t>(a.k_scales[s]) << (8 * n);
-        places.v_scales |= static_cast<uint32_t>(a.v_scales[s]) << (8 * n);
+        // (of a group that no token sees the scale may be anything: 255 would make NaN of the
+        // zeros that are read in its place)
+        const int key = key0 + 16 * n;
+        const bool is = is_page(of) && key < end && (key + 16 > low || key < a.sinks);
+        const int64_t s = static_cast<int64_t>(is ? of : 0) * a.n_kv + h;
+        const uint32_t ks = a.k_scales[s], vs = a.v_scales[s];
+        places.k_scales |= (is ? ks : 127u) << (8 * n);
+        places.v_scales |= (is ? vs : 127u) << (8 * n);
       }
     }
     whole = __ballot(is_page(page) && mine + 16 <= end && (mine >= low || mine + 16 <= a.sinks));
@@ -441,6 +446,13 @@ __global__ __launch_bounds__(kPagedThreads, 2) void prompt_kernel(AttendArgs a) 
     spread(now.v_scales, vscale);
     if (!all) {
       clean(i & 1);
+      if constexpr (Q8) {  // (a scale of 255, too: under it a zero code is NaN)
+        uint32_t bytes = now.v_scales;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          if ((bytes >> (8 * n) & 255) == 255) bytes ^= 128u << (8 * n);
+        spread(bytes, vscale);
+      }
       lds_barrier();
     }
     if (i + 1 < count) copy_v(i + 1, next);

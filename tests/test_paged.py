@@ -1146,6 +1146,47 @@ def test_refusals():
     assert paged.attention_paged(x, k[:1].expand(4, 2, 16, 128), v, t, n).shape == x.shape
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,n_heads", [(1, 4), (3, 8), (6, 8), (40, 8), (90, 8)])
+def test_scales_of_pages_that_are_not_seen(T, n_heads, dtype, D):
+    """What the scale is of a page that nothing sees does not matter: of pages that no
+    sequence has (the first among them), of those that a table names for rows to come."""
+    for n, window, sinks in ((37, None, 0), (130, None, 0), (300, 60, 20)):
+        q, cache, lengths, _ = attention_case(T, n_heads, 2, D, 16, [n, n // 2], dtype, 8,
+                                              width=-(-(n + T) // 16) + 3)
+        cache.table[cache.table == 0] = -1
+        seen = torch.zeros(len(cache.k), dtype=torch.bool)
+        for b, first in enumerate(lengths.tolist()):
+            for m, page in enumerate(cache.table[b].tolist()):
+                in_window = window is None or (m + 1) * 16 > first - window + 1 or m * 16 < sinks
+                seen[page] |= page >= 0 and m * 16 < first + T and in_window
+        assert not seen[0]
+        for s in cache.scales:
+            s[~seen] = 255
+        check_attention(q, cache, lengths, None, window, sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,n_heads", [(6, 2), (6, 8), (24, 8), (40, 8), (90, 8)])
+def test_a_scale_that_is_none(T, n_heads, dtype):
+    """The values of a page whose scale is 255 are NaN, for the tokens that see it alone."""
+    for n in (14, 125):  # its rows: the last token's own, and some before
+        q, cache, lengths, _ = attention_case(T, n_heads, 2, 128, 16, [n, n], dtype, 8)
+        first = (n + T - 1) // 16
+        want, bound = oracle_attention(q, cache, lengths, None, None, 0, 128 ** -0.5)
+        for which in range(2):
+            was = cache.scales[which].clone()
+            cache.scales[which][cache.table[0, first]] = 255
+            got = run_attention(q, cache, lengths).cpu().double()
+            cache.scales[which][:] = was
+            nan = torch.zeros((2, T), dtype=torch.bool)
+            nan[0] = n + torch.arange(T) >= 16 * first
+            assert got[nan].isnan().all() and ((got - want).abs() <= bound)[~nan].all()
+
+
 # ---------------------------------------------------------------------------
 # the built code
 # ---------------------------------------------------------------------------
