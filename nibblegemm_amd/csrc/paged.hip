@@ -284,7 +284,9 @@ __device__ __forceinline__ void append_page(const PagedArgs& a) {
     }
   }
   if (me == 0 && e != was) *scale = static_cast<uint8_t>(e);
-  const float inverse = power(254 - e), most = e >= kHighExponent<E> ? kFloat8LastMax : kFloat8Max;
+  // (2^-127, the inverse of a caller's scale of 254, is subnormal)
+  const float inverse = e == 254 ? 0x1p-127f : power(254 - e);
+  const float most = e >= kHighExponent<E> ? kFloat8LastMax : kFloat8Max;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     if (!live[n]) continue;

@@ -1187,6 +1187,18 @@ def test_a_scale_that_is_none(T, n_heads, dtype):
             assert got[nan].isnan().all() and ((got - want).abs() <= bound)[~nan].all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("was,size", [(254, 1.0), (254, 2.0 ** 13), (253, 2.0 ** 13), (0, 1.0), (1, 2.0 ** -14)])
+def test_append_beside_any_scale(was, size, dtype):
+    """Pages of earlier rows whose scale a caller wrote: one of all that a byte holds."""
+    size = size if dtype == F16 else size ** 9.5
+    cache, qkv, lengths, _ = append_case(5, 2, 2, 64, 16, [13, 8, 1, 0], dtype, 8, size=size,
+                                         exponents=(was - 121, was - 120))
+    assert cache.scales[0].eq(was).all() and qkv.isfinite().all()
+    check_append(cache, qkv, lengths)
+
+
 # ---------------------------------------------------------------------------
 # the built code
 # ---------------------------------------------------------------------------
