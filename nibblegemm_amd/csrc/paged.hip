@@ -266,10 +266,10 @@ __device__ __forceinline__ void append_page(const PagedArgs& a) {
   char* const base = which != 0 ? a.v + page * a.vp + h * a.vh : a.k + page * a.kp + h * a.kh;
   const int64_t stride = which != 0 ? a.vr : a.kr;
   const int need = exponent_for<E>(top);
-  const bool fresh = begin == first;
-  const int e = fresh ? need : min(max(need, was), 254);
+  const bool fresh = begin == first, none = was == 255;  // no power: earlier rows are NaN
+  const int e = fresh || none ? need : max(need, was);
   if (!fresh && e != was) {  // earlier rows, on the new power of two
-    const float by = power(max(127 + was - e, 1));
+    const float by = none ? __builtin_nanf("") : power(max(127 + was - e, 1));
 #pragma unroll 1
     for (int i = me; i < (begin - first) * LANES; i += WAVES * 64) {
       u4_t* const at = reinterpret_cast<u4_t*>(base + (i / LANES) * stride + 16 * (i % LANES));

@@ -1199,6 +1199,46 @@ def test_append_beside_any_scale(was, size, dtype):
     check_append(cache, qkv, lengths)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_append_beside_rows_without_a_scale(dtype):
+    """Earlier rows under a scale of 255 are NaN, and stay so under the new rows' scale,
+    which is that of a page of their own."""
+    cache, qkv, lengths, _ = append_case(5, 2, 2, 64, 16, [11, 8, 1], dtype, 8)
+    for s in cache.scales:
+        s[:] = 255
+    k, v, table, scales = cache.on_gpu()
+    paged.paged_append(to_dev(qkv), k, v, table, to_dev(lengths), scales=scales)
+    alone = Cache([5] * 3, 2, 64, 16, dtype, 8)
+    k1, v1, t1, s1 = alone.on_gpu()
+    paged.paged_append(to_dev(qkv), k1, v1, t1, to_dev(ints([0] * 3)), scales=s1)
+    for got, want in zip(paged.paged_values(k, v, table, to_dev(lengths + 5), scales, dtype),
+                         paged.paged_values(k1, v1, t1, to_dev(ints([5] * 3)), s1, dtype)):
+        for b, n in enumerate(lengths.tolist()):
+            assert got[b, :, :n].isnan().all()
+            assert torch.equal(got[b, :, n:n + 5], want[b, :, :5])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_values_of_every_code_and_scale(dtype):
+    """All codes under all scales: the value that the two stand for, rounded once (it
+    has four bits); a scale of 255 is no power, its values are NaN."""
+    codes = torch.arange(256, dtype=torch.uint8).view(1, 1, 4, 64).expand(256, 1, 4, 64)
+    k = torch.zeros((256, 1, 16, 64), dtype=torch.uint8)
+    k[:, :, :4] = codes
+    scales = torch.arange(256, dtype=torch.uint8).view(256, 1)
+    k, s = k.view(F8), scales
+    got, same = paged.paged_values(k.to(dev), k.to(dev), torch.arange(256, device=dev, dtype=torch.int32)[None],
+                                   to_dev(ints([4096])), (s.to(dev), s.to(dev)), dtype)
+    want = torch.ldexp(k.double(), scales[:, :, None, None].double() - 127).to(dtype)
+    want[255] = math.nan
+    have = got.view(256, 1, 16, 64).cpu()
+    assert torch.equal(have.isnan(), want.isnan())
+    assert (have == want)[~want.isnan()].all()
+    assert torch.equal(same.view(torch.int16), got.view(torch.int16))
+
+
 # ---------------------------------------------------------------------------
 # the built code
 # ---------------------------------------------------------------------------
