@@ -85,6 +85,7 @@ def _check_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
                 raise RuntimeError(f"{name} must be float8_e4m3fn beside scales, got {t.dtype}")
             if t.get_device() != index:
                 raise RuntimeError(f"{name} must live on GPU {index}, got {t.device}")
+            _check_no_backward(name, t)
         for name, t in zip(("k_scales", "v_scales"), scales):
             if t.get_device() != index:
                 _check_gpu(name, t, k_pages)

@@ -1239,6 +1239,36 @@ def test_values_of_every_code_and_scale(dtype):
     assert torch.equal(same.view(torch.int16), got.view(torch.int16))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", [0, 1])
+def test_8_bit_pages_that_autograd_follows_are_refused(which):
+    """A followed cache, in reverse and in forward mode: no gradient is cut off, and
+    no followed page is written."""
+    k, v, scales = paged.paged_cache(3, 1, 16, 64, F8)
+    n, t = torch.zeros(1, dtype=torch.int32, device=dev), torch.zeros((1, 2), dtype=torch.int32, device=dev)
+    x = torch.zeros((1, 1, 3 * 64), dtype=F16, device=dev)
+    calls = [lambda p: paged.paged_append(x, *p, t, n, scales=scales),
+             lambda p: paged.attention_paged(x, *p, t, n, scales=scales),
+             lambda p: paged.paged_values(*p, t, n, scales)]
+    leaf = (k, v)[which].clone().requires_grad_()
+    made = torch.ones((3, 1, 16, 64), device=dev, requires_grad=True).to(F8)
+    assert made.grad_fn is not None
+    for call in calls:
+        for followed in (leaf, made):
+            pages = [k, v]
+            pages[which] = followed
+            with pytest.raises(RuntimeError, match="no backward"):
+                call(pages)
+            with torch.no_grad():  # followed by nothing here
+                call(pages)
+        with torch.autograd.forward_ad.dual_level():
+            pages = [k, v]
+            call(pages)
+            pages[which] = torch.autograd.forward_ad.make_dual(pages[which], torch.ones_like(pages[which]))
+            with pytest.raises(RuntimeError, match="no backward"):
+                call(pages)
+
+
 # ---------------------------------------------------------------------------
 # the built code
 # ---------------------------------------------------------------------------
