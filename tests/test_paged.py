@@ -1269,6 +1269,41 @@ def test_8_bit_pages_that_autograd_follows_are_refused(which):
                 call(pages)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("T,qpk,n_kv,B,D", [
+    (1, 1, 1024, 2, 128), (1, 2, 1024, 2, 64), (6, 4, 1024, 2, 128),  # a decode step's, not split
+    (1, 1, 128, 9, 64), (6, 4, 128, 9, 64), (9, 2, 128, 2, 128),  # cut in a line, and each by itself
+    (40, 1, 256, 2, 64), (70, 1, 256, 2, 128), (40, 1, 128, 2, 128)])  # prompts', and split
+def test_pieces_of_many_tiles(T, qpk, n_kv, B, D, bits):
+    """More tiles than the 64 whose places are looked up at once in one workgroup: pages
+    in any order, their scales, pages that are missing and masks that end in later ones.
+    All kv heads read the same pages (a stride of zero) under scales of their own."""
+    dtype = F16 if T % 2 else BF16
+    lengths = [9000 - 70 * b for b in range(B)]
+    q, cache, n, _ = attention_case(T, qpk * n_kv, 1, D, 16, lengths, dtype, bits, seed=T)
+    for m in (0, 270, 300, 301, 520):  # tiles 0, 67, 75, 130
+        cache.table[:, m] = -1 if m % 2 else cache.k.shape[0]
+    g = torch.Generator().manual_seed(T)
+    heads = [0, 1, n_kv - 1]  # those that are compared
+    few = Cache([1], 1, D, 16, dtype, bits)
+    few.B, few.table = B, cache.table
+    few.k, few.v = (x.expand(-1, 3, -1, -1) for x in (cache.k, cache.v))
+    scales = None
+    if bits == 8:
+        scales = [torch.randint(119, 124, (len(cache.k), n_kv), generator=g).to(torch.uint8) for _ in range(2)]
+        few.scales = [s[:, heads] for s in scales]
+        scales = tuple(s.to(dev) for s in scales)
+    k, v = (to_dev(x).expand(-1, n_kv, -1, -1) for x in (cache.k, cache.v))
+    some = q.view(B, T, n_kv, qpk, D)[:, :, heads].reshape(B, T, 3 * qpk, D)
+    flat, table = to_dev(q.reshape(B, T, -1)), to_dev(cache.table)
+    for window, sinks in ((None, 0), (3000, 4200)):
+        got = paged.attention_paged(flat, k, v, table, to_dev(n), None, window, sinks, scales=scales)
+        got = got.cpu().double().view(B, T, n_kv, qpk, D)[:, :, heads].reshape(B, T, 3 * qpk, D)
+        want, bound = oracle_attention(some, few, n, None, window, sinks, D ** -0.5)
+        assert ((got - want).abs() <= bound).all()
+
+
 # ---------------------------------------------------------------------------
 # the built code
 # ---------------------------------------------------------------------------
