@@ -485,7 +485,8 @@ NIBBLE_API size_t nibble_attention_tree_workspace_bytes(int64_t batch, int64_t t
  * n_pages) is no page.  The elements are 16 bits wide (dtype: 0 fp16, 1 bf16, as of the
  * call's other tensors), or, with scales, 8: the value is code 2^(scale - 127), code an
  * 8-bit float (e4m3 without infinities), scale uint8 [n_pages, n_kv_heads], one a page
- * and head.  head_dim 64 or 128.  K, V 16-byte aligned, the table 4.
+ * and head (255: the values are NaN).  head_dim 64 or 128.  K, V 16-byte aligned, the
+ * table 4.
  */
 typedef struct {
   void* K;
@@ -505,12 +506,13 @@ typedef struct {
  * Q_out [batch, tokens, n_heads head_dim], k and v of token t < sizes[b] (NULL: tokens)
  * to row lengths[b] + t of sequence b.  positions int32 [batch, tokens] (NULL: a token's
  * row).  A token without a page or without a position in the tables writes no row, and
- * zeros to Q_out.  8-bit pages: a page whose first row is new takes the least scale
- * under which its new rows fit (of those whose products with all codes are values of
- * dtype); one with earlier rows the larger of its own and that, its earlier rows
- * rescaled; rows behind are left.  Magnitudes beyond dtype's largest value count as
- * that value; infinities and NaN become NaN.  Pages that a call writes belong to one
- * sequence each.  batch at most 65535, tokens 2^20; a launch ends at 2^24 - 1
+ * zeros to Q_out.  8-bit pages: a page whose first row is new takes the least scale under
+ * which its new rows fit, of 127 - 15 to 127 + 8 (bf16: 127 - 117 to 127 + 120; under
+ * the last codes end at 240, for larger ones are not values of dtype); one with earlier
+ * rows the larger of its own and that, its earlier rows rescaled (of 255, that, and its
+ * earlier rows stay NaN); rows behind are left.  Magnitudes beyond dtype's largest value
+ * count as that value; infinities and NaN become NaN.  Pages that a call writes belong to
+ * one sequence each.  batch at most 65535, tokens 2^20; a launch ends at 2^24 - 1
  * workgroups. */
 NIBBLE_API int nibble_paged_append(const void* QKV, int64_t dtype, int64_t batch, int64_t tokens,
                                    int64_t n_heads, const nibble_paged_cache* cache,
@@ -522,9 +524,10 @@ NIBBLE_API int nibble_paged_append(const void* QKV, int64_t dtype, int64_t batch
 
 /* Attention of the newest tokens of several sequences over their pages: Q [batch,
  * tokens, n_heads head_dim]; token i < sizes[b] (NULL: tokens) of sequence b is row r =
- * lengths[b] + i and sees the rows j <= r that have a page, of these, with window > 0,
- * those with r - j < window or j < sinks.  Out [batch, tokens, n_heads head_dim] =
- * softmax(scale q k^T) v, zeros for tokens that see nothing and behind a sequence's
+ * lengths[b] + i (lengths from 0 to the rows of the table; r may be behind it) and sees
+ * the rows j <= r that have a page, of these, with window > 0, those with r - j <
+ * window or j < sinks.  Out [batch, tokens, n_heads head_dim] = softmax(scale q k^T) v,
+ * zeros for tokens that see nothing and behind a sequence's
  * last.  scale is finite, also times log2(e).  window (0: none) and sinks are at most
  * 2^30.  The workspace (nibble_attention_paged_workspace_bytes, 256-byte aligned; NULL
  * when that is 0) begins with nibble_attention_paged_counter_bytes that are zero before

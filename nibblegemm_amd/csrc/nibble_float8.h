@@ -8,9 +8,9 @@
 
 namespace nibble {
 
-// The powers of two, biased by 127, whose product with every 8-bit float is a value
-// of a 16-bit type: from subnormals on the type's smallest step to 240 times the
-// last (beyond it the type ends; a code of that power is at most kLastCode).
+// The powers of two, biased by 127, under which 8-bit floats are values of a 16-bit
+// type: the smallest of the first, 2^-9, is fp16's least step or bf16's least normal
+// value; the last ends at 240 (kFloat8LastMax), beyond which the type does.
 constexpr float kFloat8Max = 448.0f, kFloat8LastMax = 240.0f;
 template <class E>
 constexpr int kLowExponent = std::is_same_v<E, Half> ? 127 - 15 : 127 - 117;

@@ -18,7 +18,9 @@
 // Memory bounds both: every value is read once and written once.  What is written goes
 // past the caches (nt), which keep what is read, the product before, instead: 4 x 2000
 // tokens of 32 + 2 x 8 heads of 128 take 36 to 39 us in place of 41 (44 if the reads go
-// past them, too).
+// past them, too).  A decode step, whose q and new rows the attention reads next, is the
+// same either way: 1 over 1000 rows 14.1 us (14.0 without), 64 over 300 17.3 (17.5), 16
+// over 2000 25.9 (25.9).
 #include <cmath>
 
 #include "nibble_common.h"

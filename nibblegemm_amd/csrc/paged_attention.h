@@ -38,14 +38,14 @@ struct AttendArgs {
   const int32_t* lengths;  // [B]
   const int32_t* sizes;    // [B] or null: T each
   void* out;               // [B, T, n_heads, D]
-  float* partial;          // [n_kv][shares][rows][D], then [..][2] (top, sum), when shares > 0
+  float* partial;          // [n_kv][slots][rows][D], then [..][2] (top, sum), when shares > 0
   int* runs;               // [B][2]: a sequence's first share and their number
   int* counters;           // [B][n_kv], zero on entry and on exit: pieces that are written
   int64_t kp, kh, kr, vp, vh, vr;
   int B, T, n_heads, n_kv, qpk, width, n_pages, shift;
   int window, sinks;      // window: 2^30 where there is none
   int shares, row_tiles;  // shares: 0 where no sequence's rows are split
-  int slots;              // of sums and statistics
+  int slots;              // of sums and statistics: one a share, or two (rows_kernel)
   float join_cost;        // of one share, in tiles
   bool fold;              // row tiles from both ends to the middle
   float scale;            // its magnitude times log2(e); 1 for a scale of zero

@@ -10,8 +10,8 @@
 //
 // The queries of a kv head's group (tokens x query heads, `rows`) go to the matrix cores
 // together: up to 32 to rows_kernel, which memory bounds (a decode step's tokens: 4 to
-// 256 operations for each byte of the cache), more to prompt_kernel, which the matrix
-// cores bound.  In both keys are a product's rows and queries its columns, so that a lane
+// 256 operations for each byte of the cache), more to prompt_kernel, which matrix and
+// vector instructions bound.  In both keys are a product's rows and queries its columns, so that a lane
 // has scores of one query and its probabilities are already where the second product (V^T
 // P^T, queries as columns again) wants them, if that product's k index runs over a lane's
 // keys in turn.  V is read transposed from LDS (ds_read_b64_tr_b16, _tr_b8).  8-bit rows

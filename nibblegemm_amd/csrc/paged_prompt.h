@@ -32,14 +32,16 @@ __device__ __forceinline__ int prompt_swizzle(int r) {
 // and its probabilities are where the second product (V^T P^T) wants them, if its k runs
 // over a lane's keys in turn.
 //
-// The matrix cores bound it, and their power: of 2048 tokens of 32 + 2 x 8 heads of 128
-// the products alone would take 86 us at the rate of a large library product, and it takes
-// 113 to 130, by the card's clock, which falls to 1.9 GHz meanwhile.  What fills the time
-// between products was taken out: exponentials run beside the next scores' products, the
-// maximum beside the sums' products, addresses of 64 tiles are worked out at once.  Waves
-// whose rows are behind the last copy alone (64 rows over 32 x 4096 of 8 bits: 5 us of 58
-// less than if they compute, too; as much as by workgroups of two waves, which take 4 more
-// than these on 16 bits).
+// The SIMDs bound it, matrix and vector instructions together, and the clock that falls
+// under them: of 2048 tokens of 32 + 2 x 8 heads of 128 the products alone would take 86 us
+// at the rate of a large library product, and it takes 110 to 119.  By the counters the
+// matrix cores are busy 54% of the cycles (a ninth of that with the sums of the
+// probabilities) and other vector instructions issue in 39%, at 1.7 GHz: the two hardly
+// overlap, though two waves share a SIMD.  What fills the time between products was taken
+// out: exponentials run beside the next scores' products, the maximum beside the sums'
+// products, addresses of 64 tiles are worked out at once.  Waves whose rows are behind the
+// last copy alone (64 rows over 32 x 4096 of 8 bits: 5 us of 58 less than if they compute,
+// too; as much as by workgroups of two waves, which take 4 more than these on 16 bits).
 template <class E, int D, bool Q8>
 __global__ __launch_bounds__(kPagedThreads, 2) void prompt_kernel(AttendArgs a) {
   using T = typename E::type;

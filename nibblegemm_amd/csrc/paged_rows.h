@@ -122,6 +122,11 @@ __device__ __forceinline__ int rows_swizzle(int r) {
 // a kernel reaches that only reads.  Where there is little, what comes one behind the other
 // does: 4 us from the launch to the first rows (lengths, pages, rows), 4 to 5 from the
 // last piece to the output (sums, counter, sums), of 13 us for one token over 4000 rows.
+// 32 x one token over up to 8100 rows of 16 bits take 111 us (6.1 TB/s), of heads of 64 66
+// (5.1), in 8 bits 47 to 51 (3.3 to 3.6: the least data a unit, and its instructions are as
+// many); 32 x 6 tokens over 8000, two tiles of query rows, 140 us of 16 bits (4.8 TB/s) and
+// 83 of 8 (4.1).  That form, of heads of 128, spills 18 (8 bits: 4) vector registers, in what
+// it does once a sequence; all forms keep 84 to 141 scalars in lanes, which loops read back.
 // The copies go past the caches (nt), for a row is read once a call: 15% more of the rate.
 // 8 KB a wave are enough on their way; with 16 a step of 16 to 100 sequences takes 4 to 8%
 // longer.
